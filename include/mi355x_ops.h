@@ -487,6 +487,87 @@ mi_status_t mi_layer_norm_backward(const mi_tensor_t* grad_input,
                                    const mi_tensor_t* weight,
                                    int64_t normalized_numel, mi_stream_t stream);
 
+/* ---- 8-bit key/value cache ------------------------------------------------
+ * No counterpart in the reference.  A pool of pages holds e4m3 codes (one
+ * byte each) of the keys and values, with one float32 scale per page and k/v
+ * head: value = code * scale.  mi_kv8_append and mi_kv8_evict write powers of
+ * two, the smallest s >= 2^-110 with amax <= 448 s; reading takes any scale.
+ *
+ *   k, v              uint8   [pages, heads, page, head_dim]; head_dim 64 or
+ *                     128, page a power of two from 16 to 256; a page's head
+ *                     dense and 16-byte aligned, pages and heads at any
+ *                     non-overlapping strides
+ *   k_scale, v_scale  float32 [pages, heads]
+ *
+ * A call is about sequences b = 0 .. B - 1:
+ *   block_table  int32 [B, W]  the pages of each, in order of position
+ *   lengths      int32 [B]     tokens that the cache holds of each, the call's
+ *                              new ones among them
+ *   starts       int32 [B + 1] new tokens starts[b] .. starts[b + 1] - 1 of the
+ *                              packed tensors are sequence b's last ones: token
+ *                              i of n is at position lengths[b] - n + i
+ * All three are read on the device, when the kernels run.  Nothing out of
+ * bounds is touched whatever they hold: a length outside [0, W page] makes the
+ * sequence empty, a page outside the pool is not written and not seen, starts
+ * are clamped to the tokens; the first two are recorded for
+ * mi_index_fault_take.  Only entries for positions below lengths[b] are read. */
+typedef struct {
+  mi_tensor_t k;
+  mi_tensor_t v;
+  mi_tensor_t k_scale;
+  mi_tensor_t v_scale;
+} mi_kv8_cache_t;
+
+/* Writes k, v [tokens, heads, head_dim] (bf16 or f16) at their positions.  A
+ * page that holds earlier tokens of the sequence keeps its scale or, where a
+ * new token is too large for it, takes the larger one and its codes are
+ * rewritten; a page whose first position is written starts anew.  Slots past
+ * the sequence's end stay as they were.  A token with an infinite or NaN
+ * element makes NaN for every query that sees it, and for no other.  Each
+ * page written may belong to one sequence only; lengths[b] less than the new
+ * tokens is recorded as a fault and writes nothing. */
+mi_status_t mi_kv8_append(const mi_kv8_cache_t* cache, const mi_tensor_t* k,
+                          const mi_tensor_t* v, const mi_tensor_t* block_table,
+                          const mi_tensor_t* lengths, const mi_tensor_t* starts,
+                          mi_stream_t stream);
+
+/* out[t, h] = sum_j softmax_j(scale q[t, h] . k_j) v_j over positions j up to
+ * token t's own, k/v head h / (H / heads); lse [tokens, H] float32 the natural
+ * log of the softmax sums.  A token that sees nothing has out 0 and lse -inf.
+ * q and out bf16 or f16 [tokens, H, head_dim].  Rows of no sequence are left as
+ * they were, or with fill_rest set to 0 and -inf.  fp32 scores, sums and
+ * accumulation; softmax weights are rounded to q's type.  Partial sums of cut
+ * sequences take workspace. */
+mi_status_t mi_kv8_attention(const mi_tensor_t* out, const mi_tensor_t* lse,
+                             const mi_tensor_t* q, const mi_kv8_cache_t* cache,
+                             const mi_tensor_t* block_table,
+                             const mi_tensor_t* lengths, const mi_tensor_t* starts,
+                             double scale, int32_t fill_rest, mi_stream_t stream);
+
+/* weights[b, g, j] += sum over sequence b's new tokens t and the heads h of
+ * group g of exp(scale q[t, h] . k_j - lse[t, h]), j up to t's position: the
+ * weights that mi_kv8_attention (which gave lse) gave position j.  weights
+ * float32 [B, heads, >= W page]; positions from lengths[b] on stay as they
+ * were.  The order of the sums is fixed. */
+mi_status_t mi_kv8_weigh(const mi_tensor_t* weights, const mi_tensor_t* q,
+                         const mi_tensor_t* lse, const mi_kv8_cache_t* cache,
+                         const mi_tensor_t* block_table, const mi_tensor_t* lengths,
+                         const mi_tensor_t* starts, double scale, mi_stream_t stream);
+
+/* Keeps min(keep, lengths[b]) tokens per sequence and head: the first `sink`,
+ * the last `recent`, and the others of largest weight (ties: the lower
+ * position; NaN counts as no weight), in their order.  They are written to the
+ * pages of new_table (int32 [B, >= ceil(keep / page)]), which no block_table
+ * row of the call may name; the old pages stay as they were.  kept int32
+ * [B, heads, keep] the old positions, then -1; new_lengths int32 [B];
+ * new_weights like weights, the kept ones, then 0. */
+mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor_t* weights,
+                         const mi_tensor_t* block_table, const mi_tensor_t* new_table,
+                         const mi_tensor_t* lengths, int64_t keep, int64_t recent,
+                         int64_t sink, const mi_tensor_t* kept,
+                         const mi_tensor_t* new_lengths,
+                         const mi_tensor_t* new_weights, mi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

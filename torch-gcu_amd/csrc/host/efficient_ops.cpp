@@ -302,6 +302,20 @@ TORCH_LIBRARY(torch_gcu, m) {
   m.def("int8_linear(Tensor x, Tensor weight, Tensor scales, Tensor? bias=None) -> Tensor");
   m.def("linear_residual(Tensor x, Tensor weight, Tensor residual) -> Tensor");
   m.def("linear_silu_mul(Tensor x, Tensor w_gate, Tensor w_up) -> Tensor");
+  m.def(
+      "kv8_append(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+      "Tensor k, Tensor v, Tensor block_table, Tensor lengths, Tensor starts) -> ()");
+  m.def(
+      "kv8_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, "
+      "Tensor block_table, Tensor lengths, Tensor starts, float? scale=None) -> (Tensor, Tensor)");
+  m.def(
+      "kv8_weigh_(Tensor(a!) weights, Tensor q, Tensor lse, Tensor k_cache, Tensor v_cache, "
+      "Tensor k_scale, Tensor v_scale, Tensor block_table, Tensor lengths, Tensor starts, "
+      "float? scale=None) -> ()");
+  m.def(
+      "kv8_evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
+      "Tensor weights, Tensor block_table, Tensor new_table, Tensor lengths, int keep, int recent, "
+      "int sink=0) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(torch_gcu, PrivateUse1, m) {
@@ -313,4 +327,8 @@ TORCH_LIBRARY_IMPL(torch_gcu, PrivateUse1, m) {
   m.impl("int8_linear", TORCH_FN(torch_gcu::efficient::int8_linear));
   m.impl("linear_residual", TORCH_FN(torch_gcu::efficient::linear_residual));
   m.impl("linear_silu_mul", TORCH_FN(torch_gcu::efficient::linear_silu_mul));
+  m.impl("kv8_append", TORCH_FN(torch_gcu::efficient::kv8_append));
+  m.impl("kv8_attention", TORCH_FN(torch_gcu::efficient::kv8_attention));
+  m.impl("kv8_weigh_", TORCH_FN(torch_gcu::efficient::kv8_weigh_));
+  m.impl("kv8_evict", TORCH_FN(torch_gcu::efficient::kv8_evict));
 }

@@ -24,5 +24,26 @@ at::Tensor linear_residual(const at::Tensor& x, const at::Tensor& weight,
                            const at::Tensor& residual);
 at::Tensor linear_silu_mul(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up);
 
+// 8-bit key/value cache (kv8_ops.cpp)
+void kv8_append(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& k_scale, at::Tensor& v_scale,
+                const at::Tensor& k, const at::Tensor& v, const at::Tensor& block_table,
+                const at::Tensor& lengths, const at::Tensor& starts);
+std::tuple<at::Tensor, at::Tensor> kv8_attention(const at::Tensor& q, const at::Tensor& k_cache,
+                                                 const at::Tensor& v_cache,
+                                                 const at::Tensor& k_scale,
+                                                 const at::Tensor& v_scale,
+                                                 const at::Tensor& block_table,
+                                                 const at::Tensor& lengths,
+                                                 const at::Tensor& starts,
+                                                 std::optional<double> scale);
+void kv8_weigh_(at::Tensor& weights, const at::Tensor& q, const at::Tensor& lse,
+                const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale,
+                const at::Tensor& v_scale, const at::Tensor& block_table,
+                const at::Tensor& lengths, const at::Tensor& starts, std::optional<double> scale);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> kv8_evict(
+    at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& k_scale, at::Tensor& v_scale,
+    const at::Tensor& weights, const at::Tensor& block_table, const at::Tensor& new_table,
+    const at::Tensor& lengths, int64_t keep, int64_t recent, int64_t sink);
+
 }  // namespace efficient
 }  // namespace torch_gcu

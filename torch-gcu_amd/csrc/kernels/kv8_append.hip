@@ -1,0 +1,184 @@
+// Writes new tokens' keys and values into the pages of an 8-bit cache.
+//
+// A block (page and k/v head) has one power-of-two scale s, the smallest with
+// amax <= 448 s: e4m3 is a floating type, so a power of two loses nothing of
+// its precision, and when a larger token makes the scale of a page grow, the
+// codes that are there move by an exact shift of their exponents (but for
+// numbers that become subnormal).  Tokens written one by one so end up as
+// tokens written together.
+//
+// What bounds it: a prompt's bytes (16-bit tokens read, codes written), a
+// decode step's chain of dependent reads (starts, table, token, scale).  One
+// thread block per touched page and head owns that page's scale, so nothing
+// is shared between blocks.
+//
+// A token with an infinite or NaN element has NaN codes for its whole key, so
+// that every query that sees it gets NaN, and 0 in place of the bad elements
+// of its value: a bad value reaches the queries that see its token through
+// the score, and no other (0 x NaN in a masked place would).
+#include <algorithm>
+
+#include "kv8_common.h"
+
+namespace mi {
+namespace {
+
+struct Kv8New {
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_st, k_sh, v_st, v_sh;  // strides of a token and a head, in elements
+};
+
+template <typename T>
+__device__ __forceinline__ void widen8(const uint16_t* p, float* x) {
+  union {
+    u32x4 w;
+    uint16_t e[8];
+  } u;
+  u.w = *(const u32x4*)p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = Num<T>::load(u.e[i]);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
+  constexpr int CH = D / 8;  // 8-element pieces of a token's row
+  __shared__ int bad[256];   // tokens of the page with a non-finite element
+  __shared__ float most[2][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int cap = a.width << a.c.shift, shift = a.c.shift, size = 1 << shift;
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    kv8_report_lengths(a.lengths, a.seqs, cap, a.fault);
+    for (int b = threadIdx.x; b < a.seqs; b += blockDim.x) {
+      const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap);
+      if (!s.bad && s.n > s.len) record_index_fault(a.fault, s.len - s.n, cap);
+    }
+  }
+  int seq, nth;
+  const bool found = kv8_find(
+      a.seqs, blockIdx.x,
+      [&](int b) {
+        return kv8_touched(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), shift);
+      },
+      &seq, &nth);
+  if (!found) return;
+  const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, seq, a.tokens, cap);
+  const int old = s.len - s.n;  // position of the first new token
+  const int index = (old >> shift) + nth;
+  const int entry = a.table[seq * a.t_sb + index], page = kv8_page(entry, a.c.pages);
+  if (page < 0) {
+    if (threadIdx.x == 0) record_index_fault(a.fault, entry, a.c.pages);
+    return;
+  }
+  const int lo = max(old - (index << shift), 0), hi = min(s.len - (index << shift), size);
+  const int head = blockIdx.y;
+  const int64_t row0 = (int64_t)s.first + (index << shift) - old;  // token of slot 0
+  const uint16_t* src[2] = {x.k + row0 * x.k_st + head * x.k_sh, x.v + row0 * x.v_st + head * x.v_sh};
+  const int64_t st[2] = {x.k_st, x.v_st};
+  uint8_t* dst[2] = {(uint8_t*)a.c.k + page * a.c.k_sp + head * a.c.k_sh,
+                     (uint8_t*)a.c.v + page * a.c.v_sp + head * a.c.v_sh};
+  float* scales[2] = {(float*)a.c.k_scale + page * a.c.ks_sp + head * a.c.ks_sh,
+                      (float*)a.c.v_scale + page * a.c.vs_sp + head * a.c.vs_sh};
+
+  for (int i = threadIdx.x; i < size; i += 256) bad[i] = 0;
+  __syncthreads();
+  float am[2] = {0.f, 0.f};
+  for (int i = threadIdx.x + lo * CH; i < hi * CH; i += 256) {
+    const int slot = i / CH, c = i % CH;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float e[8];
+      widen8<T>(src[w] + slot * st[w] + 8 * c, e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (kv8_finite(e[j])) am[w] = fmaxf(am[w], fabsf(e[j]));
+        else bad[slot] = 1;  // every writer writes the same
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    am[w] = wave_fmax(am[w]);
+    if (lane == 0) most[w][wave] = am[w];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const float m = fmaxf(fmaxf(most[w][0], most[w][1]), fmaxf(most[w][2], most[w][3]));
+    const float before = *scales[w];
+    // a page starts anew with its first slot, whatever scale it had
+    float scale = kv8_scale_of(m);
+    if (lo > 0) scale = fmaxf(scale, before);
+    if (lo > 0 && scale != before) {
+      const float ratio = before / scale;
+      for (int i = threadIdx.x; i < lo * (D / 16); i += 256) {
+        u32x4* p = (u32x4*)dst[w] + i;
+        u32x4 v = *p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = f32x4_to_fp8(fp8x4_to_f32(v[j]) * ratio);
+        *p = v;
+      }
+    }
+    const float inv = 1.0f / scale;
+    for (int i = threadIdx.x + lo * CH; i < hi * CH; i += 256) {
+      const int slot = i / CH, c = i % CH;
+      float e[8];
+      widen8<T>(src[w] + slot * st[w] + 8 * c, e);
+      const bool nan = w == 0 && bad[slot] != 0;
+      f32x4 p[2];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = kv8_finite(e[j]) ? e[j] * inv : 0.f;
+        p[j >> 2][j & 3] = nan ? NAN : y;
+      }
+      *(u32x2*)(dst[w] + slot * D + 8 * c) = u32x2{f32x4_to_fp8(p[0]), f32x4_to_fp8(p[1])};
+    }
+    __syncthreads();  // every thread has read the scale
+    if (threadIdx.x == 0) *scales[w] = scale;
+  }
+}
+
+}  // namespace
+}  // namespace mi
+
+extern "C" mi_status_t mi_kv8_append(const mi_kv8_cache_t* cache, const mi_tensor_t* k,
+                                     const mi_tensor_t* v, const mi_tensor_t* block_table,
+                                     const mi_tensor_t* lengths, const mi_tensor_t* starts,
+                                     mi_stream_t stream) {
+  using namespace mi;
+  clear_error();
+  const char* op = "kv8_append";
+  Kv8Args a{};
+  int64_t dim = 0;
+  a.group = 1;
+  MI_RETURN_IF(kv8_check_cache(op, cache, &a.c, &dim));
+  MI_RETURN_IF(validate(k, "k"));
+  MI_RETURN_IF(validate(v, "v"));
+  for (const mi_tensor_t* t : {k, v}) {
+    MI_CHECK_ARG(t->ndim == 3 && t->sizes[1] == a.c.heads && t->sizes[2] == dim,
+                 "%s: k and v must be [tokens, heads, head_dim] of the cache's heads and head_dim",
+                 op);
+    MI_CHECK_ARG((t->dtype == MI_BF16 || t->dtype == MI_F16) && t->dtype == k->dtype,
+                 "%s: k and v must both be bfloat16 or float16", op);
+    MI_CHECK_ARG(t->sizes[0] == k->sizes[0], "%s: k and v have different numbers of tokens", op);
+    if (t->strides[2] != 1 || t->strides[0] % 8 != 0 || t->strides[1] % 8 != 0 ||
+        (uintptr_t)t->data % 16 != 0)
+      MI_FAIL(MI_ERR_UNSUPPORTED, "%s: rows of k and v must be dense and 16-byte aligned", op);
+  }
+  MI_RETURN_IF(kv8_check_seqs(op, block_table, lengths, starts, k->sizes[0], &a));
+  if (a.tokens == 0 || a.seqs == 0) return MI_OK;
+  a.fault = index_fault_word();
+  const Kv8New x{(const uint16_t*)k->data, (const uint16_t*)v->data, k->strides[0], k->strides[1],
+                 v->strides[0], v->strides[1]};
+  const dim3 grid((unsigned)kv8_touched_most(a.tokens, a.seqs, a.c.shift), (unsigned)a.c.heads);
+  hipStream_t s = (hipStream_t)stream;
+  if (k->dtype == MI_BF16 && dim == 128)
+    hipLaunchKernelGGL((kv8_append_kernel<BF16, 128>), grid, dim3(256), 0, s, a, x);
+  else if (k->dtype == MI_BF16)
+    hipLaunchKernelGGL((kv8_append_kernel<BF16, 64>), grid, dim3(256), 0, s, a, x);
+  else if (dim == 128)
+    hipLaunchKernelGGL((kv8_append_kernel<F16, 128>), grid, dim3(256), 0, s, a, x);
+  else
+    hipLaunchKernelGGL((kv8_append_kernel<F16, 64>), grid, dim3(256), 0, s, a, x);
+  return check_launch(op);
+}

@@ -1,0 +1,466 @@
+// Attention of a few query rows per sequence (decode steps, drafted tokens)
+// over the 8-bit cache: o = softmax(scale q k^T) v over the positions up to the
+// query's own, D = 64 or 128, bf16 / f16 queries.
+//
+// What bounds it: the codes are read once from HBM, one byte an element; the
+// G query heads of a k/v head times the sequence's new tokens share the read as
+// the rows of one MFMA tile (16 NB).
+//
+//   S^T = K Q^T   16 keys x 32 d (v_mfma_f32_16x16x32): lane (c, g) = (lane % 16,
+//                 lane / 16) loads 16 codes of key c at d = 64 h + 16 g: two
+//                 operands of 8, converted in registers (e4m3 is exact in both
+//                 16-bit types).  Which d an operand's place means is free as
+//                 long as Q's agree.
+//   O^T = V^T P^T accumulator (row c, keys 4 g + i) of two S^T tiles is the P^T
+//                 operand as it stands.  V^T needs 8 keys of one d per lane: the
+//                 lane loads D / 16 codes of each of its 8 keys, and the bytes
+//                 are turned around by v_perm before the conversion, so neither
+//                 K nor V passes through LDS.
+//
+// The scales multiply scores (K) and weights (V) in fp32: one scalar per 16
+// keys, since a page holds a multiple of 16.  P is rounded to the input type;
+// for f16 the weights are taken relative to the largest V scale met, or small
+// scales would push them under f16's range.
+//
+// Work: kv8_plan cuts each sequence's keys into parts so that all sequences
+// together make a few blocks per CU, whatever their lengths; the device reads
+// the lengths, so a captured call follows them.  A block's waves take 32-key
+// tiles in turn, never wait for each other, and are merged through LDS; parts
+// are merged by kv8_combine_kernel in a fixed order.
+#include <algorithm>
+
+#include "kv8_common.h"
+
+namespace mi {
+namespace {
+
+template <typename T>
+struct Mma16;
+template <>
+struct Mma16<BF16> {
+  static __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma16<F16> {
+  static __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+constexpr int RKT = 32;  // keys of a wave's tile
+
+template <int D>
+struct RowsTile {
+  u32x4 k[2][D / 64];       // [16-key half][64-d piece]
+  uint32_t v[8][D / 64];    // [key of the lane][4-d piece]
+  float ks[2], vs[2];
+  bool ok[2];               // the 16-key half lies in a page
+};
+
+template <typename T, int D, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv8_rows_kernel(Kv8Args a) {
+  typedef typename AttnOp<T>::vec vec;
+  constexpr bool F = std::is_same<T, F16>::value;
+  constexpr int RT = 16 * NB, KS = D / 32, DT = D / 16, W = D / 64;
+  __shared__ float red[NW * NB * DT * 4 * 64];
+  __shared__ float ml[NW][RT][3];
+
+  kv8_rest<D>(a);
+  Kv8Item it;
+  if (!kv8_item<RT, RKT>(a, blockIdx.x, &it)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int group = a.group, rows = it.cut.rows, row0 = it.tile * RT, len = it.s.len;
+
+  vec qf[NB][KS];
+  int lim[NB];
+  int64_t q_at[NB], o_at[NB], l_at[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = row0 + 16 * nb + c, rc = min(row, rows - 1);
+    const int64_t t = it.s.first + rc / group, h = it.head * group + rc % group;
+    lim[nb] = row < rows ? kv8_limit(it.s, rc / group) : 0;
+    q_at[nb] = t * a.q_st + h * a.q_sh;
+    o_at[nb] = t * a.o_st + h * a.o_sh;
+    l_at[nb] = t * a.lse_st + h * a.lse_sh;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      qf[nb][k] = *(const vec*)(a.q + q_at[nb] + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
+  }
+  // what the tile's first and last rows see
+  const int least = kv8_limit(it.s, row0 / group);
+  const int most = kv8_limit(it.s, (min(rows, row0 + RT) - 1) / group);
+  const int tiles = (most + RKT - 1) / RKT;
+  const int lo = (int)((int64_t)tiles * it.part / it.parts);
+  const int hi = (int)((int64_t)tiles * (it.part + 1) / it.parts);
+
+  const int shift = a.c.shift, in_page = (1 << shift) - 1;
+  const int* table = a.table + it.seq * a.t_sb;
+  const uint8_t* kc = a.c.k + it.head * a.c.k_sh + c * D + 16 * g;
+  const uint8_t* vc = a.c.v + it.head * a.c.v_sh + 4 * g * D + W * 4 * c;
+  const float* ksc = a.c.k_scale + it.head * a.c.ks_sh;
+  const float* vsc = a.c.v_scale + it.head * a.c.vs_sh;
+  auto entries = [&](int j, int* e) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      e[t] = ld_const(table + min((j * RKT + 16 * t) >> shift, a.width - 1));
+  };
+  auto load = [&](int j, const int* e, RowsTile<D>& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int pos = j * RKT + 16 * t;
+      const int p = kv8_page(e[t], a.c.pages);
+      x.ok[t] = pos < len && p >= 0;
+      if (pos < len && p < 0 && lane == 0) record_index_fault(a.fault, e[t], a.c.pages);
+      const int64_t page = max(p, 0);  // a page that is not there: page 0 is read, and nothing of it used
+      const int off = (pos & in_page) * D;
+      const uint8_t* kp = kc + page * a.c.k_sp + off;
+      const uint8_t* vp = vc + page * a.c.v_sp + off;
+#pragma unroll
+      for (int h = 0; h < W; ++h) x.k[t][h] = *(const u32x4*)(kp + 64 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (W == 2) {
+          const u32x2 y = *(const u32x2*)(vp + i * D);
+          x.v[4 * t + i][0] = y[0];
+          x.v[4 * t + i][1] = y[1];
+        } else {
+          x.v[4 * t + i][0] = *(const uint32_t*)(vp + i * D);
+        }
+      }
+      x.ks[t] = ld_const(ksc + page * a.c.ks_sp);
+      x.vs[t] = ld_const(vsc + page * a.c.vs_sp);
+    }
+  };
+
+  f32x4 o[NB][DT];
+  float m_run[NB], l_run[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    m_run[nb] = -INFINITY;
+    l_run[nb] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[nb][i] = f32x4{};
+  }
+  float vref = 0x1p-126f;  // f16: the largest V scale met; o holds sums over it
+
+  auto compute = [&](int j, RowsTile<D>& x) __attribute__((always_inline)) {
+    const bool edge = j * RKT + RKT > least || !x.ok[0] || !x.ok[1];
+    float vs[2] = {x.ok[0] ? x.vs[0] : 0.f, x.ok[1] ? x.vs[1] : 0.f};
+    if constexpr (F) {
+      const float top = fmaxf(vs[0], vs[1]);
+      if (top > vref) {
+        const float r = vref / top;
+        vref = top;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < DT; ++i) o[nb][i] *= r;
+      }
+      vs[0] /= vref;
+      vs[1] /= vref;
+    }
+    vec kf[2][KS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        kf[t][k] = fp8x8_to<T>(x.k[t][k >> 1][2 * (k & 1)], x.k[t][k >> 1][2 * (k & 1) + 1]);
+    vec pk[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      f32x8 s;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 acc = f32x4{};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) acc = Mma16<T>::mma(kf[t][k], qf[nb][k], acc);
+        const float sc = a.scale_log2 * x.ks[t];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i] * sc;
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = j * RKT + 16 * (i >> 2) + 4 * g + (i & 3);
+          s[i] = key < lim[nb] && x.ok[i >> 2] ? s[i] : -INFINITY;
+        }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                       fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      if (mx > m_run[nb]) {
+        const float corr = __builtin_amdgcn_exp2f(m_run[nb] - mx);
+        m_run[nb] = mx;
+        l_run[nb] *= corr;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[nb][i] *= corr;
+      }
+      const float m_use = m_run[nb] == -INFINITY ? 0.f : m_run[nb];
+      f32x8 p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(s[i] - m_use);
+        l_run[nb] += e;
+        p[i] = e * vs[i >> 2];
+      }
+      pk[nb] = __builtin_convertvector(p, vec);
+    }
+    if (j * RKT + RKT > len || !x.ok[0] || !x.ok[1]) {
+      // what lies behind the last token, or on a page that is not there, may
+      // hold anything, NaN codes too: 0 x NaN must not come in
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = j * RKT + 16 * (i >> 2) + 4 * g + (i & 3);
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          x.v[i][w] = key < len && x.ok[i >> 2] ? x.v[i][w] : 0u;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      union {
+        typename Fp8To<T>::pair p[4];
+        vec v;
+      } vf[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // bytes 0, 1 (then 2, 3) of keys 2 q and 2 q + 1, side by side
+        const uint32_t e0 = __builtin_amdgcn_perm(x.v[2 * q + 1][w], x.v[2 * q][w], 0x05010400u);
+        const uint32_t e1 = __builtin_amdgcn_perm(x.v[2 * q + 1][w], x.v[2 * q][w], 0x07030602u);
+        vf[0].p[q] = Fp8To<T>::template cvt<false>(e0);
+        vf[1].p[q] = Fp8To<T>::template cvt<true>(e0);
+        vf[2].p[q] = Fp8To<T>::template cvt<false>(e1);
+        vf[3].p[q] = Fp8To<T>::template cvt<true>(e1);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          o[nb][4 * w + e] = Mma16<T>::mma(vf[e].v, pk[nb], o[nb][4 * w + e]);
+    }
+  };
+
+  // this wave's tiles lo + wave, then every NW-th; the next one's codes are on
+  // their way while one is computed, its table entries one step before that
+  int j = lo + wave;
+  if (j < hi) {
+    RowsTile<D> x0, x1;
+    int e0[2], e1[2];
+    entries(j, e0);
+    entries(j + NW, e1);
+    load(j, e0, x0);
+    while (true) {
+      entries(j + 2 * NW, e0);
+      if (j + NW < hi) load(j + NW, e1, x1);
+      compute(j, x0);
+      j += NW;
+      if (j >= hi) break;
+      entries(j + 2 * NW, e1);
+      if (j + NW < hi) load(j + NW, e0, x0);
+      compute(j, x1);
+      j += NW;
+      if (j >= hi) break;
+    }
+  }
+
+  // merge the waves: common max, scaled sums, O added in wave order
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    float l = l_run[nb];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (g == 0) {
+      ml[wave][16 * nb + c][0] = m_run[nb];
+      ml[wave][16 * nb + c][1] = l;
+    }
+  }
+  __syncthreads();
+  float M[NB], l[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    M[nb] = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M[nb] = fmaxf(M[nb], ml[w][16 * nb + c][0]);
+    const float mu = M[nb] == -INFINITY ? 0.f : M[nb];
+    l[nb] = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+      l[nb] += ml[w][16 * nb + c][1] * __builtin_amdgcn_exp2f(ml[w][16 * nb + c][0] - mu);
+    float own = __builtin_amdgcn_exp2f(m_run[nb] - mu);
+    if constexpr (F) own *= vref;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        red[(((wave * NB + nb) * DT + i) * 4 + r) * 64 + lane] = o[nb][i][r] * own;
+  }
+  __syncthreads();
+  const bool whole = it.parts == 1;
+  const int64_t part0 = (int64_t)blockIdx.x * RT;
+  if (!whole && (int)blockIdx.x >= a.slots) return;
+  // run (nb, r, i4): the four d = D / 4 g + D / 16 r + 4 i4 .. + 3 of the lane's row
+  for (int run = wave; run < NB * DT; run += NW) {
+    const int nb = run / DT, r = run % DT / (DT / 4), i4 = run % (DT / 4);
+    f32x4 x = f32x4{};
+#pragma unroll
+    for (int w = 0; w < NW; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] += red[(((w * NB + nb) * DT + 4 * i4 + e) * 4 + r) * 64 + lane];
+    const int d = D / 4 * g + D / 16 * r + 4 * i4;
+    const int row = 16 * nb + c;
+    const float ln = nb == 0 ? l[0] : l[NB - 1];
+    if (row0 + row >= rows) continue;
+    if (whole) {
+      typedef typename AttnOp<T>::elem E;
+      typedef E e4 __attribute__((ext_vector_type(4)));
+      const float inv = ln == 0.f ? 0.f : 1.0f / ln;  // no visible key: 0
+      *(e4*)(a.o + (nb == 0 ? o_at[0] : o_at[NB - 1]) + d) = __builtin_convertvector(x * inv, e4);
+    } else {
+      *(f32x4*)(a.part_o + (part0 + row) * D + d) = x;
+    }
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int row = 16 * nb + c;
+    if (wave != nb % NW || g != 0 || row0 + row >= rows) continue;
+    if (whole) {
+      a.lse[l_at[nb]] = l[nb] == 0.f ? -INFINITY
+                                     : (M[nb] + __builtin_amdgcn_logf(l[nb])) * 0.6931471805599453f;
+    } else {
+      a.part_ml[(part0 + row) * 2] = M[nb];
+      a.part_ml[(part0 + row) * 2 + 1] = l[nb];
+    }
+  }
+}
+
+// A wave per output row of a sequence that was cut: its parts' partials merged
+// in a fixed order.
+template <typename T, int D, int RT, int KT>
+__global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
+  constexpr int E = D / 64;
+  typedef float fe __attribute__((ext_vector_type(E)));
+  const int lane = threadIdx.x & 63;
+  const int heads = a.c.heads * a.group;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (int64_t)a.tokens * heads) return;
+  const int t = (int)(id / heads), h = (int)(id % heads);
+  const int cap = a.width << a.c.shift;
+  // the sequence whose tokens hold t, and the items before it
+  const int chunk = kv8_plan<RT, KT>(a, cap);
+  int64_t before = 0;
+  int seq = -1;
+  for (int b0 = 0; b0 < a.seqs && seq < 0; b0 += 64) {
+    int n = 0;
+    bool mine = false;
+    if (b0 + lane < a.seqs) {
+      const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b0 + lane, a.tokens, cap);
+      const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
+      n = a.c.heads * c.row_tiles * c.parts(chunk);
+      mine = t >= s.first && t < s.first + s.n;
+    }
+    const uint64_t hit = __ballot(mine);
+    const int upto = wave_scan(n, lane);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      seq = b0 + l;
+      before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+    } else {
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  if (seq < 0) return;
+  const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, seq, a.tokens, cap);
+  const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
+  const int parts = c.parts(chunk);
+  if (parts == 1) return;
+  const int row = (t - s.first) * a.group + h % a.group;
+  const int64_t item = before + ((int64_t)(row / RT) * a.c.heads + h / a.group) * parts;
+  if (item + parts > a.slots) return;
+  const float* pm = a.part_ml + (item * RT + row % RT) * 2;
+  const float* po = a.part_o + (item * RT + row % RT) * D + lane * E;
+  float M = -INFINITY;
+  for (int p = lane; p < parts; p += 64) M = fmaxf(M, pm[(int64_t)p * RT * 2]);
+  M = wave_fmax(M);
+  const float mu = M == -INFINITY ? 0.f : M;
+  float l = 0.f;
+  for (int p = lane; p < parts; p += 64)
+    l += pm[(int64_t)p * RT * 2 + 1] * __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
+  l = wave_sum(l);
+  fe acc = {};
+  for (int p = 0; p < parts; ++p)
+    acc += *(const fe*)(po + (int64_t)p * RT * D) *
+           __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  typedef typename AttnOp<T>::elem Et;
+  typedef Et ee __attribute__((ext_vector_type(E)));
+  *(ee*)(a.o + t * a.o_st + h * a.o_sh + lane * E) = __builtin_convertvector(acc * inv, ee);
+  if (lane == 0)
+    a.lse[t * a.lse_st + h * a.lse_sh] =
+        l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+template <typename T, int D>
+mi_status_t run_rows(Kv8Args& a, hipStream_t s) {
+  constexpr int NB = 1, NW = 8, RT = 16 * NB;
+  // two blocks of eight waves per CU; a part is at least a tile per wave
+  a.target = 2 * cu_count();
+  a.least = NW;
+  const int64_t base = kv8_row_tiles_most(a.tokens, a.seqs, a.group, RT) * a.c.heads;
+  const int64_t key_tiles = ((int64_t)a.width << a.c.shift) / RKT + 1;
+  const bool cut = key_tiles > a.least;
+  a.slots = (int)std::max<int64_t>(base + (cut ? a.target : 0), 1);
+  Workspace ws;
+  if (cut) {
+    const size_t rows = (size_t)a.slots * RT;
+    MI_RETURN_IF(ws.alloc(rows * (D + 2) * sizeof(float), s));
+    a.part_o = (float*)ws.get();
+    a.part_ml = a.part_o + rows * D;
+  }
+  hipLaunchKernelGGL((kv8_rows_kernel<T, D, NB, NW>), dim3((unsigned)a.slots), dim3(64 * NW), 0, s, a);
+  MI_RETURN_IF(check_launch("kv8_attention"));
+  if (!cut) return MI_OK;
+  const int64_t rows = (int64_t)a.tokens * a.c.heads * a.group;
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D, RT, RKT>), dim3(ceil_div_u(rows, 4)), dim3(256), 0, s, a);
+  return check_launch("kv8_attention");
+}
+
+}  // namespace
+}  // namespace mi
+
+extern "C" mi_status_t mi_kv8_attention(const mi_tensor_t* out, const mi_tensor_t* lse,
+                                        const mi_tensor_t* q, const mi_kv8_cache_t* cache,
+                                        const mi_tensor_t* block_table, const mi_tensor_t* lengths,
+                                        const mi_tensor_t* starts, double scale, int32_t fill_rest,
+                                        mi_stream_t stream) {
+  using namespace mi;
+  clear_error();
+  const char* op = "kv8_attention";
+  Kv8Args a{};
+  int64_t dim = 0;
+  MI_RETURN_IF(kv8_check_cache(op, cache, &a.c, &dim));
+  MI_RETURN_IF(kv8_check_queries(op, q, lse, dim, &a));
+  MI_RETURN_IF(validate(out, "out"));
+  MI_CHECK_ARG(out->dtype == q->dtype && out->ndim == 3 && out->sizes[0] == q->sizes[0] &&
+                   out->sizes[1] == q->sizes[1] && out->sizes[2] == dim,
+               "%s: out must have q's shape and type", op);
+  if (out->strides[2] != 1 || out->strides[0] % 8 != 0 || out->strides[1] % 8 != 0 ||
+      (uintptr_t)out->data % 16 != 0)
+    MI_FAIL(MI_ERR_UNSUPPORTED, "%s: rows of out must be dense and 16-byte aligned", op);
+  MI_RETURN_IF(kv8_check_seqs(op, block_table, lengths, starts, q->sizes[0], &a));
+  MI_CHECK_ARG(std::isfinite(scale), "%s: scale is not finite", op);
+  if (a.tokens == 0) return MI_OK;
+  a.o = (uint16_t*)out->data;
+  a.o_st = out->strides[0];
+  a.o_sh = out->strides[1];
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.fill_rest = fill_rest;
+  a.fault = index_fault_word();
+  hipStream_t s = (hipStream_t)stream;
+  if (q->dtype == MI_BF16) return dim == 128 ? run_rows<BF16, 128>(a, s) : run_rows<BF16, 64>(a, s);
+  return dim == 128 ? run_rows<F16, 128>(a, s) : run_rows<F16, 64>(a, s);
+}

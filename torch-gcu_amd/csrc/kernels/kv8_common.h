@@ -1,0 +1,229 @@
+// Shared by the kernels of the 8-bit key/value cache: arguments, the cut of a
+// call over blocks, and conversions between e4m3 codes and wider types.
+#pragma once
+
+#include <cmath>
+
+#include "attention_common.h"
+#include "kv8_index.h"
+
+namespace mi {
+
+struct Kv8Cache {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_sp, k_sh, v_sp, v_sh;      // strides of a page and a head, in bytes
+  int64_t ks_sp, ks_sh, vs_sp, vs_sh;  // the scales', in elements
+  int pages, heads, shift;             // page size = 1 << shift
+};
+
+struct Kv8Args {
+  Kv8Cache c;
+  const int* table;
+  int64_t t_sb;     // table row stride
+  int width;        // table entries per sequence
+  const int* lengths;
+  const int* starts;
+  int seqs, tokens, group;
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  uint16_t* o;
+  int64_t o_st, o_sh;
+  float* lse;
+  int64_t lse_st, lse_sh;
+  float scale_log2;  // softmax scale * log2(e)
+  int fill_rest;     // rows of no sequence: zeros (0: left as they were)
+  int target, least, slots;  // parts aimed at, fewest key tiles of one, partials there is room for
+  float* part_o;     // [slots][rows of a tile][D], not normalised
+  float* part_ml;    // [slots][rows of a tile][2]: max (log2 units), sum
+  IndexFault* fault;
+};
+
+namespace {
+
+template <typename T>
+struct Fp8To;
+template <>
+struct Fp8To<BF16> {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  template <bool HI>
+  static __device__ __forceinline__ pair cvt(uint32_t v) {
+    return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, HI);
+  }
+};
+template <>
+struct Fp8To<F16> {
+  typedef _Float16 pair __attribute__((ext_vector_type(2)));
+  template <bool HI>
+  static __device__ __forceinline__ pair cvt(uint32_t v) {
+    return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, HI);
+  }
+};
+
+// Eight e4m3 codes as an MFMA operand of eight 16-bit numbers (exact: both
+// types hold every e4m3 number).
+template <typename T>
+__device__ __forceinline__ typename AttnOp<T>::vec fp8x8_to(uint32_t lo, uint32_t hi) {
+  union {
+    typename Fp8To<T>::pair p[4];
+    typename AttnOp<T>::vec v;
+  } u;
+  u.p[0] = Fp8To<T>::template cvt<false>(lo);
+  u.p[1] = Fp8To<T>::template cvt<true>(lo);
+  u.p[2] = Fp8To<T>::template cvt<false>(hi);
+  u.p[3] = Fp8To<T>::template cvt<true>(hi);
+  return u.v;
+}
+
+// Four codes to floats and back (to nearest, ties to even; the caller has
+// scaled to |x| <= 448, NaN becomes the NaN code).
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 fp8x4_to_f32(uint32_t v) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
+  const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+  return f32x4{a[0], a[1], b[0], b[1]};
+}
+__device__ __forceinline__ uint32_t f32x4_to_fp8(f32x4 x) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], r, true);
+}
+
+__device__ __forceinline__ bool kv8_finite(float x) {
+  return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+}
+
+__device__ __forceinline__ Kv8Seq kv8_load_seq(const int* starts, const int* lengths, int b,
+                                               int tokens, int cap) {
+  return kv8_seq(starts[b], starts[b + 1], lengths[b], tokens, cap);
+}
+
+// Wave-uniform reads of memory that the kernel does not write: through the
+// scalar cache's loads, whatever stores the compiler sees elsewhere.
+template <typename V>
+__device__ __forceinline__ V ld_const(const V* p) {
+  return *(const __attribute__((address_space(4))) V*)p;
+}
+
+template <typename V>
+__device__ __forceinline__ V wave_total(V v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(v, off, 64);
+    if (lane >= off) v += o;
+  }
+  return v;
+}
+
+// Finds, over the sequences' counts (count(b) of sequence b, summed in order),
+// the sequence that item `item` belongs to, and the item's place in it.  Every
+// lane gets the same answer; false if there are fewer items.  All lanes of the
+// wave take part.
+template <typename F>
+__device__ __forceinline__ bool kv8_find(int seqs, int64_t item, F count, int* seq, int* place) {
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0;
+  for (int b0 = 0; b0 < seqs; b0 += 64) {
+    const int mine = b0 + lane < seqs ? count(b0 + lane) : 0;
+    const int upto = wave_scan(mine, lane);
+    const uint64_t hit = __ballot(before + upto > item);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      *seq = b0 + l;
+      const int n = __builtin_amdgcn_readlane(mine, l);
+      *place = (int)(item - before) - (__builtin_amdgcn_readlane(upto, l) - n);
+      return *place >= 0 && *place < n;  // always, unless starts that overlap overflowed the sums
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// One block's share of a call over query rows and keys: row tile `tile` of k/v
+// head `head` of sequence `seq`, part `part` of its `parts` of keys.
+struct Kv8Item {
+  Kv8Seq s;
+  Kv8Cut cut;
+  int seq, head, tile, part, parts;
+};
+
+// Key tiles per part, from all sequences' work; the same in every wave.
+template <int RT, int KT>
+__device__ __forceinline__ int kv8_plan(const Kv8Args& a, int cap) {
+  const int lane = threadIdx.x & 63;
+  int64_t work = 0;
+  for (int b = lane; b < a.seqs; b += 64)
+    work += kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, RT, KT).work();
+  return kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least);
+}
+
+template <int RT, int KT>
+__device__ __forceinline__ bool kv8_item(const Kv8Args& a, int64_t item, Kv8Item* it) {
+  const int cap = a.width << a.c.shift;
+  const int chunk = kv8_plan<RT, KT>(a, cap);
+  int place;
+  const bool found = kv8_find(
+      a.seqs, item,
+      [&](int b) {
+        const Kv8Cut c =
+            kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, RT, KT);
+        return a.c.heads * c.row_tiles * c.parts(chunk);
+      },
+      &it->seq, &place);
+  if (!found) return false;
+  it->s = kv8_load_seq(a.starts, a.lengths, it->seq, a.tokens, cap);
+  it->cut = kv8_cut(it->s, a.group, RT, KT);
+  it->parts = it->cut.parts(chunk);
+  it->part = place % it->parts;
+  it->head = place / it->parts % a.c.heads;
+  it->tile = place / it->parts / a.c.heads;
+  return true;
+}
+
+// What no item covers: rows of no sequence, and sequences whose length is out
+// of range, which are reported (they count as empty).
+__device__ __forceinline__ void kv8_report_lengths(const int* lengths, int seqs, int cap,
+                                                   IndexFault* fault) {
+  for (int b = threadIdx.x; b < seqs; b += blockDim.x) {
+    const int n = lengths[b];
+    if (n < 0 || n > cap) record_index_fault(fault, n, (int64_t)cap + 1);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void kv8_rest(const Kv8Args& a) {
+  if (blockIdx.x == 0) kv8_report_lengths(a.lengths, a.seqs, a.width << a.c.shift, a.fault);
+  if (!a.fill_rest) return;
+  const int lo = kv8_clamp(a.starts[0], 0, a.tokens);
+  const int hi = kv8_clamp(a.starts[a.seqs], lo, a.tokens);
+  const int rest = a.tokens - (hi - lo), heads = a.c.heads * a.group;
+  for (int i = blockIdx.x; i < rest; i += gridDim.x) {
+    const int64_t t = i < lo ? i : i - lo + hi;
+    for (int x = threadIdx.x; x < heads * (D / 8); x += blockDim.x)
+      *(u32x4*)(a.o + t * a.o_st + (x / (D / 8)) * a.o_sh + x % (D / 8) * 8) = u32x4{};
+    for (int h = threadIdx.x; h < heads; h += blockDim.x)
+      a.lse[t * a.lse_st + h * a.lse_sh] = -INFINITY;
+  }
+}
+
+}  // namespace
+
+// Host side (kv8_cache.cpp): the cache's own checks, and the tensors that say
+// which sequences a call is about.
+mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cache* c, int64_t* dim);
+mi_status_t kv8_check_queries(const char* op, const mi_tensor_t* q, const mi_tensor_t* lse,
+                              int64_t dim, Kv8Args* a);
+mi_status_t kv8_check_seqs(const char* op, const mi_tensor_t* table, const mi_tensor_t* lengths,
+                           const mi_tensor_t* starts, int64_t tokens, Kv8Args* a);
+// float32 [sequences, heads, at least the table's positions], dense rows
+mi_status_t kv8_check_weights(const char* op, const mi_tensor_t* w, const char* name,
+                              const Kv8Args& a);
+
+}  // namespace mi

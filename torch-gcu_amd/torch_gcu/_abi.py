@@ -52,6 +52,10 @@ class MiAdamwHparams(ctypes.Structure):
                 ("amsgrad", ctypes.c_int32), ("maximize", ctypes.c_int32)]
 
 
+class MiKv8Cache(ctypes.Structure):
+    _fields_ = [("k", MiTensor), ("v", MiTensor), ("k_scale", MiTensor), ("v_scale", MiTensor)]
+
+
 class MiError(RuntimeError):
     """A kernel-library call returned a status other than MI_OK."""
 
@@ -121,6 +125,13 @@ _SIGNATURES = {
     "mi_linear_silu_mul": ([_T, _T, _T, _T, _S], ctypes.c_int),
     "mi_flash_attention_fwd": ([_T, _T, _T, _T, _T, ctypes.c_int32, ctypes.c_double, _S],
                                ctypes.c_int),
+    "mi_kv8_append": ([ctypes.POINTER(MiKv8Cache)] + [_T] * 5 + [_S], ctypes.c_int),
+    "mi_kv8_attention": ([_T] * 3 + [ctypes.POINTER(MiKv8Cache)] + [_T] * 3
+                         + [ctypes.c_double, ctypes.c_int32, _S], ctypes.c_int),
+    "mi_kv8_weigh": ([_T] * 3 + [ctypes.POINTER(MiKv8Cache)] + [_T] * 3 + [ctypes.c_double, _S],
+                     ctypes.c_int),
+    "mi_kv8_evict": ([ctypes.POINTER(MiKv8Cache)] + [_T] * 4 + [ctypes.c_int64] * 3 + [_T] * 3
+                     + [_S], ctypes.c_int),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -521,3 +532,43 @@ def flash_attention_fwd(out, lse, q, k, v, is_causal=True, scale=None):
           lib().mi_flash_attention_fwd(desc(out), desc(lse), desc(q), desc(k), desc(v),
                                        int(is_causal), float(scale), stream_of(out)))
     return out
+
+
+def _kv8_cache(cache):
+    return MiKv8Cache(*(desc(t) for t in cache))
+
+
+def kv8_append(k, v, cache, block_table, lengths, starts):
+    """cache: (k, v, k_scale, v_scale), as for the other kv8 calls."""
+    check("mi_kv8_append",
+          lib().mi_kv8_append(_kv8_cache(cache), desc(k), desc(v), desc(block_table), desc(lengths),
+                              desc(starts), stream_of(k)))
+
+
+def kv8_attention(out, lse, q, cache, block_table, lengths, starts, scale=None, fill_rest=False):
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    check("mi_kv8_attention",
+          lib().mi_kv8_attention(desc(out), desc(lse), desc(q), _kv8_cache(cache),
+                                 desc(block_table), desc(lengths), desc(starts), float(scale),
+                                 int(fill_rest), stream_of(out)))
+    return out, lse
+
+
+def kv8_weigh(weights, q, lse, cache, block_table, lengths, starts, scale=None):
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    check("mi_kv8_weigh",
+          lib().mi_kv8_weigh(desc(weights), desc(q), desc(lse), _kv8_cache(cache),
+                             desc(block_table), desc(lengths), desc(starts), float(scale),
+                             stream_of(weights)))
+    return weights
+
+
+def kv8_evict(cache, weights, block_table, new_table, lengths, keep, recent, sink, kept,
+              new_lengths, new_weights):
+    check("mi_kv8_evict",
+          lib().mi_kv8_evict(_kv8_cache(cache), desc(weights), desc(block_table), desc(new_table),
+                             desc(lengths), keep, recent, sink, desc(kept), desc(new_lengths),
+                             desc(new_weights), stream_of(weights)))
+    return kept, new_lengths, new_weights
