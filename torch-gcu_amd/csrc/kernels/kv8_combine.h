@@ -1,0 +1,102 @@
+// Merging of the partial results of an attention call over the 8-bit cache whose
+// sequences were cut along their keys.
+#pragma once
+
+#include "kv8_common.h"
+
+namespace mi {
+namespace {
+
+// A wave per output row of a sequence that was cut: its parts' partials merged
+// in a fixed order.
+template <typename T, int D, int RT, int KT, bool LAST_FIRST>
+__global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
+  constexpr int E = D / 64;
+  typedef float fe __attribute__((ext_vector_type(E)));
+  const int lane = threadIdx.x & 63;
+  const int heads = a.c.heads * a.group;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (int64_t)a.tokens * heads) return;
+  const int t = (int)(id / heads), h = (int)(id % heads);
+  const int cap = a.width << a.c.shift;
+  // the sequence whose tokens hold t, and the items before it
+  const int chunk = kv8_plan<RT, KT>(a, cap);
+  int64_t before = 0;
+  int seq = -1;
+  for (int b0 = 0; b0 < a.seqs && seq < 0; b0 += 64) {
+    int n = 0;
+    bool mine = false;
+    if (b0 + lane < a.seqs) {
+      const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b0 + lane, a.tokens, cap);
+      const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
+      n = a.c.heads * c.row_tiles * c.parts(chunk);
+      mine = t >= s.first && t < s.first + s.n;
+    }
+    const uint64_t hit = __ballot(mine);
+    const int upto = wave_scan(n, lane);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      seq = b0 + l;
+      before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+    } else {
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+  }
+  if (seq < 0) return;
+  const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, seq, a.tokens, cap);
+  const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
+  const int parts = c.parts(chunk);
+  if (parts == 1) return;
+  const int row = (t - s.first) * a.group + h % a.group;
+  const int tile = LAST_FIRST ? c.row_tiles - 1 - row / RT : row / RT;
+  const int64_t item = before + ((int64_t)tile * a.c.heads + h / a.group) * parts;
+  if (item + parts > a.slots) return;
+  const float* pm = a.part_ml + (item * RT + row % RT) * 2;
+  const float* po = a.part_o + (item * RT + row % RT) * D + lane * E;
+  float M = -INFINITY;
+  for (int p = lane; p < parts; p += 64) M = fmaxf(M, pm[(int64_t)p * RT * 2]);
+  M = wave_fmax(M);
+  const float mu = M == -INFINITY ? 0.f : M;
+  float l = 0.f;
+  for (int p = lane; p < parts; p += 64)
+    l += pm[(int64_t)p * RT * 2 + 1] * __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
+  l = wave_sum(l);
+  fe acc = {};
+  for (int p = 0; p < parts; ++p)
+    acc += *(const fe*)(po + (int64_t)p * RT * D) *
+           __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  typedef typename AttnOp<T>::elem Et;
+  typedef Et ee __attribute__((ext_vector_type(E)));
+  *(ee*)(a.o + t * a.o_st + h * a.o_sh + lane * E) = __builtin_convertvector(acc * inv, ee);
+  if (lane == 0)
+    a.lse[t * a.lse_st + h * a.lse_sh] =
+        l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+// Room for the partials of a call whose parts are planned with a.target and
+// a.least, then the attention kernel and, where anything can have been cut,
+// the merge.
+template <typename T, int D, int RT, int KT, bool LAST_FIRST, typename K>
+mi_status_t kv8_launch(Kv8Args& a, K kernel, int threads, hipStream_t s) {
+  const int64_t base = kv8_row_tiles_most(a.tokens, a.seqs, a.group, RT) * a.c.heads;
+  const bool cut = ((int64_t)a.width << a.c.shift) / KT + 1 > a.least;
+  a.slots = (int)std::max<int64_t>(base + (cut ? a.target : 0), 1);
+  Workspace ws;
+  if (cut) {
+    const size_t rows = (size_t)a.slots * RT;
+    MI_RETURN_IF(ws.alloc(rows * (D + 2) * sizeof(float), s));
+    a.part_o = (float*)ws.get();
+    a.part_ml = a.part_o + rows * D;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)a.slots), dim3(threads), 0, s, a);
+  MI_RETURN_IF(check_launch("kv8_attention"));
+  if (!cut) return MI_OK;
+  const int64_t rows = (int64_t)a.tokens * a.c.heads * a.group;
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D, RT, KT, LAST_FIRST>), dim3(ceil_div_u(rows, 4)),
+                     dim3(256), 0, s, a);
+  return check_launch("kv8_attention");
+}
+
+}  // namespace
+}  // namespace mi

@@ -2,7 +2,9 @@
 // call over blocks, and conversions between e4m3 codes and wider types.
 #pragma once
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attention_common.h"
 #include "kv8_index.h"
@@ -222,6 +224,8 @@ mi_status_t kv8_check_queries(const char* op, const mi_tensor_t* q, const mi_ten
                               int64_t dim, Kv8Args* a);
 mi_status_t kv8_check_seqs(const char* op, const mi_tensor_t* table, const mi_tensor_t* lengths,
                            const mi_tensor_t* starts, int64_t tokens, Kv8Args* a);
+// Attention of many query rows per sequence (kv8_prompt.hip).
+mi_status_t kv8_prompt(Kv8Args& a, int64_t dim, bool f16, hipStream_t s);
 // float32 [sequences, heads, at least the table's positions], dense rows
 mi_status_t kv8_check_weights(const char* op, const mi_tensor_t* w, const char* name,
                               const Kv8Args& a);

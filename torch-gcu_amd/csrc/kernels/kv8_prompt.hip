@@ -1,0 +1,289 @@
+// Attention of many query rows per sequence (pieces of prompts) over the 8-bit
+// cache.
+//
+// What bounds it: 4 D flops per query row and key on the matrix instructions,
+// and beside them about as much time of exp2, maxima and sums on the vector
+// unit.  A block takes 32 NW query rows of one k/v head (the group's heads of
+// consecutive tokens), a wave 32 of them, and walks the keys in tiles of 64:
+//   S^T = K Q^T, O^T = V^T P^T (v_mfma_f32_32x32x16), P^T taken from the S^T
+//   accumulators as they stand.
+// The codes of the next tile are loaded into registers while a tile is
+// computed, converted once per block (e4m3 is exact in both 16-bit types) and
+// written to the other of two LDS buffers: K by rows, V transposed, both in
+// 16-byte pieces whose places are XORed so that neither the writes nor the
+// fragment reads conflict.  One barrier a tile.
+// A key's scale multiplies its scores inside the exponent's FMA (one scalar per
+// 16 keys); a value's scale multiplies the weights, and only where it differs
+// from the largest one met so far, which the accumulators are relative to.
+#include <algorithm>
+
+#include "kv8_combine.h"
+
+namespace mi {
+namespace {
+
+constexpr int PKT = 64;  // keys per tile
+
+template <int D>
+__device__ __forceinline__ int swz_vt(int d) {
+  return ((d >> 1) & 7) ^ ((d >> 4) & 1);
+}
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
+  typedef typename AttnOp<T>::vec vec;
+  constexpr int RT = 32 * NW, NT = 64 * NW;
+  constexpr int KS = D / 16, DT = D / 32;
+  constexpr int VU = D / 4 * 8;              // V units: 4 d of 8 keys
+  constexpr int KU = PKT * D / 16;           // K units: 16 d of a key
+  constexpr int KN = NW == 8 ? KU / 256 : KU / NT;  // a thread's K units
+  __shared__ __align__(16) uint16_t kt[2][PKT * D];
+  __shared__ __align__(16) uint16_t vt[2][PKT * D];
+
+  kv8_rest<D>(a);
+  Kv8Item it;
+  if (!kv8_item<RT, PKT>(a, blockIdx.x, &it)) return;
+  it.tile = it.cut.row_tiles - 1 - it.tile;  // the longest rows first
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5, col = lane & 31;
+  const int group = a.group, rows = it.cut.rows, len = it.s.len;
+  const int row0 = it.tile * RT, wrow0 = row0 + 32 * wave;
+
+  const int row = wrow0 + col, rc = min(row, rows - 1);
+  const int64_t tok = it.s.first + rc / group, head = it.head * group + rc % group;
+  const int lim = row < rows ? kv8_limit(it.s, rc / group) : 0;
+  vec qf[KS];
+#pragma unroll
+  for (int t = 0; t < KS; ++t) {
+    qf[t] = *(const vec*)(a.q + tok * a.q_st + head * a.q_sh + 16 * t + 8 * half);
+    if (a.scale_log2 < 0.f) qf[t] = -qf[t];  // scales below are positive
+  }
+  const float scale = fabsf(a.scale_log2);
+  // positions that the block's rows see, and this wave's: all, and any
+  const int most = kv8_limit(it.s, (min(rows, row0 + RT) - 1) / group);
+  const int w_least = wrow0 < rows ? kv8_limit(it.s, wrow0 / group) : 0;
+  const int w_most = wrow0 < rows ? kv8_limit(it.s, (min(rows, wrow0 + 32) - 1) / group) : 0;
+  const int tiles = (most + PKT - 1) / PKT;
+  const int lo = (int)((int64_t)tiles * it.part / it.parts);
+  const int hi = (int)((int64_t)tiles * (it.part + 1) / it.parts);
+
+  const int shift = a.c.shift, in_page = (1 << shift) - 1;
+  const int* table = a.table + it.seq * a.t_sb;
+  const uint8_t* kc = a.c.k + it.head * a.c.k_sh;
+  const uint8_t* vc = a.c.v + it.head * a.c.v_sh;
+  const float* ksc = a.c.k_scale + it.head * a.c.ks_sh;
+  const float* vsc = a.c.v_scale + it.head * a.c.vs_sh;
+  auto entry_of = [&](int pos) __attribute__((always_inline)) {
+    return table[min(pos >> shift, a.width - 1)];
+  };
+
+  // this thread's units of a tile
+  const bool has_v = tid < VU, has_k = NW != 8 || tid >= 256;
+  const int ku = NW == 8 ? tid - 256 : tid;
+  const int v_dc = tid % (D / 4), v_kg = tid / (D / 4) & 7;
+  const int v_key = 16 * (v_kg >> 1) + 4 * (v_kg & 1);  // then + 1, 2, 3, 8, 9, 10, 11
+  u32x4 kr[KN];
+  uint32_t vr[8];
+  auto load = [&](int j) __attribute__((always_inline)) {
+    const int key0 = j * PKT;
+    if (has_k) {
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        const int u = ku + n * (NW == 8 ? 256 : NT);
+        const int pos = key0 + u / (D / 16);
+        const int64_t page = max(kv8_page(entry_of(pos), a.c.pages), 0);
+        kr[n] = *(const u32x4*)(kc + page * a.c.k_sp + (pos & in_page) * D + 16 * (u % (D / 16)));
+      }
+    }
+    if (has_v) {
+      const int pos = key0 + v_key;
+      const int p = kv8_page(entry_of(pos), a.c.pages);
+      const uint8_t* vp = vc + max(p, 0) * a.c.v_sp + (pos & in_page) * D + 4 * v_dc;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        vr[i] = *(const uint32_t*)(vp + (i < 4 ? i : i + 4) * D);
+        // behind the last token, or on a page that is not there, may lie
+        // anything, NaN codes too: 0 x NaN must not come in
+        if (p < 0 || pos + (i < 4 ? i : i + 4) >= len) vr[i] = 0;
+      }
+    }
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+    if (has_k) {
+#pragma unroll
+      for (int n = 0; n < KN; ++n) {
+        const int u = ku + n * (NW == 8 ? 256 : NT);
+        const int key = u / (D / 16), c = 2 * (u % (D / 16)), sw = swz_k_of<D>(key);
+        *(vec*)(kt[buf] + key * D + 8 * (c ^ sw)) = fp8x8_to<T>(kr[n][0], kr[n][1]);
+        *(vec*)(kt[buf] + key * D + 8 * ((c + 1) ^ sw)) = fp8x8_to<T>(kr[n][2], kr[n][3]);
+      }
+    }
+    if (has_v) {
+      union {
+        typename Fp8To<T>::pair p[4];
+        vec v;
+      } vf[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t e0 = __builtin_amdgcn_perm(vr[2 * q + 1], vr[2 * q], 0x05010400u);
+        const uint32_t e1 = __builtin_amdgcn_perm(vr[2 * q + 1], vr[2 * q], 0x07030602u);
+        vf[0].p[q] = Fp8To<T>::template cvt<false>(e0);
+        vf[1].p[q] = Fp8To<T>::template cvt<true>(e0);
+        vf[2].p[q] = Fp8To<T>::template cvt<false>(e1);
+        vf[3].p[q] = Fp8To<T>::template cvt<true>(e1);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 4 * v_dc + e;
+        *(vec*)(vt[buf] + d * PKT + 8 * (v_kg ^ swz_vt<D>(d))) = vf[e].v;
+      }
+    }
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) o[i] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  float vref = 0x1p-126f;  // the largest V scale met; o holds sums over it
+
+  if (lo < hi) {
+    load(lo);
+    store(0);
+  }
+  for (int j = lo; j < hi; ++j) {
+    const int buf = (j - lo) & 1, key0 = j * PKT;
+    __syncthreads();
+    if (j + 1 < hi) load(j + 1);
+    if (key0 < w_most) {
+      // scales of the tile's four 16-key groups
+      float sc[4], vs[4];
+      bool ok[4], all = true;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int pos = key0 + 16 * g;
+        const int e = ld_const(table + min(pos >> shift, a.width - 1));
+        const int p = kv8_page(e, a.c.pages);
+        ok[g] = pos < len && p >= 0;
+        all = all && ok[g];
+        if (pos < len && p < 0 && lane == 0) record_index_fault(a.fault, e, a.c.pages);
+        const int64_t page = max(p, 0);
+        const float k = scale * ld_const(ksc + page * a.c.ks_sp);
+        sc[g] = k < 0x1p-100f ? 0x1p-100f : k;  // masked scores stay -inf when multiplied by it
+        vs[g] = ok[g] ? ld_const(vsc + page * a.c.vs_sp) : 0.f;
+      }
+      f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const uint16_t* kp = kt[buf] + col * D + 8 * ((2 * t + half) ^ swz_k_of<D>(col));
+        s[0] = AttnOp<T>::mma(*(const vec*)kp, qf[t], s[0]);
+        s[1] = AttnOp<T>::mma(*(const vec*)(kp + 32 * D), qf[t], s[1]);
+      }
+      // accumulator r of half st is key 32 st + 8 (r / 4) + 4 half + r % 4, of
+      // the 16-key group 2 st + r / 8
+      if (key0 + PKT > w_least || !all) {
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = key0 + 32 * st + 8 * (r >> 2) + 4 * half + (r & 3);
+            s[st][r] = key < lim && ok[2 * st + (r >> 3)] ? s[st][r] : -INFINITY;
+          }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float x = s[g >> 1][8 * (g & 1)];
+#pragma unroll
+        for (int r = 1; r < 8; ++r) x = fmaxf(x, s[g >> 1][8 * (g & 1) + r]);
+        mx = fmaxf(mx, x * sc[g]);
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+      float corr = 1.f;
+      if (top > vref) {
+        corr = vref / top;
+        vref = top;
+      }
+      if (mx > m_run || corr != 1.f) {
+        const float grow = mx > m_run ? __builtin_amdgcn_exp2f(m_run - mx) : 1.f;
+        m_run = fmaxf(m_run, mx);
+        l_run *= grow;
+        corr *= grow;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][r] *= corr;
+      }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      const bool plain = vs[0] == vref && vs[1] == vref && vs[2] == vref && vs[3] == vref;
+      vec pk[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        f32x8 p;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + r], sc[g], -m_use));
+          l_run += p[r];
+        }
+        if (!plain) p *= vs[g] / vref;
+        pk[g] = __builtin_convertvector(p, vec);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const int d = 32 * i + col;
+          const vec vf = *(const vec*)(vt[buf] + d * PKT + 8 * ((2 * g + half) ^ swz_vt<D>(d)));
+          o[i] = AttnOp<T>::mma(vf, pk[g], o[i]);
+        }
+    }
+    if (j + 1 < hi) store(buf ^ 1);
+  }
+
+  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  if (row >= rows) return;
+  const bool whole = it.parts == 1;
+  if (!whole && (int)blockIdx.x >= a.slots) return;
+  const int64_t at = (int64_t)blockIdx.x * RT + 32 * wave + col;
+  const float f = whole ? (l == 0.f ? 0.f : vref / l) : vref;
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int d = 32 * i + 8 * q + 4 * half;
+      const f32x4 x = f32x4{o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]} * f;
+      if (whole) {
+        typedef typename AttnOp<T>::elem E;
+        typedef E e4 __attribute__((ext_vector_type(4)));
+        *(e4*)(a.o + tok * a.o_st + head * a.o_sh + d) = __builtin_convertvector(x, e4);
+      } else {
+        *(f32x4*)(a.part_o + at * D + d) = x;
+      }
+    }
+  if (half != 0) return;
+  if (whole) {
+    a.lse[tok * a.lse_st + head * a.lse_sh] =
+        l == 0.f ? -INFINITY : (m_run + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  } else {
+    a.part_ml[at * 2] = m_run;
+    a.part_ml[at * 2 + 1] = l;
+  }
+}
+
+template <typename T, int D>
+mi_status_t run_prompt(Kv8Args& a, hipStream_t s) {
+  constexpr int NW = 4;
+  a.target = 2 * cu_count();
+  a.least = 4;
+  return kv8_launch<T, D, 32 * NW, PKT, true>(a, kv8_prompt_kernel<T, D, NW>, 64 * NW, s);
+}
+
+}  // namespace
+
+mi_status_t kv8_prompt(Kv8Args& a, int64_t dim, bool f16, hipStream_t s) {
+  if (f16) return dim == 128 ? run_prompt<F16, 128>(a, s) : run_prompt<F16, 64>(a, s);
+  return dim == 128 ? run_prompt<BF16, 128>(a, s) : run_prompt<BF16, 64>(a, s);
+}
+
+}  // namespace mi
