@@ -85,6 +85,15 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
   const int v_key = 16 * (v_kg >> 1) + 4 * (v_kg & 1);  // then + 1, 2, 3, 8, 9, 10, 11
   u32x4 kr[KN];
   uint32_t vr[8];
+  int ke[KN], ve = 0;
+  auto entries = [&](int j) __attribute__((always_inline)) {
+    if (has_k) {
+#pragma unroll
+      for (int n = 0; n < KN; ++n)
+        ke[n] = entry_of(j * PKT + (ku + n * (NW == 8 ? 256 : NT)) / (D / 16));
+    }
+    if (has_v) ve = entry_of(j * PKT + v_key);
+  };
   auto load = [&](int j) __attribute__((always_inline)) {
     const int key0 = j * PKT;
     if (has_k) {
@@ -92,13 +101,13 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
       for (int n = 0; n < KN; ++n) {
         const int u = ku + n * (NW == 8 ? 256 : NT);
         const int pos = key0 + u / (D / 16);
-        const int64_t page = max(kv8_page(entry_of(pos), a.c.pages), 0);
+        const int64_t page = max(kv8_page(ke[n], a.c.pages), 0);
         kr[n] = *(const u32x4*)(kc + page * a.c.k_sp + (pos & in_page) * D + 16 * (u % (D / 16)));
       }
     }
     if (has_v) {
       const int pos = key0 + v_key;
-      const int p = kv8_page(entry_of(pos), a.c.pages);
+      const int p = kv8_page(ve, a.c.pages);
       const uint8_t* vp = vc + max(p, 0) * a.c.v_sp + (pos & in_page) * D + 4 * v_dc;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -147,14 +156,22 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
   float m_run = -INFINITY, l_run = 0.f;
   float vref = 0x1p-126f;  // the largest V scale met; o holds sums over it
 
+  // tile j's codes are loaded two steps before it is computed and converted one
+  // step before, their table entries a step earlier still
   if (lo < hi) {
+    entries(lo);
     load(lo);
+    entries(lo + 1);
     store(0);
+    load(lo + 1);
+    entries(lo + 2);
   }
   for (int j = lo; j < hi; ++j) {
     const int buf = (j - lo) & 1, key0 = j * PKT;
     __syncthreads();
-    if (j + 1 < hi) load(j + 1);
+    if (j + 1 < hi) store(buf ^ 1);
+    if (j + 2 < hi) load(j + 2);
+    entries(j + 3);
     if (key0 < w_most) {
       // scales of the tile's four 16-key groups
       float sc[4], vs[4];
@@ -216,6 +233,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
           for (int r = 0; r < 16; ++r) o[i][r] *= corr;
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      float ls[4] = {0.f, 0.f, 0.f, 0.f};
       const bool plain = vs[0] == vref && vs[1] == vref && vs[2] == vref && vs[3] == vref;
       vec pk[4];
 #pragma unroll
@@ -224,11 +242,12 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + r], sc[g], -m_use));
-          l_run += p[r];
+          ls[r & 3] += p[r];
         }
         if (!plain) p *= vs[g] / vref;
         pk[g] = __builtin_convertvector(p, vec);
       }
+      l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -238,7 +257,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
           o[i] = AttnOp<T>::mma(vf, pk[g], o[i]);
         }
     }
-    if (j + 1 < hi) store(buf ^ 1);
   }
 
   const float l = l_run + __shfl_xor(l_run, 32, 64);
