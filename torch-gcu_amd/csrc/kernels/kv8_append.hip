@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
       },
       &seq, &nth);
   if (!found) return;
-  const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, seq, a.tokens, cap);
+  const Kv8Seq s = kv8_block_seq(a, seq, cap);
   const int old = s.len - s.n;  // position of the first new token
   const int index = (old >> shift) + nth;
   const int entry = a.table[seq * a.t_sb + index], page = kv8_page(entry, a.c.pages);

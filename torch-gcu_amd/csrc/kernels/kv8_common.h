@@ -109,6 +109,10 @@ __device__ __forceinline__ V ld_const(const V* p) {
   return *(const __attribute__((address_space(4))) V*)p;
 }
 
+// A value that is the same in all lanes, told to the compiler: what is derived
+// from it stays in scalar registers, and branches on it are scalar.
+__device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 template <typename V>
 __device__ __forceinline__ V wave_total(V v) {
 #pragma unroll
@@ -138,9 +142,9 @@ __device__ __forceinline__ bool kv8_find(int seqs, int64_t item, F count, int* s
     const uint64_t hit = __ballot(before + upto > item);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
-      *seq = b0 + l;
+      *seq = wave_uniform(b0 + l);
       const int n = __builtin_amdgcn_readlane(mine, l);
-      *place = (int)(item - before) - (__builtin_amdgcn_readlane(upto, l) - n);
+      *place = wave_uniform((int)(item - before) - (__builtin_amdgcn_readlane(upto, l) - n));
       return *place >= 0 && *place < n;  // always, unless starts that overlap overflowed the sums
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -163,7 +167,16 @@ __device__ __forceinline__ int kv8_plan(const Kv8Args& a, int cap) {
   int64_t work = 0;
   for (int b = lane; b < a.seqs; b += 64)
     work += kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, RT, KT).work();
-  return kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least);
+  return wave_uniform(kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least));
+}
+
+// The sequence of a block, in scalar registers.
+__device__ __forceinline__ Kv8Seq kv8_block_seq(const Kv8Args& a, int b, int cap) {
+  Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap);
+  s.first = wave_uniform(s.first);
+  s.n = wave_uniform(s.n);
+  s.len = wave_uniform(s.len);
+  return s;
 }
 
 template <int RT, int KT>
@@ -180,7 +193,7 @@ __device__ __forceinline__ bool kv8_item(const Kv8Args& a, int64_t item, Kv8Item
       },
       &it->seq, &place);
   if (!found) return false;
-  it->s = kv8_load_seq(a.starts, a.lengths, it->seq, a.tokens, cap);
+  it->s = kv8_block_seq(a, it->seq, cap);
   it->cut = kv8_cut(it->s, a.group, RT, KT);
   it->parts = it->cut.parts(chunk);
   it->part = place % it->parts;

@@ -86,6 +86,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
   u32x4 kr[KN];
   uint32_t vr[8];
   int ke[KN], ve = 0;
+  int v_left = 0;  // of this thread's 8 keys those nearer than this exist
   auto entries = [&](int j) __attribute__((always_inline)) {
     if (has_k) {
 #pragma unroll
@@ -109,13 +110,9 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
       const int pos = key0 + v_key;
       const int p = kv8_page(ve, a.c.pages);
       const uint8_t* vp = vc + max(p, 0) * a.c.v_sp + (pos & in_page) * D + 4 * v_dc;
+      v_left = p < 0 ? 0 : len - pos;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        vr[i] = *(const uint32_t*)(vp + (i < 4 ? i : i + 4) * D);
-        // behind the last token, or on a page that is not there, may lie
-        // anything, NaN codes too: 0 x NaN must not come in
-        if (p < 0 || pos + (i < 4 ? i : i + 4) >= len) vr[i] = 0;
-      }
+      for (int i = 0; i < 8; ++i) vr[i] = *(const uint32_t*)(vp + (i < 4 ? i : i + 4) * D);
     }
   };
   auto store = [&](int buf) __attribute__((always_inline)) {
@@ -129,6 +126,12 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
       }
     }
     if (has_v) {
+      // behind the last token, or on a page that is not there, may lie
+      // anything, NaN codes too: 0 x NaN must not come in
+      if (v_left < 12) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) vr[i] = (i < 4 ? i : i + 4) < v_left ? vr[i] : 0u;
+      }
       union {
         typename Fp8To<T>::pair p[4];
         vec v;
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
       const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
       float corr = 1.f;
       if (top > vref) {
-        corr = vref / top;
+        corr = vref * __builtin_amdgcn_rcpf(top);
         vref = top;
       }
       if (mx > m_run || corr != 1.f) {
@@ -235,18 +238,22 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       float ls[4] = {0.f, 0.f, 0.f, 0.f};
       const bool plain = vs[0] == vref && vs[1] == vref && vs[2] == vref && vs[3] == vref;
-      vec pk[4];
+      f32x8 p[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        f32x8 p;
+      for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + r], sc[g], -m_use));
-          ls[r & 3] += p[r];
+          p[g][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + r], sc[g], -m_use));
+          ls[r & 3] += p[g][r];
         }
-        if (!plain) p *= vs[g] / vref;
-        pk[g] = __builtin_convertvector(p, vec);
+      if (!plain) {
+        const float inv = __builtin_amdgcn_rcpf(vref);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) p[g] *= vs[g] * inv;
       }
+      vec pk[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) pk[g] = __builtin_convertvector(p[g], vec);
       l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
       for (int g = 0; g < 4; ++g)

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(64 * WNW, 2) void kv8_weigh_kernel(Kv8Args a, Kv8We
         kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, WRT, WKT);
     work += c.work();
   }
-  const int chunk = kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least);
+  const int chunk = wave_uniform(kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least));
   int seq, place;
   const bool found = kv8_find(
       a.seqs, blockIdx.x,
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(64 * WNW, 2) void kv8_weigh_kernel(Kv8Args a, Kv8We
       },
       &seq, &place);
   if (!found) return;
-  const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, seq, a.tokens, cap);
+  const Kv8Seq s = kv8_block_seq(a, seq, cap);
   const int parts = weigh_parts(s, a.group, chunk), part = place % parts, head = place / parts;
   const Kv8Cut cut = kv8_cut(s, a.group, WRT, WKT);
   const int lo = (int)((int64_t)cut.key_tiles * part / parts);
