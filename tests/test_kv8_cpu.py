@@ -218,7 +218,8 @@ int main() {
   for (int round = 0; round < 2000; ++round) {
     const int seqs = 1 + rand() % 200, heads = 1 + rand() % 16, group = 1 + rand() % 8;
     const int rt = rand() % 2 ? 16 : 128, kt = rt == 16 ? 32 : 64, target = 512;
-    long tokens = 0, work = 0, items = 0, touched = 0;
+    long tokens = 0, items = 0, touched = 0;
+    float work = 0;
     static Kv8Seq all[200];
     for (int b = 0; b < seqs; ++b) {
       const int m = rand() % 4 ? rand() % 3 : rand() % 500;

@@ -50,19 +50,15 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
   if (blockIdx.x == 0 && blockIdx.y == 0) {
     kv8_report_lengths(a.lengths, a.seqs, cap, a.fault);
     for (int b = threadIdx.x; b < a.seqs; b += blockDim.x) {
-      const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap);
+      const Kv8Seq s = kv8_seq(a.starts[b], a.starts[b + 1], a.lengths[b], a.tokens, cap);
       if (!s.bad && s.n > s.len) record_index_fault(a.fault, s.len - s.n, cap);
     }
   }
   int seq, nth;
-  const bool found = kv8_find(
-      a.seqs, blockIdx.x,
-      [&](int b) {
-        return kv8_touched(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), shift);
-      },
-      &seq, &nth);
+  Kv8Seq s;
+  const bool found = Kv8Lanes(a).find(
+      blockIdx.x, [&](const Kv8Seq& x) { return kv8_touched(x, shift); }, &seq, &s, &nth);
   if (!found) return;
-  const Kv8Seq s = kv8_block_seq(a, seq, cap);
   const int old = s.len - s.n;  // position of the first new token
   const int index = (old >> shift) + nth;
   const int entry = a.table[seq * a.t_sb + index], page = kv8_page(entry, a.c.pages);

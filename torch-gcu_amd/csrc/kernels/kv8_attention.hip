@@ -60,7 +60,7 @@ struct RowsTile {
 };
 
 template <typename T, int D, int NB, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void kv8_rows_kernel(Kv8Args a) {
+__global__ __launch_bounds__(64 * NW, 4) void kv8_rows_kernel(Kv8Args a) {
   typedef typename AttnOp<T>::vec vec;
   constexpr bool F = std::is_same<T, F16>::value;
   constexpr int RT = 16 * NB, KS = D / 32, DT = D / 16, W = D / 64;
@@ -244,26 +244,17 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_rows_kernel(Kv8Args a) {
     }
   };
 
-  // this wave's tiles lo + wave, then every NW-th; the next one's codes are on
-  // their way while one is computed, its table entries one step before that
+  // this wave's tiles lo + wave, then every NW-th, their table entries one step
+  // ahead; the other waves of the SIMD cover the loads
   int j = lo + wave;
   if (j < hi) {
-    RowsTile<D> x0, x1;
-    int e0[2], e1[2];
-    entries(j, e0);
-    entries(j + NW, e1);
-    load(j, e0, x0);
-    while (true) {
-      entries(j + 2 * NW, e0);
-      if (j + NW < hi) load(j + NW, e1, x1);
-      compute(j, x0);
-      j += NW;
-      if (j >= hi) break;
-      entries(j + 2 * NW, e1);
-      if (j + NW < hi) load(j + NW, e0, x0);
-      compute(j, x1);
-      j += NW;
-      if (j >= hi) break;
+    RowsTile<D> x;
+    int e[2];
+    entries(j, e);
+    for (; j < hi; j += NW) {
+      load(j, e, x);
+      entries(j + NW, e);
+      compute(j, x);
     }
   }
 

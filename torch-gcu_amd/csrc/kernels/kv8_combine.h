@@ -8,70 +8,85 @@ namespace mi {
 namespace {
 
 // A wave per output row of a sequence that was cut: its parts' partials merged
-// in a fixed order.
+// in a fixed order, eight loads in flight.  Calls in which nothing was cut end
+// with the plan.
 template <typename T, int D, int RT, int KT, bool LAST_FIRST>
 __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
-  constexpr int E = D / 64;
+  constexpr int E = D / 64, U = 8;
   typedef float fe __attribute__((ext_vector_type(E)));
-  const int lane = threadIdx.x & 63;
   const int heads = a.c.heads * a.group;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= (int64_t)a.tokens * heads) return;
-  const int t = (int)(id / heads), h = (int)(id % heads);
-  const int cap = a.width << a.c.shift;
-  // the sequence whose tokens hold t, and the items before it
-  const int chunk = kv8_plan<RT, KT>(a, cap);
-  int64_t before = 0;
-  int seq = -1;
-  for (int b0 = 0; b0 < a.seqs && seq < 0; b0 += 64) {
-    int n = 0;
-    bool mine = false;
-    if (b0 + lane < a.seqs) {
-      const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b0 + lane, a.tokens, cap);
-      const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
-      n = a.c.heads * c.row_tiles * c.parts(chunk);
-      mine = t >= s.first && t < s.first + s.n;
-    }
-    const uint64_t hit = __ballot(mine);
-    const int upto = wave_scan(n, lane);
-    if (hit != 0) {
-      const int l = __builtin_ctzll(hit);
-      seq = b0 + l;
-      before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
-    } else {
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
+  const Kv8Lanes lanes(a);
+  const int lane = lanes.lane;
+  bool some = false;
+  const int chunk =
+      lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, RT, KT).work(); });
+  for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+    const Kv8Seq s = lanes.at(b0);
+    some = some || __ballot(s.n > 0 && kv8_cut(s, a.group, RT, KT).parts(chunk) > 1) != 0;
   }
-  if (seq < 0) return;
-  const Kv8Seq s = kv8_load_seq(a.starts, a.lengths, seq, a.tokens, cap);
-  const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
-  const int parts = c.parts(chunk);
-  if (parts == 1) return;
-  const int row = (t - s.first) * a.group + h % a.group;
-  const int tile = LAST_FIRST ? c.row_tiles - 1 - row / RT : row / RT;
-  const int64_t item = before + ((int64_t)tile * a.c.heads + h / a.group) * parts;
-  if (item + parts > a.slots) return;
-  const float* pm = a.part_ml + (item * RT + row % RT) * 2;
-  const float* po = a.part_o + (item * RT + row % RT) * D + lane * E;
-  float M = -INFINITY;
-  for (int p = lane; p < parts; p += 64) M = fmaxf(M, pm[(int64_t)p * RT * 2]);
-  M = wave_fmax(M);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float l = 0.f;
-  for (int p = lane; p < parts; p += 64)
-    l += pm[(int64_t)p * RT * 2 + 1] * __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
-  l = wave_sum(l);
-  fe acc = {};
-  for (int p = 0; p < parts; ++p)
-    acc += *(const fe*)(po + (int64_t)p * RT * D) *
-           __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  typedef typename AttnOp<T>::elem Et;
-  typedef Et ee __attribute__((ext_vector_type(E)));
-  *(ee*)(a.o + t * a.o_st + h * a.o_sh + lane * E) = __builtin_convertvector(acc * inv, ee);
-  if (lane == 0)
-    a.lse[t * a.lse_st + h * a.lse_sh] =
-        l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  if (!some) return;
+  const int64_t all = (int64_t)a.tokens * heads;
+  for (int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); id < all;
+       id += (int64_t)gridDim.x * 4) {
+    const int t = wave_uniform((int)(id / heads)), h = wave_uniform((int)(id % heads));
+    // the sequence that token t is of, and the items before it
+    int64_t before = 0;
+    bool found = false;
+    Kv8Seq s{};
+    for (int b0 = 0; b0 < a.seqs && !found; b0 += 64) {
+      const Kv8Seq mine = lanes.at(b0);
+      const Kv8Cut c = kv8_cut(mine, a.group, RT, KT);
+      const int n = a.c.heads * c.row_tiles * c.parts(chunk), upto = wave_scan(n);
+      const uint64_t hit = __ballot(t >= mine.first && t < mine.first + mine.n);
+      if (hit != 0) {
+        const int l = __builtin_ctzll(hit);
+        found = true;
+        s = Kv8Lanes::pick(mine, l);
+        before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
+      } else {
+        before += __builtin_amdgcn_readlane(upto, 63);
+      }
+    }
+    if (!found) continue;
+    const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
+    const int parts = c.parts(chunk);
+    if (parts == 1) continue;
+    const int row = (t - s.first) * a.group + h % a.group;
+    const int tile = LAST_FIRST ? c.row_tiles - 1 - row / RT : row / RT;
+    const int64_t item = before + ((int64_t)tile * a.c.heads + h / a.group) * parts;
+    if (item < 0 || item + parts > a.slots) continue;
+    const float* pm = a.part_ml + (item * RT + row % RT) * 2;
+    const float* po = a.part_o + (item * RT + row % RT) * D + lane * E;
+    float M = -INFINITY;
+    for (int p = lane; p < parts; p += 64) M = fmaxf(M, pm[(int64_t)p * RT * 2]);
+    M = wave_fmax(M);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    for (int p = lane; p < parts; p += 64)
+      l += pm[(int64_t)p * RT * 2 + 1] * __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
+    l = wave_sum(l);
+    fe acc = {};
+    for (int p0 = 0; p0 < parts; p0 += U) {
+      fe v[U];
+      float w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t p = min(p0 + u, parts - 1);
+        v[u] = *(const fe*)(po + p * RT * D);
+        w[u] = pm[p * RT * 2];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p0 + u < parts) acc += v[u] * __builtin_amdgcn_exp2f(w[u] - mu);
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    typedef typename AttnOp<T>::elem Et;
+    typedef Et ee __attribute__((ext_vector_type(E)));
+    *(ee*)(a.o + t * a.o_st + h * a.o_sh + lane * E) = __builtin_convertvector(acc * inv, ee);
+    if (lane == 0)
+      a.lse[t * a.lse_st + h * a.lse_sh] =
+          l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  }
 }
 
 // Room for the partials of a call whose parts are planned with a.target and
@@ -93,8 +108,8 @@ mi_status_t kv8_launch(Kv8Args& a, K kernel, int threads, hipStream_t s) {
   MI_RETURN_IF(check_launch("kv8_attention"));
   if (!cut) return MI_OK;
   const int64_t rows = (int64_t)a.tokens * a.c.heads * a.group;
-  hipLaunchKernelGGL((kv8_combine_kernel<T, D, RT, KT, LAST_FIRST>), dim3(ceil_div_u(rows, 4)),
-                     dim3(256), 0, s, a);
+  const unsigned grid = (unsigned)std::min<int64_t>((rows + 3) / 4, 8 * cu_count());
+  hipLaunchKernelGGL((kv8_combine_kernel<T, D, RT, KT, LAST_FIRST>), dim3(grid), dim3(256), 0, s, a);
   return check_launch("kv8_attention");
 }
 

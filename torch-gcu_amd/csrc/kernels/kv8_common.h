@@ -97,11 +97,6 @@ __device__ __forceinline__ bool kv8_finite(float x) {
   return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
 }
 
-__device__ __forceinline__ Kv8Seq kv8_load_seq(const int* starts, const int* lengths, int b,
-                                               int tokens, int cap) {
-  return kv8_seq(starts[b], starts[b + 1], lengths[b], tokens, cap);
-}
-
 // Wave-uniform reads of memory that the kernel does not write: through the
 // scalar cache's loads, whatever stores the compiler sees elsewhere.
 template <typename V>
@@ -113,44 +108,69 @@ __device__ __forceinline__ V ld_const(const V* p) {
 // from it stays in scalar registers, and branches on it are scalar.
 __device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-template <typename V>
-__device__ __forceinline__ V wave_total(V v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+// Inclusive sums over the lanes, by DPP within rows of 16 and two row broadcasts.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(v, off, 64);
-    if (lane >= off) v += o;
-  }
-  return v;
+__device__ __forceinline__ int wave_scan(int v) {
+  v = scan_step<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v = scan_step<0x112, 0xF>(v);
+  v = scan_step<0x114, 0xF>(v);
+  v = scan_step<0x118, 0xF>(v);
+  v = scan_step<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return scan_step<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-// Finds, over the sequences' counts (count(b) of sequence b, summed in order),
-// the sequence that item `item` belongs to, and the item's place in it.  Every
-// lane gets the same answer; false if there are fewer items.  All lanes of the
-// wave take part.
-template <typename F>
-__device__ __forceinline__ bool kv8_find(int seqs, int64_t item, F count, int* seq, int* place) {
-  const int lane = threadIdx.x & 63;
-  int64_t before = 0;
-  for (int b0 = 0; b0 < seqs; b0 += 64) {
-    const int mine = b0 + lane < seqs ? count(b0 + lane) : 0;
-    const int upto = wave_scan(mine, lane);
-    const uint64_t hit = __ballot(before + upto > item);
-    if (hit != 0) {
-      const int l = __builtin_ctzll(hit);
-      *seq = wave_uniform(b0 + l);
-      const int n = __builtin_amdgcn_readlane(mine, l);
-      *place = wave_uniform((int)(item - before) - (__builtin_amdgcn_readlane(upto, l) - n));
-      return *place >= 0 && *place < n;  // always, unless starts that overlap overflowed the sums
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
+// The call's sequences, a lane each, 64 at a time; the first 64 stay in
+// registers, so that a call of up to 64 reads its index tensors once.
+struct Kv8Lanes {
+  const Kv8Args& a;
+  int lane, cap;
+  Kv8Seq head;
+
+  __device__ __forceinline__ explicit Kv8Lanes(const Kv8Args& args)
+      : a(args), lane(threadIdx.x & 63), cap(args.width << args.c.shift) {
+    head = load(lane);
   }
-  return false;
-}
+  __device__ __forceinline__ Kv8Seq load(int b) const {
+    if (b >= a.seqs) return Kv8Seq{0, 0, 0, false};
+    return kv8_seq(a.starts[b], a.starts[b + 1], a.lengths[b], a.tokens, cap);
+  }
+  __device__ __forceinline__ Kv8Seq at(int b0) const { return b0 == 0 ? head : load(b0 + lane); }
+  static __device__ __forceinline__ Kv8Seq pick(const Kv8Seq& s, int l) {
+    return {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.n, l),
+            __builtin_amdgcn_readlane(s.len, l), __builtin_amdgcn_readlane((int)s.bad, l) != 0};
+  }
+  // Key tiles per part, from all sequences' work; the same in every wave.
+  template <typename F>
+  __device__ __forceinline__ int chunk(F work) const {
+    float sum = work(head);
+    for (int b0 = 64; b0 < a.seqs; b0 += 64) sum += work(load(b0 + lane));
+    return wave_uniform(kv8_chunk(wave_sum(sum) * a.c.heads, a.target, a.least));
+  }
+  // The sequence that item `item` belongs to, counted by count(s) per sequence
+  // in order, and its place in it; false if there are fewer items.  Every lane
+  // gets the same answer.
+  template <typename F>
+  __device__ __forceinline__ bool find(int item, F count, int* seq, Kv8Seq* s, int* place) const {
+    int64_t before = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+      const Kv8Seq mine = at(b0);
+      const int n = count(mine), upto = wave_scan(n);
+      const uint64_t hit = __ballot(before + upto > item);
+      if (hit != 0) {
+        const int l = __builtin_ctzll(hit), m = __builtin_amdgcn_readlane(n, l);
+        *seq = wave_uniform(b0 + l);
+        *s = pick(mine, l);
+        *place = wave_uniform((int)(item - before) - (__builtin_amdgcn_readlane(upto, l) - m));
+        return *place >= 0 && *place < m;  // always, unless starts that overlap overflowed the sums
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+  }
+};
 
 // One block's share of a call over query rows and keys: row tile `tile` of k/v
 // head `head` of sequence `seq`, part `part` of its `parts` of keys.
@@ -160,40 +180,20 @@ struct Kv8Item {
   int seq, head, tile, part, parts;
 };
 
-// Key tiles per part, from all sequences' work; the same in every wave.
 template <int RT, int KT>
-__device__ __forceinline__ int kv8_plan(const Kv8Args& a, int cap) {
-  const int lane = threadIdx.x & 63;
-  int64_t work = 0;
-  for (int b = lane; b < a.seqs; b += 64)
-    work += kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, RT, KT).work();
-  return wave_uniform(kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least));
-}
-
-// The sequence of a block, in scalar registers.
-__device__ __forceinline__ Kv8Seq kv8_block_seq(const Kv8Args& a, int b, int cap) {
-  Kv8Seq s = kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap);
-  s.first = wave_uniform(s.first);
-  s.n = wave_uniform(s.n);
-  s.len = wave_uniform(s.len);
-  return s;
-}
-
-template <int RT, int KT>
-__device__ __forceinline__ bool kv8_item(const Kv8Args& a, int64_t item, Kv8Item* it) {
-  const int cap = a.width << a.c.shift;
-  const int chunk = kv8_plan<RT, KT>(a, cap);
+__device__ __forceinline__ bool kv8_item(const Kv8Args& a, int item, Kv8Item* it) {
+  const Kv8Lanes lanes(a);
+  const int chunk =
+      lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, RT, KT).work(); });
   int place;
-  const bool found = kv8_find(
-      a.seqs, item,
-      [&](int b) {
-        const Kv8Cut c =
-            kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, RT, KT);
+  const bool found = lanes.find(
+      item,
+      [&](const Kv8Seq& s) {
+        const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
         return a.c.heads * c.row_tiles * c.parts(chunk);
       },
-      &it->seq, &place);
+      &it->seq, &it->s, &place);
   if (!found) return false;
-  it->s = kv8_block_seq(a, it->seq, cap);
   it->cut = kv8_cut(it->s, a.group, RT, KT);
   it->parts = it->cut.parts(chunk);
   it->part = place % it->parts;

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
         int h[4], sum = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum += h[k] = hist[255 - 4 * lane - k];
-        const int upto = wave_scan(sum, lane);
+        const int upto = wave_scan(sum);
         int above = upto - sum;
         const uint64_t hit = __ballot(upto >= ties);
         if (lane == __builtin_ctzll(hit)) {

@@ -54,7 +54,7 @@ struct Kv8Cut {
   int rows;       // n * group
   int row_tiles;
   int key_tiles;
-  MI_HD int64_t work() const { return (int64_t)row_tiles * (key_tiles > 0 ? key_tiles : 1); }
+  MI_HD float work() const { return (float)row_tiles * (float)key_tiles; }
   MI_HD int parts(int chunk) const { return key_tiles > chunk ? (key_tiles + chunk - 1) / chunk : 1; }
 };
 
@@ -67,10 +67,12 @@ MI_HD Kv8Cut kv8_cut(const Kv8Seq& s, int group, int rt, int kt) {
 }
 
 // Key tiles a part takes, so that `work` tiles (all sequences and k/v heads)
-// make about `target` parts; never under `least`.
-MI_HD int kv8_chunk(int64_t work, int target, int least) {
-  const int64_t c = (work + target - 1) / target;
-  return c < least ? least : c > 0x40000000 ? 0x40000000 : (int)c;
+// make at most `target` parts more than there are tiles of rows; never under
+// `least`.  work is a float sum, a few units of 2^-24 off, which the factor
+// makes up for.
+MI_HD int kv8_chunk(float work, int target, int least) {
+  const float c = work / (float)target * 1.00001f + 1.0f;
+  return c < (float)least ? least : c > 1073741824.f ? 1073741824 : (int)c;
 }
 
 // Row tiles that tokens x group rows in at most `seqs` sequences can make.

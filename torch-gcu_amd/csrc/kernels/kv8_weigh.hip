@@ -28,7 +28,7 @@ constexpr int WKT = 32, WRT = 32, WNW = 4;
 __device__ __forceinline__ int weigh_parts(const Kv8Seq& s, int group, int chunk) {
   const Kv8Cut c = kv8_cut(s, group, WRT, WKT);
   if (c.row_tiles == 0 || c.key_tiles == 0) return 0;
-  const int64_t parts = (c.work() + chunk - 1) / chunk;
+  const int64_t parts = ((int64_t)c.row_tiles * c.key_tiles + chunk - 1) / chunk;
   return (int)(parts < c.key_tiles ? parts : c.key_tiles);
 }
 
@@ -40,23 +40,15 @@ __global__ __launch_bounds__(64 * WNW, 2) void kv8_weigh_kernel(Kv8Args a, Kv8We
   const int half = lane >> 5, col = lane & 31;
   const int cap = a.width << a.c.shift;
   if (blockIdx.x == 0) kv8_report_lengths(a.lengths, a.seqs, cap, a.fault);
-  int64_t work = 0;
-  for (int b = lane; b < a.seqs; b += 64) {
-    const Kv8Cut c =
-        kv8_cut(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, WRT, WKT);
-    work += c.work();
-  }
-  const int chunk = wave_uniform(kv8_chunk(wave_total(work) * a.c.heads, a.target, a.least));
+  const Kv8Lanes lanes(a);
+  const int chunk =
+      lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, WRT, WKT).work(); });
   int seq, place;
-  const bool found = kv8_find(
-      a.seqs, blockIdx.x,
-      [&](int b) {
-        return a.c.heads *
-               weigh_parts(kv8_load_seq(a.starts, a.lengths, b, a.tokens, cap), a.group, chunk);
-      },
-      &seq, &place);
+  Kv8Seq s;
+  const bool found = lanes.find(
+      blockIdx.x, [&](const Kv8Seq& x) { return a.c.heads * weigh_parts(x, a.group, chunk); }, &seq,
+      &s, &place);
   if (!found) return;
-  const Kv8Seq s = kv8_block_seq(a, seq, cap);
   const int parts = weigh_parts(s, a.group, chunk), part = place % parts, head = place / parts;
   const Kv8Cut cut = kv8_cut(s, a.group, WRT, WKT);
   const int lo = (int)((int64_t)cut.key_tiles * part / parts);
