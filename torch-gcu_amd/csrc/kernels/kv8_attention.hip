@@ -34,21 +34,6 @@
 namespace mi {
 namespace {
 
-template <typename T>
-struct Mma16;
-template <>
-struct Mma16<BF16> {
-  static __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma16<F16> {
-  static __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-};
-
 constexpr int RKT = 32;  // keys of a wave's tile
 
 template <int D>

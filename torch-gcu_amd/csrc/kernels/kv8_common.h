@@ -45,6 +45,8 @@ struct Kv8Args {
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 template <typename T>
 struct Fp8To;
 template <>
@@ -79,10 +81,27 @@ __device__ __forceinline__ typename AttnOp<T>::vec fp8x8_to(uint32_t lo, uint32_
   return u.v;
 }
 
+// 16 x 16 tiles, 32 deep: lane l holds row (column) l % 16 at depth 8 (l / 16)
+// + 0 .. 7 of its operands, and rows 4 (l / 16) + 0 .. 3 of column l % 16 of the
+// result.
+template <typename T>
+struct Mma16;
+template <>
+struct Mma16<BF16> {
+  static __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma16<F16> {
+  static __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Four codes to floats and back (to nearest, ties to even; the caller has
 // scaled to |x| <= 448, NaN becomes the NaN code).
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 fp8x4_to_f32(uint32_t v) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false);
   const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);

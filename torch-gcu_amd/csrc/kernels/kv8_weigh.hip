@@ -6,10 +6,14 @@
 // no atomics, the same sums every time.
 //
 // What bounds it: a decode step reads the keys' codes once; a prompt's scores
-// are one matrix product.  A wave keeps 32 keys as MFMA operands and takes the
-// query rows 32 at a time (S^T = K Q^T, v_mfma_f32_32x32x16); a lane adds its 16
-// scores' weights over all rows of its column and the 32 columns are added at
-// the end.
+// are one matrix product with an exp2 for each.
+//   kv8_weigh_rows_kernel    few rows: a wave takes 32 keys and the rows 16 at a
+//     time (S^T = K Q^T, v_mfma_f32_16x16x32, the key layout of the decode
+//     attention), and adds the 16 columns by DPP.
+//   kv8_weigh_prompt_kernel  many rows: a wave keeps 32 keys as operands
+//     (32x32x16), the block's four waves share tiles of 64 rows in LDS, and a
+//     lane adds its 16 keys' weights over all rows of its column before the 32
+//     columns are added at the end.
 #include <algorithm>
 
 #include "kv8_common.h"
@@ -22,60 +26,191 @@ struct Kv8Weights {
   int64_t sb, sh;
 };
 
-constexpr int WKT = 32, WRT = 32, WNW = 4;
+constexpr int WKT = 32, WNW = 4;  // keys of a wave, waves of a block
 
-// Parts that a sequence's keys are cut into, by its work in 32 x 32 tiles.
-__device__ __forceinline__ int weigh_parts(const Kv8Seq& s, int group, int chunk) {
-  const Kv8Cut c = kv8_cut(s, group, WRT, WKT);
-  if (c.row_tiles == 0 || c.key_tiles == 0) return 0;
-  const int64_t parts = ((int64_t)c.row_tiles * c.key_tiles + chunk - 1) / chunk;
-  return (int)(parts < c.key_tiles ? parts : c.key_tiles);
-}
-
-template <typename T, int D>
-__global__ __launch_bounds__(64 * WNW, 2) void kv8_weigh_kernel(Kv8Args a, Kv8Weights wt) {
-  typedef typename AttnOp<T>::vec vec;
-  constexpr int P = D / 32;  // 16-byte pieces of a lane's half of a key
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = lane >> 5, col = lane & 31;
-  const int cap = a.width << a.c.shift;
-  if (blockIdx.x == 0) kv8_report_lengths(a.lengths, a.seqs, cap, a.fault);
-  const Kv8Lanes lanes(a);
-  const int chunk =
-      lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, WRT, WKT).work(); });
-  int seq, place;
+// The keys' tiles (of KT) of sequences with new tokens, weighed by their tiles of
+// RT rows, in parts; a part is a range of tiles of one k/v head.
+template <int RT, int KT>
+struct WeighItem {
   Kv8Seq s;
-  const bool found = lanes.find(
-      blockIdx.x, [&](const Kv8Seq& x) { return a.c.heads * weigh_parts(x, a.group, chunk); }, &seq,
-      &s, &place);
-  if (!found) return;
-  const int parts = weigh_parts(s, a.group, chunk), part = place % parts, head = place / parts;
-  const Kv8Cut cut = kv8_cut(s, a.group, WRT, WKT);
-  const int lo = (int)((int64_t)cut.key_tiles * part / parts);
-  const int hi = (int)((int64_t)cut.key_tiles * (part + 1) / parts);
-  const int group = a.group, in_page = (1 << a.c.shift) - 1;
-  const int* table = a.table + seq * a.t_sb;
-  float* out = wt.w + seq * wt.sb + head * wt.sh;
+  int seq, head, lo, hi, rows;
 
-  for (int j = lo + wave; j < hi; j += WNW) {
-    const int key0 = j * WKT;
-    // the lane's key: page, codes, scale of each 16 keys
-    bool ok[2];
-    float sc[2];
-    int64_t at[2];
+  static __device__ __forceinline__ int parts(const Kv8Seq& s, int group, int chunk) {
+    const Kv8Cut c = kv8_cut(s, group, RT, KT);
+    if (c.row_tiles == 0 || c.key_tiles == 0) return 0;
+    const int64_t parts = ((int64_t)c.row_tiles * c.key_tiles + chunk - 1) / chunk;
+    return (int)(parts < c.key_tiles ? parts : c.key_tiles);
+  }
+  __device__ __forceinline__ bool find(const Kv8Args& a) {
+    const Kv8Lanes lanes(a);
+    const int chunk =
+        lanes.chunk([&](const Kv8Seq& x) { return kv8_cut(x, a.group, RT, KT).work(); });
+    int place;
+    if (!lanes.find(
+            blockIdx.x, [&](const Kv8Seq& x) { return a.c.heads * parts(x, a.group, chunk); }, &seq,
+            &s, &place))
+      return false;
+    const Kv8Cut cut = kv8_cut(s, a.group, RT, KT);
+    const int n = parts(s, a.group, chunk), part = place % n;
+    head = place / n;
+    lo = (int)((int64_t)cut.key_tiles * part / n);
+    hi = (int)((int64_t)cut.key_tiles * (part + 1) / n);
+    rows = cut.rows;
+    return true;
+  }
+};
+
+// Pages of a wave's 32 keys from position key0 on: where the codes of each 16
+// lie, their scale times the softmax scale, and whether they exist.
+struct WeighKeys {
+  bool ok[2];
+  float sc[2];
+  int64_t at[2];
+
+  __device__ __forceinline__ WeighKeys(const Kv8Args& a, const Kv8Seq& s, int seq, int head,
+                                       int key0, int D) {
+    const int* table = a.table + seq * a.t_sb;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int pos = key0 + 16 * t;
       const int entry = ld_const(table + min(pos >> a.c.shift, a.width - 1));
       const int p = kv8_page(entry, a.c.pages);
       ok[t] = pos < s.len && p >= 0;
-      if (pos < s.len && p < 0 && lane == 0) record_index_fault(a.fault, entry, a.c.pages);
-      const int64_t page = max(p, 0);
-      at[t] = page * a.c.k_sp + (pos & in_page) * D;
+      if (pos < s.len && p < 0 && (threadIdx.x & 63) == 0)
+        record_index_fault(a.fault, entry, a.c.pages);
+      const int64_t page = max(p, 0);  // read instead, and nothing of it used
+      at[t] = page * a.c.k_sp + head * a.c.k_sh + (pos & ((1 << a.c.shift) - 1)) * D;
       sc[t] = a.scale_log2 * ld_const(a.c.k_scale + page * a.c.ks_sp + head * a.c.ks_sh);
     }
-    const uint8_t* kp =
-        a.c.k + head * a.c.k_sh + (col < 16 ? at[0] : at[1]) + (col & 15) * D + 16 * half;
+  }
+};
+
+// The first row of a group that sees a key: that of the token at its position.
+__device__ __forceinline__ int first_row(const Kv8Seq& s, int key, int group) {
+  return kv8_clamp(key - (s.len - s.n), 0, s.n) * group;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WNW, 4) void kv8_weigh_rows_kernel(Kv8Args a, Kv8Weights wt) {
+  typedef typename AttnOp<T>::vec vec;
+  constexpr int RT = 16, KS = D / 32;
+  if (blockIdx.x == 0)
+    kv8_report_lengths(a.lengths, a.seqs, a.width << a.c.shift, a.fault);
+  WeighItem<RT, WKT> it;
+  if (!it.find(a)) return;
+  const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4, group = a.group;
+  const Kv8Seq s = it.s;
+  const int past = s.len - s.n;
+  float* out = wt.w + it.seq * wt.sb + it.head * wt.sh;
+  vec qf[KS];
+  float lse = 0.f;
+  auto rows = [&](int r0) __attribute__((always_inline)) {
+    const int rc = min(r0 + c, it.rows - 1);
+    const int64_t t = s.first + rc / group, h = it.head * group + rc % group;
+    const uint16_t* q = a.q + t * a.q_st + h * a.q_sh + 16 * g;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qf[k] = *(const vec*)(q + 64 * (k >> 1) + 8 * (k & 1));
+    lse = a.lse[t * a.lse_st + h * a.lse_sh] * 1.4426950408889634f;
+  };
+  rows(0);
+  for (int j = it.lo + wave; j < it.hi; j += WNW) {
+    const int key0 = j * WKT;
+    const WeighKeys keys(a, s, it.seq, it.head, key0, D);
+    u32x4 x[2][D / 64];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int h = 0; h < D / 64; ++h)
+        x[t][h] = *(const u32x4*)(a.c.k + keys.at[t] + c * D + 16 * g + 64 * h);
+    // lane c = 4 t + i of each 16 will hold key 16 t + 4 g + i
+    const int mine = key0 + 16 * (c >> 2 & 1) + 4 * g + (c & 3);
+    const bool owner = c < 8 && mine < s.len && (c & 4 ? keys.ok[1] : keys.ok[0]);
+    const float before = owner ? out[mine] : 0.f;
+    vec kf[2][KS];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        kf[t][k] = fp8x8_to<T>(x[t][k >> 1][2 * (k & 1)], x[t][k >> 1][2 * (k & 1) + 1]);
+    float sum[8] = {};
+    // rows before these see none of the keys
+    for (int r0 = max(0, key0 - past) * group / RT * RT; r0 < it.rows; r0 += RT) {
+      if (it.rows > RT) rows(r0);
+      const int row = r0 + c;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 acc = f32x4{};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) acc = Mma16<T>::mma(kf[t][k], qf[k], acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 16 * t + 4 * g + i;
+          const bool sees = row < it.rows && row >= first_row(s, key, group);
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i], keys.sc[t], -lse));
+          sum[4 * t + i] += sees ? e : 0.f;
+        }
+      }
+    }
+    float got = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = sum[i];
+      v += dpp_f32<0xB1>(v);
+      v += dpp_f32<0x4E>(v);
+      v += dpp_f32<0x141>(v);
+      v += dpp_f32<0x140>(v);
+      got = c == i ? v : got;
+    }
+    if (owner) out[mine] = before + got;
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a, Kv8Weights wt) {
+  typedef typename AttnOp<T>::vec vec;
+  constexpr int RT = 64, KT = WKT * WNW, P = D / 32, CH = D / 8;
+  constexpr int N = RT * CH / (64 * WNW);  // 16-byte pieces of a row tile a thread stages
+  __shared__ __align__(16) uint16_t qs[2][RT * D];
+  __shared__ float ls[2][RT];
+  if (blockIdx.x == 0)
+    kv8_report_lengths(a.lengths, a.seqs, a.width << a.c.shift, a.fault);
+  WeighItem<RT, KT> it;
+  if (!it.find(a)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6);
+  const int half = lane >> 5, col = lane & 31, group = a.group;
+  const Kv8Seq s = it.s;
+  const int past = s.len - s.n;
+  float* out = wt.w + it.seq * wt.sb + it.head * wt.sh;
+  // what this thread stages of a row tile: piece tid % CH of rows tid / CH + ...
+  u32x4 qr[N];
+  float lr = 0.f;
+  auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int rc = min(r0 + tid / CH + n * (64 * WNW / CH), it.rows - 1);
+      const int64_t t = s.first + rc / group, h = it.head * group + rc % group;
+      qr[n] = *(const u32x4*)(a.q + t * a.q_st + h * a.q_sh + 8 * (tid % CH));
+    }
+    if (tid < RT) {
+      const int rc = min(r0 + tid, it.rows - 1);
+      const int64_t t = s.first + rc / group, h = it.head * group + rc % group;
+      lr = a.lse[t * a.lse_st + h * a.lse_sh] * 1.4426950408889634f;
+    }
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = tid / CH + n * (64 * WNW / CH);
+      *(u32x4*)(qs[buf] + r * D + 8 * (tid % CH ^ swz_k_of<D>(r & 31))) = qr[n];
+    }
+    if (tid < RT) ls[buf][tid] = lr;
+  };
+
+  for (int j = it.lo; j < it.hi; ++j) {
+    const int key0 = j * KT + wave * WKT;
+    const WeighKeys keys(a, s, it.seq, it.head, min(key0, s.len - 1), D);
+    const uint8_t* kp = a.c.k + (col < 16 ? keys.at[0] : keys.at[1]) + (col & 15) * D + 16 * half;
     vec kf[2 * P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -84,25 +219,47 @@ __global__ __launch_bounds__(64 * WNW, 2) void kv8_weigh_kernel(Kv8Args a, Kv8We
       kf[2 * p + 1] = fp8x8_to<T>(x[2], x[3]);
     }
     f32x16 sum = f32x16{};
-    // rows before this one see none of the keys
-    const int first = max(0, key0 - (s.len - s.n)) * group / WRT;
-    for (int r0 = first * WRT; r0 < cut.rows; r0 += WRT) {
-      const int row = r0 + col, rc = min(row, cut.rows - 1);
-      const int64_t t = s.first + rc / group, h = head * group + rc % group;
-      const int lim = row < cut.rows ? kv8_limit(s, rc / group) : 0;
-      const uint16_t* q = a.q + t * a.q_st + h * a.q_sh + 16 * half;
-      const float lse = a.lse[t * a.lse_st + h * a.lse_sh] * 1.4426950408889634f;
-      f32x16 x = f32x16{};
+    // rows before `first` see none of the block's keys, from `full` on all of
+    // the wave's
+    const int first = max(0, j * KT - past) * group / RT * RT;
+    const int full = first_row(s, key0 + WKT - 1, group);
+    __syncthreads();  // the buffers' last readers
+    load(first);
+    store(0);
+    if (first + RT < it.rows) load(first + RT);
+    int buf = 0;
+    for (int r0 = first; r0 < it.rows; r0 += RT, buf ^= 1) {
+      __syncthreads();
+      if (r0 + RT < it.rows) store(buf ^ 1);
+      if (r0 + 2 * RT < it.rows) load(r0 + 2 * RT);
+      if (key0 >= s.len) continue;
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        x = AttnOp<T>::mma(kf[2 * p], *(const vec*)(q + 32 * p), x);
-        x = AttnOp<T>::mma(kf[2 * p + 1], *(const vec*)(q + 32 * p + 8), x);
-      }
+      for (int u = 0; u < RT / 32; ++u) {
+        const uint16_t* q = qs[buf] + (32 * u + col) * D;
+        const float lse = ls[buf][32 * u + col];
+        f32x16 x = f32x16{};
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int key = key0 + 8 * (r >> 2) + 4 * half + (r & 3);
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], sc[r >> 3], -lse));
-        sum[r] += key < lim ? e : 0.f;
+        for (int p = 0; p < P; ++p) {
+          // d = 32 p + 16 half + 0 .. 15: pieces 4 p + 2 half and the next
+          const int ch = 4 * p + 2 * half, sw = swz_k_of<D>(col);
+          x = AttnOp<T>::mma(kf[2 * p], *(const vec*)(q + 8 * (ch ^ sw)), x);
+          x = AttnOp<T>::mma(kf[2 * p + 1], *(const vec*)(q + 8 * ((ch + 1) ^ sw)), x);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], keys.sc[r >> 3], -lse));
+        const int row = r0 + 32 * u;
+        if (row >= full && row + 32 <= it.rows) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum[r] += x[r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = key0 + 8 * (r >> 2) + 4 * half + (r & 3);
+            const bool sees = row + col < it.rows && row + col >= first_row(s, key, group);
+            sum[r] += sees ? x[r] : 0.f;
+          }
+        }
       }
     }
 #pragma unroll
@@ -114,9 +271,23 @@ __global__ __launch_bounds__(64 * WNW, 2) void kv8_weigh_kernel(Kv8Args a, Kv8We
       v += dpp_f32<0x140>(v);
       v += __shfl_xor(v, 16, 64);
       const int key = key0 + 8 * (r >> 2) + 4 * half + (r & 3);
-      if (col == r && key < s.len && ok[r >> 3]) out[key] += v;
+      if (col == r && key < s.len && keys.ok[r >> 3]) out[key] += v;
     }
   }
+}
+
+template <typename T, int D>
+mi_status_t run_weigh(Kv8Args& a, const Kv8Weights& w, hipStream_t s) {
+  a.least = 1;
+  const int some = std::min(a.seqs, a.tokens);
+  const dim3 block(64 * WNW);
+  // blocks of few rows: four a CU at once
+  const bool few = (int64_t)a.tokens * a.group <= (int64_t)32 * some;
+  a.target = 4 * cu_count();
+  const dim3 grid((unsigned)(a.target + some * a.c.heads));
+  if (few) hipLaunchKernelGGL((kv8_weigh_rows_kernel<T, D>), grid, block, 0, s, a, w);
+  else hipLaunchKernelGGL((kv8_weigh_prompt_kernel<T, D>), grid, block, 0, s, a, w);
+  return check_launch("kv8_weigh");
 }
 
 }  // namespace
@@ -139,19 +310,8 @@ extern "C" mi_status_t mi_kv8_weigh(const mi_tensor_t* weights, const mi_tensor_
   if (a.tokens == 0 || a.seqs == 0) return MI_OK;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.fault = index_fault_word();
-  a.target = 8 * cu_count();
-  a.least = 1;
   const Kv8Weights w{(float*)weights->data, weights->strides[0], weights->strides[1]};
-  const dim3 grid((unsigned)(a.target + (int64_t)std::min(a.seqs, a.tokens) * a.c.heads));
   hipStream_t s = (hipStream_t)stream;
-  const dim3 block(64 * WNW);
-  if (q->dtype == MI_BF16 && dim == 128)
-    hipLaunchKernelGGL((kv8_weigh_kernel<BF16, 128>), grid, block, 0, s, a, w);
-  else if (q->dtype == MI_BF16)
-    hipLaunchKernelGGL((kv8_weigh_kernel<BF16, 64>), grid, block, 0, s, a, w);
-  else if (dim == 128)
-    hipLaunchKernelGGL((kv8_weigh_kernel<F16, 128>), grid, block, 0, s, a, w);
-  else
-    hipLaunchKernelGGL((kv8_weigh_kernel<F16, 64>), grid, block, 0, s, a, w);
-  return check_launch(op);
+  if (q->dtype == MI_BF16) return dim == 128 ? run_weigh<BF16, 128>(a, w, s) : run_weigh<BF16, 64>(a, w, s);
+  return dim == 128 ? run_weigh<F16, 128>(a, w, s) : run_weigh<F16, 64>(a, w, s);
 }
