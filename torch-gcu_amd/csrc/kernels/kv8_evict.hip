@@ -5,7 +5,7 @@
 //
 // kv8_select_kernel, a block per sequence and head: the weight of rank r among
 // the candidates is found by a radix selection on order-preserving integers, 8
-// bits a pass; then one pass in order writes the kept positions and weights.
+// bits a pass; then one scan writes the kept positions and weights in order.
 // kv8_move_kernel, a block per new page and head: gathers the tokens' codes,
 // takes their largest magnitude, and writes them under the new page's scale.
 // Scales are powers of two, so codes move by an exact shift unless they become
@@ -33,22 +33,33 @@ struct Kv8Evict {
   int keep, recent, sink;
 };
 
-// Larger weight, larger integer; -0 as 0, NaN below everything.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Larger weight, larger integer; -0 as 0, NaN below every number but above 0,
+// which stands for positions that are no candidates.
 __device__ __forceinline__ uint32_t rank_of(float w) {
   const uint32_t u = __float_as_uint(w + 0.f);
-  if (w != w) return 0;
+  if (w != w) return 1;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int SELT = 1024;
+constexpr int SELT = 1024;      // threads, four positions each: a chunk
+constexpr int SELN = 16 * SELT;  // positions of a round: four chunks
 
+// Up to SELN positions the candidates' ranks are made once and stay in LDS,
+// longer sequences make them again in each pass.  What stays is counted per 256
+// positions (a wave's four a lane), and one scan of the counts, which every wave
+// makes for itself, places it.  Loops stay rolled: with few sequences the
+// kernel is a chain of latencies, and the fetch of unrolled code was the longest
+// of them (1 x 8 heads of 1000 positions: 16 us with the weights in registers,
+// 7.5 like this).
 __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e) {
-  __shared__ int hist[256];
-  __shared__ int pick[2];
-  __shared__ int sums[2][SELT / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) uint32_t ranks[SELN];
+  __shared__ __align__(16) int hist[4][256][4];  // [pass][bin][copy]: copies ease the adds to one bin
+  __shared__ int counts[64];  // sure + (ties << 16) of each 256 positions of a round
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6);
   const int head = blockIdx.x, b = blockIdx.y, cap = a.width << a.c.shift;
-  const int raw = a.lengths[b];
+  const int raw = ld_const(a.lengths + b);
   const int len = raw < 0 || raw > cap ? 0 : raw;
   if (len != raw && head == 0 && tid == 0) record_index_fault(a.fault, raw, (int64_t)cap + 1);
   const float* w = e.w + b * e.w_sb + head * e.w_sh;
@@ -60,75 +71,121 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
   const bool cut = len > e.keep;
   const int lo = cut ? e.sink : len, hi = cut ? len - e.recent : len;
   const int want = cut ? e.keep - e.sink - e.recent : 0;
+  const bool held = len <= SELN;
+  auto rank_at = [&](int i) __attribute__((always_inline)) {
+    return i >= lo && i < hi ? rank_of(w[i]) : 0u;
+  };
+  auto ranks_at = [&](int i) __attribute__((always_inline)) {
+    if (held) return *(const u32x4*)(ranks + i);
+    return u32x4{rank_at(i), rank_at(i + 1), rank_at(i + 2), rank_at(i + 3)};
+  };
+  if (held && want > 0) {
+    // all of a thread's loads in flight at once
+    float x[SELN / SELT];
+#pragma unroll
+    for (int k = 0; k < SELN / SELT; ++k) {
+      const int i = k * SELT + tid;
+      x[k] = w[min(i, len - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < SELN / SELT; ++k) {
+      const int i = k * SELT + tid;
+      if (k * SELT < len) ranks[i] = i >= lo && i < hi ? rank_of(x[k]) : 0u;
+    }
+  }
+  for (int i = tid; i < 4 * 256 * 4; i += SELT) (&hist[0][0][0])[i] = 0;
+  __syncthreads();
   uint32_t prefix = 0, mask = 0;
   int ties = want;  // how many of the candidates at the threshold stay
   if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += SELT) hist[i] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += SELT) {
-        const uint32_t u = rank_of(w[i]);
-        if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & 255], 1);
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+      const int shift = 24 - 8 * pass;
+#pragma unroll 1
+      for (int i = 4 * tid; i < len; i += 4 * SELT) {
+        const u32x4 u = ranks_at(i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if ((u[k] & mask) == prefix) atomicAdd(&hist[pass][(u[k] >> shift) & 255][lane & 3], 1);
       }
       __syncthreads();
-      if (wave == 0) {
-        // lane l: the four bins 255 - 4 l - 0 .. 3, from the largest down
-        int h[4], sum = 0;
+      // lane l: the four bins 252 - 4 l + 3 .. 0, from the largest down; every
+      // wave finds the bin of rank `ties` for itself (the zeros of positions
+      // that are no candidates lie behind all candidates)
+      int h[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum += h[k] = hist[255 - 4 * lane - k];
-        const int upto = wave_scan(sum);
-        int above = upto - sum;
-        const uint64_t hit = __ballot(upto >= ties);
-        if (lane == __builtin_ctzll(hit)) {
-          int k = 0;
-          while (above + h[k] < ties) above += h[k++];
-          pick[0] = 255 - 4 * lane - k;
-          pick[1] = ties - above;
+      for (int k = 0; k < 4; ++k) {
+        const i32x4 c = *(const i32x4*)hist[pass][252 - 4 * lane + k];
+        h[k] = c[0] + c[1] + c[2] + c[3];
+      }
+      const int sum = h[0] + h[1] + h[2] + h[3], upto = wave_scan(sum);
+      const int l = __builtin_ctzll(__ballot(upto >= ties));
+      int above = upto - sum, bin = 3;
+#pragma unroll
+      for (int k = 3; k > 0; --k) {
+        if (bin == k && above + h[k] < ties) {
+          above += h[k];
+          bin = k - 1;
         }
       }
-      __syncthreads();
-      prefix |= (uint32_t)pick[0] << shift;
+      prefix |= (uint32_t)__builtin_amdgcn_readlane(252 - 4 * lane + bin, l) << shift;
       mask |= 255u << shift;
-      ties = pick[1];
-      __syncthreads();
+      ties -= __builtin_amdgcn_readlane(above, l);
     }
   }
-  // in order: what stays, and the first `ties` of those at the threshold
+  // of positions i .. i + 3: bit k, it stays for sure; bit 4 + k, it is at the
+  // threshold, where the first `ties` stay
+  auto kinds = [&](int i) __attribute__((always_inline)) {
+    if (!cut) return i + 4 <= len ? 15 : i < len ? (1 << (len - i)) - 1 : 0;
+    const u32x4 u = want > 0 && i < len ? ranks_at(i) : u32x4{};
+    int r = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool forced = i + k < lo || (i + k >= hi && i + k < len);
+      r |= (forced || (u[k] > prefix && want > 0)) << k;
+      r |= (want > 0 && u[k] == prefix) << (4 + k);
+    }
+    return r;
+  };
+  auto packed = [](int x) __attribute__((always_inline)) {
+    return __popc(x & 15) | __popc(x >> 4) << 16;
+  };
   int done = 0, tied = 0;
-  for (int i0 = 0; i0 < len; i0 += SELT) {
-    const int i = i0 + tid;
-    const float x = i < len ? w[i] : 0.f;
-    const uint32_t u = rank_of(x);
-    const bool cand = i >= lo && i < hi;
-    const bool tie = cand && want > 0 && u == prefix;
-    const bool sure = i < len && (!cand || (want > 0 && u > prefix));
-    const uint64_t mt = __ballot(tie), ms = __ballot(sure);
-    if (lane == 0) {
-      sums[0][wave] = __popcll(mt);
-      sums[1][wave] = __popcll(ms);
+  for (int r0 = 0; r0 < len; r0 += SELN) {
+    const int chunks = min((len - r0 + 4 * SELT - 1) / (4 * SELT), 4);
+    if (tid < 64) counts[tid] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < chunks; ++k) {
+      const int scan = wave_scan(packed(kinds(r0 + 4 * (k * SELT + tid))));
+      if (lane == 63) counts[k * (SELT / 64) + wave] = scan;
     }
     __syncthreads();
-    int t0 = tied, tw = 0, s_all = 0, s0 = 0;
+    const int mine = counts[lane], upto = wave_scan(mine);
+    const int all = __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll 1
+    for (int k = 0; k < chunks; ++k) {
+      const int i = r0 + 4 * (k * SELT + tid), x = kinds(i), n = packed(x);
+      const int before =
+          __builtin_amdgcn_readlane(upto - mine, k * (SELT / 64) + wave) + wave_scan(n) - n;
+      // ties before this position, of which those under `ties` stay
+      int tie_at = tied + (int)((uint32_t)before >> 16);
+      int at = done + (before & 0xffff) + min(tie_at, ties) - min(tied, ties);
 #pragma unroll
-    for (int k = 0; k < SELT / 64; ++k) {
-      if (k < wave) {
-        tw += sums[0][k];
-        s0 += sums[1][k];
+      for (int q = 0; q < 4; ++q) {
+        const bool tie = x >> (4 + q) & 1;
+        if ((x >> q & 1) || (tie && tie_at < ties)) {
+          if (at < e.keep) {
+            kept[at] = i + q;
+            nw[at] = w[i + q];
+          }
+          ++at;
+        }
+        tie_at += tie;
       }
-      t0 += sums[0][k];
-      s_all += sums[1][k];
     }
-    const uint64_t under = ((uint64_t)1 << lane) - 1;
-    const int tie_at = tied + tw + __popcll(mt & under);
-    const bool stay = sure || (tie && tie_at < ties);
-    // ties that stay before this one: all of them until `ties` are there
-    const int at = done + s0 + __popcll(ms & under) + min(tie_at, ties) - min(tied, ties);
-    if (stay && at < e.keep) {
-      kept[at] = i;
-      nw[at] = x;
-    }
-    done += s_all + min(t0, ties) - min(tied, ties);
-    tied = t0;
+    done += (all & 0xffff) + min(tied + (int)((uint32_t)all >> 16), ties) - min(tied, ties);
+    tied += (int)((uint32_t)all >> 16);
     __syncthreads();
   }
   for (int i = left + tid; i < e.keep; i += SELT) kept[i] = -1;
