@@ -192,7 +192,9 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
   for (int i = left + tid; i < e.size; i += SELT) nw[i] = 0.f;
 }
 
-template <int D>
+// U 16-byte pieces of the page a thread, in registers between the maximum and
+// the rescaling.
+template <int D, int U>
 __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8Args a, Kv8Evict e) {
   constexpr int CH = D / 16;  // 16-code pieces of a row
   __shared__ float most[4];
@@ -213,43 +215,40 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8Args a, Kv8Evict e) {
   const int64_t sp = is_v ? a.c.v_sp : a.c.k_sp, ssp = is_v ? a.c.vs_sp : a.c.ks_sp;
   const int* kept = e.kept + b * e.k_sb + head * e.k_sh + (index << shift);
   const int* table = a.table + b * a.t_sb;
-  auto source = [&](int i, u32x4* v, float* scale) __attribute__((always_inline)) {
+  u32x4 v[U];
+  float sc[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = min(tid + 256 * u, n * CH - 1);
     const int pos = kv8_clamp(kept[i / CH], 0, cap - 1);
     const int from = table[pos >> shift], p = kv8_page(from, a.c.pages);
-    *v = u32x4{};
-    *scale = 0.f;
-    if (p >= 0) {
-      *v = *(const u32x4*)(codes + p * sp + (pos & (size - 1)) * D + 16 * (i % CH));
-      *scale = scales[p * ssp];
-    } else {
-      record_index_fault(a.fault, from, a.c.pages);
-    }
-  };
+    if (p < 0) record_index_fault(a.fault, from, a.c.pages);
+    const int64_t old = max(p, 0);
+    v[u] = *(const u32x4*)(codes + old * sp + (pos & (size - 1)) * D + 16 * (i % CH));
+    sc[u] = scales[old * ssp];
+    if (p < 0) v[u] = u32x4{};  // a page that is not there: zeros
+  }
   float am = 0.f;
-  for (int i = tid; i < n * CH; i += 256) {
-    u32x4 v;
-    float sc;
-    source(i, &v, &sc);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const f32x4 x = fp8x4_to_f32(v[w]) * sc;
+      const f32x4 x = fp8x4_to_f32(v[u][w]) * sc[u];
 #pragma unroll
       for (int k = 0; k < 4; ++k) am = kv8_finite(x[k]) ? fmaxf(am, fabsf(x[k])) : am;
     }
-  }
   am = wave_fmax(am);
   if (lane == 0) most[wave] = am;
   __syncthreads();
   const float scale = kv8_scale_of(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
   const float inv = 1.0f / scale;
   uint8_t* dst = (uint8_t*)codes + page * sp;
-  for (int i = tid; i < n * CH; i += 256) {
-    u32x4 v;
-    float sc;
-    source(i, &v, &sc);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v[w] = f32x4_to_fp8(fp8x4_to_f32(v[w]) * (sc * inv));
-    *(u32x4*)(dst + (i / CH) * D + 16 * (i % CH)) = v;
+  for (int u = 0; u < U; ++u) {
+    const int i = tid + 256 * u;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[u][w] = f32x4_to_fp8(fp8x4_to_f32(v[u][w]) * (sc[u] * inv));
+    if (i < n * CH) *(u32x4*)(dst + (i / CH) * D + 16 * (i % CH)) = v[u];
   }
   if (tid == 0) ((float*)scales)[page * ssp] = scale;
 }
@@ -322,7 +321,17 @@ extern "C" mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor
                      s, a, e);
   MI_RETURN_IF(check_launch(op));
   const dim3 grid((unsigned)pages, (unsigned)a.c.heads, 2u * (unsigned)a.seqs);
-  if (dim == 128) hipLaunchKernelGGL((kv8_move_kernel<128>), grid, dim3(256), 0, s, a, e);
-  else hipLaunchKernelGGL((kv8_move_kernel<64>), grid, dim3(256), 0, s, a, e);
+  auto move = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, e); };
+  const int64_t pieces = (dim / 16) << a.c.shift;
+  if (dim == 128) {
+    if (pieces <= 256) move(kv8_move_kernel<128, 1>);
+    else if (pieces <= 512) move(kv8_move_kernel<128, 2>);
+    else if (pieces <= 1024) move(kv8_move_kernel<128, 4>);
+    else move(kv8_move_kernel<128, 8>);
+  } else {
+    if (pieces <= 256) move(kv8_move_kernel<64, 1>);
+    else if (pieces <= 512) move(kv8_move_kernel<64, 2>);
+    else move(kv8_move_kernel<64, 4>);
+  }
   return check_launch(op);
 }
