@@ -45,14 +45,13 @@ struct RowsTile {
 };
 
 template <typename T, int D, int NB, int NW>
-__global__ __launch_bounds__(64 * NW, 4) void kv8_rows_kernel(Kv8Args a) {
+__device__ __forceinline__ void rows_item(const Kv8Args& a) {
   typedef typename AttnOp<T>::vec vec;
   constexpr bool F = std::is_same<T, F16>::value;
   constexpr int RT = 16 * NB, KS = D / 32, DT = D / 16, W = D / 64;
   __shared__ float red[NW * NB * DT * 4 * 64];
   __shared__ float ml[NW][RT][3];
 
-  kv8_rest<D>(a);
   Kv8Item it;
   if (!kv8_item<RT, RKT>(a, blockIdx.x, &it)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -312,6 +311,12 @@ __global__ __launch_bounds__(64 * NW, 4) void kv8_rows_kernel(Kv8Args a) {
       a.part_ml[(part0 + row) * 2 + 1] = l[nb];
     }
   }
+}
+
+template <typename T, int D, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, 4) void kv8_rows_kernel(Kv8Args a) {
+  rows_item<T, D, NB, NW>(a);
+  kv8_rest<D>(a);
 }
 
 template <typename T, int D>

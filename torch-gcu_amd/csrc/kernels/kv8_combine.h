@@ -8,8 +8,8 @@ namespace mi {
 namespace {
 
 // A wave per output row of a sequence that was cut: its parts' partials merged
-// in a fixed order, eight loads in flight.  Calls in which nothing was cut end
-// with the plan.
+// in order, eight at a time (their loads in flight together).  Calls in which
+// nothing was cut end with the plan.
 template <typename T, int D, int RT, int KT, bool LAST_FIRST>
 __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
   constexpr int E = D / 64, U = 8;
@@ -55,29 +55,35 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
     const int tile = LAST_FIRST ? c.row_tiles - 1 - row / RT : row / RT;
     const int64_t item = before + ((int64_t)tile * a.c.heads + h / a.group) * parts;
     if (item < 0 || item + parts > a.slots) continue;
-    const float* pm = a.part_ml + (item * RT + row % RT) * 2;
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2* pm = (const f2*)a.part_ml + item * RT + row % RT;
     const float* po = a.part_o + (item * RT + row % RT) * D + lane * E;
-    float M = -INFINITY;
-    for (int p = lane; p < parts; p += 64) M = fmaxf(M, pm[(int64_t)p * RT * 2]);
-    M = wave_fmax(M);
-    const float mu = M == -INFINITY ? 0.f : M;
-    float l = 0.f;
-    for (int p = lane; p < parts; p += 64)
-      l += pm[(int64_t)p * RT * 2 + 1] * __builtin_amdgcn_exp2f(pm[(int64_t)p * RT * 2] - mu);
-    l = wave_sum(l);
+    float M = -INFINITY, l = 0.f;
     fe acc = {};
     for (int p0 = 0; p0 < parts; p0 += U) {
       fe v[U];
-      float w[U];
+      f2 ml[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t p = min(p0 + u, parts - 1);
         v[u] = *(const fe*)(po + p * RT * D);
-        w[u] = pm[p * RT * 2];
+        ml[u] = pm[p * RT];
+        if (p0 + u >= parts) ml[u] = f2{-INFINITY, 0.f};
       }
+      float top = M;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (p0 + u < parts) acc += v[u] * __builtin_amdgcn_exp2f(w[u] - mu);
+      for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u][0]);
+      const float mu = top == -INFINITY ? 0.f : top;
+      const float before = __builtin_amdgcn_exp2f(M - mu);
+      M = top;
+      l *= before;
+      acc *= before;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = __builtin_amdgcn_exp2f(ml[u][0] - mu);
+        l += ml[u][1] * w;
+        if (p0 + u < parts) acc += v[u] * w;
+      }
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     typedef typename AttnOp<T>::elem Et;

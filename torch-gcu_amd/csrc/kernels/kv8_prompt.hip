@@ -30,7 +30,7 @@ __device__ __forceinline__ int swz_vt(int d) {
 }
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
+__device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   typedef typename AttnOp<T>::vec vec;
   constexpr int RT = 32 * NW, NT = 64 * NW;
   constexpr int KS = D / 16, DT = D / 32;
@@ -40,7 +40,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
   __shared__ __align__(16) uint16_t kt[2][PKT * D];
   __shared__ __align__(16) uint16_t vt[2][PKT * D];
 
-  kv8_rest<D>(a);
   Kv8Item it;
   if (!kv8_item<RT, PKT>(a, blockIdx.x, &it)) return;
   it.tile = it.cut.row_tiles - 1 - it.tile;  // the longest rows first
@@ -50,16 +49,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
   const int group = a.group, rows = it.cut.rows, len = it.s.len;
   const int row0 = it.tile * RT, wrow0 = row0 + 32 * wave;
 
-  const int row = wrow0 + col, rc = min(row, rows - 1);
-  const int64_t tok = it.s.first + rc / group, head = it.head * group + rc % group;
-  const int lim = row < rows ? kv8_limit(it.s, rc / group) : 0;
-  vec qf[KS];
-#pragma unroll
-  for (int t = 0; t < KS; ++t) {
-    qf[t] = *(const vec*)(a.q + tok * a.q_st + head * a.q_sh + 16 * t + 8 * half);
-    if (a.scale_log2 < 0.f) qf[t] = -qf[t];  // scales below are positive
-  }
-  const float scale = fabsf(a.scale_log2);
   // positions that the block's rows see, and this wave's: all, and any
   const int most = kv8_limit(it.s, (min(rows, row0 + RT) - 1) / group);
   const int w_least = wrow0 < rows ? kv8_limit(it.s, wrow0 / group) : 0;
@@ -159,11 +148,26 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
   float m_run = -INFINITY, l_run = 0.f;
   float vref = 0x1p-126f;  // the largest V scale met; o holds sums over it
 
-  // tile j's codes are loaded two steps before it is computed and converted one
-  // step before, their table entries a step earlier still
   if (lo < hi) {
     entries(lo);
     load(lo);
+  }
+  const int row = wrow0 + col, rc = min(row, rows - 1);
+  const int64_t tok = it.s.first + rc / group, head = it.head * group + rc % group;
+  const int lim = row < rows ? kv8_limit(it.s, rc / group) : 0;
+  vec qf[KS];
+#pragma unroll
+  for (int t = 0; t < KS; ++t) {
+    qf[t] = *(const vec*)(a.q + tok * a.q_st + head * a.q_sh + 16 * t + 8 * half);
+  }
+  const float scale = fabsf(a.scale_log2);
+  if (a.scale_log2 < 0.f) {  // scales below are positive
+#pragma unroll
+    for (int t = 0; t < KS; ++t) qf[t] = -qf[t];
+  }
+  // tile j's codes are loaded two steps before it is computed and converted one
+  // step before, their table entries a step earlier still
+  if (lo < hi) {
     entries(lo + 1);
     store(0);
     load(lo + 1);
@@ -246,15 +250,17 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
           p[g][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 1][8 * (g & 1) + r], sc[g], -m_use));
           ls[r & 3] += p[g][r];
         }
+      l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      asm volatile("" : "+v"(l_run));  // the sums stay here
       if (!plain) {
-        const float inv = __builtin_amdgcn_rcpf(vref);
+        float inv = __builtin_amdgcn_rcpf(vref);
+        asm volatile("" : "+v"(inv));  // the products below stay in this branch
 #pragma unroll
         for (int g = 0; g < 4; ++g) p[g] *= vs[g] * inv;
       }
       vec pk[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) pk[g] = __builtin_convertvector(p[g], vec);
-      l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -294,6 +300,12 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
     a.part_ml[at * 2] = m_run;
     a.part_ml[at * 2 + 1] = l;
   }
+}
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
+  prompt_item<T, D, NW>(a);
+  kv8_rest<D>(a);
 }
 
 template <typename T, int D>
