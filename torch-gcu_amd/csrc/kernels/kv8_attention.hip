@@ -323,8 +323,7 @@ template <typename T, int D>
 mi_status_t run_rows(Kv8Args& a, hipStream_t s) {
   constexpr int NB = 1, NW = 8;
   // two blocks of eight waves per CU; a part is at least a tile per wave
-  a.target = 2 * cu_count();
-  a.least = NW;
+  a.plan = {cu_count(), 0, NW};
   return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW>, 64 * NW, s);
 }
 
@@ -360,8 +359,14 @@ extern "C" mi_status_t mi_kv8_attention(const mi_tensor_t* out, const mi_tensor_
   a.fill_rest = fill_rest;
   a.fault = index_fault_word();
   hipStream_t s = (hipStream_t)stream;
-  // many rows a sequence: the prompt kernel
-  if ((int64_t)a.tokens * a.group > (int64_t)32 * std::min(a.seqs, a.tokens))
+  // The kernel here reads a sequence's keys once for each 16 rows, the prompt
+  // kernel once for 128, but with more to do around it.  us, this and the prompt
+  // kernel, 32 query heads on 8, D = 128: 8 sequences of 3000, 8 new tokens (32
+  // rows) each 21 / 46, 16: 29 / 49, 24: 43 / 39; 32 of 8000, 16 tokens each 196 /
+  // 200; 1 of 2000, 64 tokens 18 / 24; 1 of 16000, 24 tokens 37 / 31.
+  const int64_t rows = (int64_t)a.tokens * a.group;
+  if (rows > (int64_t)64 * std::min(a.seqs, a.tokens) &&
+      rows * a.c.heads * ((int64_t)a.width << a.c.shift) > (int64_t)1 << 23)
     return kv8_prompt(a, dim, q->dtype == MI_F16, s);
   if (q->dtype == MI_BF16) return dim == 128 ? run_rows<BF16, 128>(a, s) : run_rows<BF16, 64>(a, s);
   return dim == 128 ? run_rows<F16, 128>(a, s) : run_rows<F16, 64>(a, s);

@@ -95,14 +95,13 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
   }
 }
 
-// Room for the partials of a call whose parts are planned with a.target and
-// a.least, then the attention kernel and, where anything can have been cut,
+// Room for the partials of a call whose parts are planned by a.plan, then the attention kernel and, where anything can have been cut,
 // the merge.
 template <typename T, int D, int RT, int KT, bool LAST_FIRST, typename K>
 mi_status_t kv8_launch(Kv8Args& a, K kernel, int threads, hipStream_t s) {
   const int64_t base = kv8_row_tiles_most(a.tokens, a.seqs, a.group, RT) * a.c.heads;
-  const bool cut = ((int64_t)a.width << a.c.shift) / KT + 1 > a.least;
-  a.slots = (int)std::max<int64_t>(base + (cut ? a.target : 0), 1);
+  const bool cut = ((int64_t)a.width << a.c.shift) / KT + 1 > a.plan.least;
+  a.slots = (int)std::max<int64_t>(base + (cut ? a.plan.most() : 0), 1);
   Workspace ws;
   if (cut) {
     const size_t rows = (size_t)a.slots * RT;

@@ -37,7 +37,8 @@ struct Kv8Args {
   int64_t lse_st, lse_sh;
   float scale_log2;  // softmax scale * log2(e)
   int fill_rest;     // rows of no sequence: zeros (0: left as they were)
-  int target, least, slots;  // parts aimed at, fewest key tiles of one, partials there is room for
+  Kv8Plan plan;
+  int slots;         // partials there is room for
   float* part_o;     // [slots][rows of a tile][D], not normalised
   float* part_ml;    // [slots][rows of a tile][2]: max (log2 units), sum
   IndexFault* fault;
@@ -166,7 +167,7 @@ struct Kv8Lanes {
   __device__ __forceinline__ int chunk(F work) const {
     float sum = work(head);
     for (int b0 = 64; b0 < a.seqs; b0 += 64) sum += work(load(b0 + lane));
-    return wave_uniform(kv8_chunk(wave_sum(sum) * a.c.heads, a.target, a.least));
+    return wave_uniform(a.plan.chunk(wave_sum(sum) * a.c.heads));
   }
   // The sequence that item `item` belongs to, counted by count(s) per sequence
   // in order, and its place in it; false if there are fewer items.  Every lane

@@ -66,14 +66,21 @@ MI_HD Kv8Cut kv8_cut(const Kv8Seq& s, int group, int rt, int kt) {
   return c;
 }
 
-// Key tiles a part takes, so that `work` tiles (all sequences and k/v heads)
-// make at most `target` parts more than there are tiles of rows; never under
-// `least`.  work is a float sum, a few units of 2^-24 off, which the factor
-// makes up for.
-MI_HD int kv8_chunk(float work, int target, int least) {
-  const float c = work / (float)target * 1.00001f + 1.0f;
-  return c < (float)least ? least : c > 1073741824.f ? 1073741824 : (int)c;
-}
+// How the key tiles of a call are cut into parts: `target` parts in all, or twice
+// as many where a part would be longer than `wide` tiles, none shorter than
+// `least`.
+struct Kv8Plan {
+  int target, wide, least;
+  // the most parts that there are beside one for each tile of rows
+  MI_HD int most() const { return 2 * target; }
+  // Key tiles a part takes.  work, of all sequences and k/v heads, is a float
+  // sum, a few units of 2^-24 off, which the factor makes up for.
+  MI_HD int chunk(float work) const {
+    float c = work / (float)target * 1.00001f + 1.0f;
+    if (c > (float)wide) c = work / (float)most() * 1.00001f + 1.0f;
+    return c < (float)least ? least : c > 1073741824.f ? 1073741824 : (int)c;
+  }
+};
 
 // Row tiles that tokens x group rows in at most `seqs` sequences can make.
 MI_HD int64_t kv8_row_tiles_most(int64_t tokens, int64_t seqs, int64_t group, int rt) {

@@ -311,8 +311,11 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
 template <typename T, int D>
 mi_status_t run_prompt(Kv8Args& a, hipStream_t s) {
   constexpr int NW = 4;
-  a.target = 2 * cu_count();
-  a.least = 4;
+  // A block per CU where its tiles are few: two share a CU at 2.9 us a tile of
+  // each, one alone takes 1.7 to 2, and a part more costs 8 us and its partials
+  // (32 sequences of 512, 32 new tokens each: 28 us uncut, 47 in halves; 1 of
+  // 16128, 128 new: 89 us with a block per CU, 67 with two).
+  a.plan = {cu_count(), 24, 4};
   return kv8_launch<T, D, 32 * NW, PKT, true>(a, kv8_prompt_kernel<T, D, NW>, 64 * NW, s);
 }
 
