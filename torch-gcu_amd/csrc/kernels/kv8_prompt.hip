@@ -203,6 +203,13 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
         s[0] = AttnOp<T>::mma(*(const vec*)kp, qf[t], s[0]);
         s[1] = AttnOp<T>::mma(*(const vec*)(kp + 32 * D), qf[t], s[1]);
       }
+      // fragments read 6 ahead of their products
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
       // accumulator r of half st is key 32 st + 8 (r / 4) + 4 half + r % 4, of
       // the 16-key group 2 st + r / 8
       if (key0 + PKT > w_least || !all) {
@@ -269,6 +276,12 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
           const vec vf = *(const vec*)(vt[buf] + d * PKT + 8 * ((2 * g + half) ^ swz_vt<D>(d)));
           o[i] = AttnOp<T>::mma(vf, pk[g], o[i]);
         }
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+      for (int i = 0; i < 4 * DT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+      }
     }
   }
 
