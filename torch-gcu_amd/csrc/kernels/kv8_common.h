@@ -128,6 +128,12 @@ __device__ __forceinline__ V ld_const(const V* p) {
 // from it stays in scalar registers, and branches on it are scalar.
 __device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// lds_copy16 from an address of each lane's own.
+__device__ __forceinline__ void lds_copy16_at(const void* p, void* lds) {
+  const uint32_t m0 = wave_uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+}
+
 // Inclusive sums over the lanes, by DPP within rows of 16 and two row broadcasts.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int scan_step(int v) {

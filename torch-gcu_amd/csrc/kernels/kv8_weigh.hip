@@ -182,29 +182,52 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
   const Kv8Seq s = it.s;
   const int past = s.len - s.n;
   float* out = wt.w + it.seq * wt.sb + it.head * wt.sh;
-  // what this thread stages of a row tile: piece tid % CH of rows tid / CH + ...
-  u32x4 qr[N];
-  float lr = 0.f;
-  auto load = [&](int r0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int rc = min(r0 + tid / CH + n * (64 * WNW / CH), it.rows - 1);
-      const int64_t t = s.first + rc / group, h = it.head * group + rc % group;
-      qr[n] = *(const u32x4*)(a.q + t * a.q_st + h * a.q_sh + 8 * (tid % CH));
-    }
-    if (tid < RT) {
-      const int rc = min(r0 + tid, it.rows - 1);
-      const int64_t t = s.first + rc / group, h = it.head * group + rc % group;
-      lr = a.lse[t * a.lse_st + h * a.lse_sh] * 1.4426950408889634f;
+  // A row tile goes from global memory straight to LDS, 16 bytes a lane: this
+  // thread copies a piece of rows tid / CH + n RPI, the one that belongs at place
+  // tid % CH of its rows (the XOR swizzle repeats with the rows of a wave's
+  // copies).  Pointers advance from tile to tile (a division per row and tile
+  // would cost more than the products); rows past the last one read the last one.
+  constexpr int RPI = 64 * WNW / CH;
+  const int piece = 8 * (tid % CH ^ swz_k_of<D>(tid / CH & 31));
+  struct RowAt {
+    int64_t at;  // offset of the row's token and head
+    int g;       // its head in the group
+  };
+  const int step_t = RT / group, step_g = RT % group;
+  auto row_at = [&](int row, int64_t st, int64_t sh) __attribute__((always_inline)) {
+    return RowAt{(s.first + row / group) * st + (it.head * group + row % group) * sh, row % group};
+  };
+  auto advance = [&](RowAt& x, int64_t st, int64_t sh) __attribute__((always_inline)) {
+    x.at += step_t * st + step_g * sh;
+    if (step_g != 0) {
+      x.g += step_g;
+      if (x.g >= group) {
+        x.g -= group;
+        x.at += st - group * sh;
+      }
     }
   };
-  auto store = [&](int buf) __attribute__((always_inline)) {
+  const int64_t q_last = row_at(it.rows - 1, a.q_st, a.q_sh).at;
+  const int64_t l_last = row_at(it.rows - 1, a.lse_st, a.lse_sh).at;
+  RowAt q_at[N], l_at;
+  float lr = 0.f;
+  auto begin = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) q_at[n] = row_at(r0 + tid / CH + n * RPI, a.q_st, a.q_sh);
+    l_at = row_at(r0 + lane, a.lse_st, a.lse_sh);
+  };
+  auto copy = [&](int r0, int buf) __attribute__((always_inline)) {  // tiles in order after begin()
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int r = tid / CH + n * (64 * WNW / CH);
-      *(u32x4*)(qs[buf] + r * D + 8 * (tid % CH ^ swz_k_of<D>(r & 31))) = qr[n];
+      int64_t at = q_at[n].at;
+      if (r0 + RT > it.rows && r0 + tid / CH + n * RPI >= it.rows) at = q_last;
+      lds_copy16_at(a.q + at + piece, qs[buf] + (wave * 64 + n * 64 * WNW) * 8);
+      advance(q_at[n], a.q_st, a.q_sh);
     }
-    if (tid < RT) ls[buf][tid] = lr;
+    if (wave == 0) {  // RT == 64: a lane each
+      lr = a.lse[r0 + lane < it.rows ? l_at.at : l_last] * 1.4426950408889634f;
+      advance(l_at, a.lse_st, a.lse_sh);
+    }
   };
 
   for (int j = it.lo; j < it.hi; ++j) {
@@ -224,14 +247,14 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
     const int first = max(0, j * KT - past) * group / RT * RT;
     const int full = first_row(s, key0 + WKT - 1, group);
     __syncthreads();  // the buffers' last readers
-    load(first);
-    store(0);
-    if (first + RT < it.rows) load(first + RT);
+    begin(first);
+    copy(first, 0);
     int buf = 0;
     for (int r0 = first; r0 < it.rows; r0 += RT, buf ^= 1) {
+      if (wave == 0) ls[buf][lane] = lr;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies of the tile
       __syncthreads();
-      if (r0 + RT < it.rows) store(buf ^ 1);
-      if (r0 + 2 * RT < it.rows) load(r0 + 2 * RT);
+      if (r0 + RT < it.rows) copy(r0 + RT, buf ^ 1);
       if (key0 >= s.len) continue;
 #pragma unroll
       for (int u = 0; u < RT / 32; ++u) {
@@ -253,9 +276,11 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
 #pragma unroll
           for (int r = 0; r < 16; ++r) sum[r] += x[r];
         } else {
+          int base = key0 + 4 * half;
+          asm volatile("" : "+v"(base));  // nothing of this branch waits in registers outside it
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int key = key0 + 8 * (r >> 2) + 4 * half + (r & 3);
+            const int key = base + 8 * (r >> 2) + (r & 3);
             const bool sees = row + col < it.rows && row + col >= first_row(s, key, group);
             sum[r] += sees ? x[r] : 0.f;
           }
