@@ -202,10 +202,10 @@ int main() {
       assert((long)c.key_tiles * kt >= s.len && ((long)c.key_tiles - 1) * kt < s.len);
       assert(c.row_tiles <= kv8_row_tiles_most(s.n, 1, group, rt));
       for (int target : {1, 256, 512}) for (int wide : {0, 24}) {
-        const Kv8Plan plan{target, wide, 8};
+        const Kv8Plan plan{target, wide, 8, 2 * target};
         const int chunk = plan.chunk(c.work() * 8), parts = c.parts(chunk);
         assert(parts >= 1 && chunk >= 8);
-        assert(8L * c.row_tiles * parts <= plan.most() + 8L * c.row_tiles);
+        assert(8L * c.row_tiles * parts <= plan.many + 8L * c.row_tiles);
       }
     }
     ++n;
@@ -219,7 +219,7 @@ int main() {
   for (int round = 0; round < 2000; ++round) {
     const int seqs = 1 + rand() % 200, heads = 1 + rand() % 16, group = 1 + rand() % 8;
     const int rt = rand() % 2 ? 16 : 128, kt = rt == 16 ? 32 : 64;
-    const Kv8Plan plan{256, rand() % 2 ? 0 : 24, 8};
+    const Kv8Plan plan{256, rand() % 2 ? 0 : 24, 8, 512};
     long tokens = 0, items = 0, touched = 0;
     float work = 0;
     static Kv8Seq all[200];
@@ -235,7 +235,7 @@ int main() {
       const Kv8Cut c = kv8_cut(all[b], group, rt, kt);
       items += (long)heads * c.row_tiles * c.parts(chunk);
     }
-    assert(items <= plan.most() + heads * kv8_row_tiles_most(tokens, seqs, group, rt));
+    assert(items <= plan.many + heads * kv8_row_tiles_most(tokens, seqs, group, rt));
     assert(touched <= kv8_touched_most(tokens, seqs, 4));
   }
   for (unsigned u = 0; u < 0x7f800000u; u += 12345) {

@@ -44,7 +44,7 @@ struct RowsTile {
   bool ok[2];               // the 16-key half lies in a page
 };
 
-template <typename T, int D, int NB, int NW>
+template <typename T, int D, int NB, int NW, bool ONCE>
 __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   typedef typename AttnOp<T>::vec vec;
   constexpr bool F = std::is_same<T, F16>::value;
@@ -91,6 +91,11 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
     for (int t = 0; t < 2; ++t)
       e[t] = ld_const(table + min((j * RKT + 16 * t) >> shift, a.width - 1));
   };
+  // codes that one block reads once are not kept in the caches
+  auto code = [](const auto* p) __attribute__((always_inline)) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return *p;
+  };
   auto load = [&](int j, const int* e, RowsTile<D>& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -103,15 +108,15 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
       const uint8_t* kp = kc + page * a.c.k_sp + off;
       const uint8_t* vp = vc + page * a.c.v_sp + off;
 #pragma unroll
-      for (int h = 0; h < W; ++h) x.k[t][h] = *(const u32x4*)(kp + 64 * h);
+      for (int h = 0; h < W; ++h) x.k[t][h] = code((const u32x4*)(kp + 64 * h));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (W == 2) {
-          const u32x2 y = *(const u32x2*)(vp + i * D);
+          const u32x2 y = code((const u32x2*)(vp + i * D));
           x.v[4 * t + i][0] = y[0];
           x.v[4 * t + i][1] = y[1];
         } else {
-          x.v[4 * t + i][0] = *(const uint32_t*)(vp + i * D);
+          x.v[4 * t + i][0] = code((const uint32_t*)(vp + i * D));
         }
       }
       x.ks[t] = ld_const(ksc + page * a.c.ks_sp);
@@ -313,18 +318,29 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   }
 }
 
-template <typename T, int D, int NB, int NW>
+template <typename T, int D, int NB, int NW, bool ONCE>
 __global__ __launch_bounds__(64 * NW, 4) void kv8_rows_kernel(Kv8Args a) {
-  rows_item<T, D, NB, NW>(a);
+  rows_item<T, D, NB, NW, ONCE>(a);
   kv8_rest<D>(a);
 }
 
 template <typename T, int D>
 mi_status_t run_rows(Kv8Args& a, hipStream_t s) {
   constexpr int NB = 1, NW = 8;
-  // two blocks of eight waves per CU; a part is at least a tile per wave
-  a.plan = {cu_count(), 0, NW};
-  return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW>, 64 * NW, s);
+  // Two blocks of eight waves per CU, and twice as many parts where they are long
+  // enough that the last ones to end count (32 sequences of 4000 to 16000: 130 ->
+  // 119 us).  A part is at least a tile per wave, and short sequences stay whole,
+  // since the merge is a launch of 4 us: up to 1024 positions (1 of 300: 13 -> 8
+  // us), or 2048 where there is a pair for each CU (32 x 8 of 2000: 29 -> 25).
+  const int cus = cu_count();
+  const int64_t tiles = (((int64_t)a.width << a.c.shift) + RKT - 1) / RKT;
+  const int64_t pairs = kv8_row_tiles_most(a.tokens, a.seqs, a.group, 16 * NB) * a.c.heads;
+  const int whole = pairs >= cus ? 8 * NW : 4 * NW;
+  a.plan = {2 * cus, 64, tiles <= whole ? whole : NW, 4 * cus};
+  // one row tile a sequence: its codes are read once
+  if ((int64_t)a.tokens * a.group <= (int64_t)16 * NB * std::min(a.seqs, a.tokens))
+    return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW, true>, 64 * NW, s);
+  return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW, false>, 64 * NW, s);
 }
 
 }  // namespace

@@ -66,18 +66,16 @@ MI_HD Kv8Cut kv8_cut(const Kv8Seq& s, int group, int rt, int kt) {
   return c;
 }
 
-// How the key tiles of a call are cut into parts: `target` parts in all, or twice
-// as many where a part would be longer than `wide` tiles, none shorter than
-// `least`.
+// How the key tiles of a call are cut into parts: `few` parts in all, or `many`
+// where a part would be longer than `wide` tiles, none shorter than `least`.
 struct Kv8Plan {
-  int target, wide, least;
-  // the most parts that there are beside one for each tile of rows
-  MI_HD int most() const { return 2 * target; }
+  int few, wide, least, many;  // few <= many
   // Key tiles a part takes.  work, of all sequences and k/v heads, is a float
-  // sum, a few units of 2^-24 off, which the factor makes up for.
+  // sum, a few units of 2^-24 off, which the factor makes up for; the parts are
+  // at most `many` more than the tiles of rows.
   MI_HD int chunk(float work) const {
-    float c = work / (float)target * 1.00001f + 1.0f;
-    if (c > (float)wide) c = work / (float)most() * 1.00001f + 1.0f;
+    float c = work / (float)few * 1.00001f + 1.0f;
+    if (c > (float)wide) c = work / (float)many * 1.00001f + 1.0f;
     return c < (float)least ? least : c > 1073741824.f ? 1073741824 : (int)c;
   }
 };

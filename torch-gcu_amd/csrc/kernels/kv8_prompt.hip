@@ -328,7 +328,10 @@ mi_status_t run_prompt(Kv8Args& a, hipStream_t s) {
   // each, one alone takes 1.7 to 2, and a part more costs 8 us and its partials
   // (32 sequences of 512, 32 new tokens each: 28 us uncut, 47 in halves; 1 of
   // 16128, 128 new: 89 us with a block per CU, 67 with two).
-  a.plan = {cu_count(), 24, 4};
+  const int cus = cu_count();
+  const int64_t tiles = (((int64_t)a.width << a.c.shift) + PKT - 1) / PKT;
+  const int64_t blocks = kv8_row_tiles_most(a.tokens, a.seqs, a.group, 32 * NW) * a.c.heads;
+  a.plan = {cus, 24, blocks >= cus && tiles <= 24 ? 24 : 4, 2 * cus};
   return kv8_launch<T, D, 32 * NW, PKT, true>(a, kv8_prompt_kernel<T, D, NW>, 64 * NW, s);
 }
 

@@ -307,8 +307,8 @@ mi_status_t run_weigh(Kv8Args& a, const Kv8Weights& w, hipStream_t s) {
   const dim3 block(64 * WNW);
   // blocks of few rows: four a CU at once
   const bool few = (int64_t)a.tokens * a.group <= (int64_t)32 * some;
-  a.plan = {2 * cu_count(), 0, 1};
-  const dim3 grid((unsigned)(a.plan.most() + some * a.c.heads));
+  a.plan = {4 * cu_count(), 0, 1, 4 * cu_count()};
+  const dim3 grid((unsigned)(a.plan.many + some * a.c.heads));
   if (few) hipLaunchKernelGGL((kv8_weigh_rows_kernel<T, D>), grid, block, 0, s, a, w);
   else hipLaunchKernelGGL((kv8_weigh_prompt_kernel<T, D>), grid, block, 0, s, a, w);
   return check_launch("kv8_weigh");
