@@ -14,6 +14,7 @@ import torch
 import torch_gcu  # noqa: F401
 from oracle import kv8 as oracle
 from torch_gcu import _abi
+from torch_gcu.utils import decoder_layer as dl
 
 pytestmark = pytest.mark.gpu
 eff = torch.gcu.efficient if hasattr(torch, "gcu") else None
@@ -547,3 +548,63 @@ def test_refusals_on_the_device():
         eff.kv8_append(s.k.to("gcu"), s.v.to("gcu"), cache, index[0], index[1].long(), index[2])
     with pytest.raises(RuntimeError, match="positions"):
         eff.kv8_weigh_(torch.zeros(1, 2, 8).to("gcu"), s.q.to("gcu"), torch.zeros(1, 4).to("gcu"), cache, *index)
+
+
+def test_decoder_layer_over_the_cache():
+    """Prompts in two pieces, then captured decode steps: the layer is what its ops
+    give one by one, its attention what the definition says, and a replay with new
+    lengths is the eager call, bit for bit."""
+    cfg = dl.LayerConfig(vocab=100, hidden=256, heads=4, head_dim=64, ffn=512)
+    w = {n: t.to("gcu") for n, t in dl.init_weights(cfg, 3).items()}
+    for n in ("wk", "wv"):  # two k/v heads
+        w[n] = w[n][:128].contiguous()
+    g = gen(1)
+    tables = [[5, 2, 9, 1], [0, 7, 3, 4]]
+    table = torch.tensor(tables, dtype=torch.int32).to("gcu")
+    cache, mine = eff.kv8_cache(10, 2, 64, 32), eff.kv8_cache(10, 2, 64, 32)
+    lens = [0, 0]
+
+    def call(new):
+        for b in range(2):
+            lens[b] += new[b]
+        ids = torch.randint(0, 100, (sum(new),), generator=g)
+        pos = torch.cat([torch.arange(n - m, n) for n, m in zip(lens, new)])
+        i32 = [torch.tensor(x, dtype=torch.int32) for x in (lens, [0, new[0], sum(new)])]
+        return [t.to("gcu") for t in (ids, *i32, pos)]
+
+    def by_hand(ids, lengths, starts, pos):
+        e, T = eff, ids.shape[0]
+        x = torch.nn.functional.embedding(ids, w["embed"])
+        h = e.rms_norm(x, w["attn_norm"], cfg.eps)
+        q, k, v = (torch.nn.functional.linear(h, w[n]).view(T, -1, 64) for n in ("wq", "wk", "wv"))
+        q, k = e.rope(q, k, pos, cfg.theta)
+        e.kv8_append(k, v, mine, table, lengths, starts)
+        a, lse = e.kv8_attention(q, mine, table, lengths, starts)
+        s = Setup.__new__(Setup)
+        s.q, s.cache, s.table, s.lens = q.cpu(), [t.cpu() for t in mine], tables, list(lens)
+        s.starts, s.d, s.dtype = starts.cpu().tolist(), 64, q.dtype
+        check_attention(s, a, lse)
+        x = x + torch.nn.functional.linear(a.view(T, -1), w["wo"])
+        h = e.rms_norm(x, w["ffn_norm"], cfg.eps)
+        m = e.silu_mul(torch.nn.functional.linear(h, w["w_gate"]), torch.nn.functional.linear(h, w["w_up"]))
+        return x + torch.nn.functional.linear(m, w["w_down"])
+
+    for new in ([40, 3], [20, 30], [1, 1]):
+        ids, lengths, starts, pos = call(new)
+        out, _, _ = dl.forward_cached(w, ids, cfg, cache, table, lengths, starts, pos)
+        assert torch.equal(out.cpu(), by_hand(ids, lengths, starts, pos).cpu())
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(cache, mine))
+    # a captured decode step: its inputs are updated in place between replays (the
+    # last eager step is done again by the capture, which runs nothing)
+    static = [ids, lengths, starts, pos]
+    graph = torch.gcu.GCUGraph()
+    with torch.gcu.graph(graph):
+        out, _, _ = dl.forward_cached(w, ids, cfg, cache, table, lengths, starts, pos)
+    for _ in range(4):
+        new = call([1, 1])
+        for t, x in zip(static, new):
+            t.copy_(x)
+        graph.replay()
+        torch.gcu.synchronize()
+        assert torch.equal(out.cpu(), by_hand(*new).cpu())
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(cache, mine))

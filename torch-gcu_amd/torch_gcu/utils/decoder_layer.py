@@ -7,6 +7,9 @@ with the residual add and the gate / up projections with the SiLU-mul fused
 into the matmul epilogue (efficient ops that give what linear + add and
 linear, linear + silu_mul give, bit for bit).
 
+``forward_cached`` is the layer of a server: the new tokens of any number of
+sequences against an 8-bit key/value cache.
+
 The same module runs on CPU tensors with the ATen compositions of the fused
 ops, which is how the tests compare the two paths.
 """
@@ -126,6 +129,35 @@ def forward(weights: dict, ids: torch.Tensor, cfg: LayerConfig,
     h = _rms_norm(x, weights["ffn_norm"], cfg.eps)
     m = _linear_silu_mul(h, weights["w_gate"], weights["w_up"])
     return _linear_residual(m, weights["w_down"], x)
+
+
+def forward_cached(weights: dict, ids: torch.Tensor, cfg: LayerConfig, cache,
+                   block_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor,
+                   pos: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The layer over the new tokens of any number of sequences, whose keys and
+    values go to (and are read from) an 8-bit cache: pieces of prompts, decode
+    steps or both in one call (gcu only).
+
+    ids [tokens], packed by sequence, with their positions pos (int64) for RoPE;
+    cache, block_table, lengths and starts as for
+    ``torch.gcu.efficient.kv8_append``.  Nothing is created on the host, so a
+    captured call can be replayed after the index tensors have been updated.
+    Returns the hidden states [tokens, hidden], and the queries and logsumexp
+    that ``kv8_weigh_`` takes."""
+    eff = torch.gcu.efficient
+    T, H, D = ids.shape[0], cfg.heads, cfg.head_dim
+    x = F.embedding(ids, weights["embed"])
+    h = _rms_norm(x, weights["attn_norm"], cfg.eps)
+    q = F.linear(h, weights["wq"]).view(T, H, D)
+    k = F.linear(h, weights["wk"]).view(T, -1, D)
+    v = F.linear(h, weights["wv"]).view(T, -1, D)
+    _rope_(q, k, pos, cfg.theta)
+    eff.kv8_append(k, v, cache, block_table, lengths, starts)
+    a, lse = eff.kv8_attention(q, cache, block_table, lengths, starts)
+    x = _linear_residual(a.view(T, H * D), weights["wo"], x)
+    h = _rms_norm(x, weights["ffn_norm"], cfg.eps)
+    m = _linear_silu_mul(h, weights["w_gate"], weights["w_up"])
+    return _linear_residual(m, weights["w_down"], x), q, lse
 
 
 def flops(cfg: LayerConfig, batch: int, seq: int) -> int:
