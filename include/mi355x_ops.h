@@ -491,7 +491,8 @@ mi_status_t mi_layer_norm_backward(const mi_tensor_t* grad_input,
  * No counterpart in the reference.  A pool of pages holds e4m3 codes (one
  * byte each) of the keys and values, with one float32 scale per page and k/v
  * head: value = code * scale.  mi_kv8_append and mi_kv8_evict write powers of
- * two, the smallest s >= 2^-110 with amax <= 448 s; reading takes any scale.
+ * two, the smallest s >= 2^-110 with amax <= 448 s; reading takes any scale
+ * that is not negative.
  *
  *   k, v              uint8   [pages, heads, page, head_dim]; head_dim 64 or
  *                     128, page a power of two from 16 to 256; a page's head
@@ -537,7 +538,7 @@ mi_status_t mi_kv8_append(const mi_kv8_cache_t* cache, const mi_tensor_t* k,
  * q and out bf16 or f16 [tokens, H, head_dim].  Rows of no sequence are left as
  * they were, or with fill_rest set to 0 and -inf.  fp32 scores, sums and
  * accumulation; softmax weights are rounded to q's type.  Partial sums of cut
- * sequences take workspace. */
+ * sequences take workspace; nothing is cut when there is none. */
 mi_status_t mi_kv8_attention(const mi_tensor_t* out, const mi_tensor_t* lse,
                              const mi_tensor_t* q, const mi_kv8_cache_t* cache,
                              const mi_tensor_t* block_table,

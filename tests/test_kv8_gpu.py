@@ -7,6 +7,9 @@ softmax weight by that share, twice over (the weight and the sum); each weight
 is rounded to q's type (u, and under f16's normal range 2^-25 of the largest
 value) and the output once more (u).  Codes, scales and kept positions are exact."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -473,6 +476,25 @@ def test_same_bits_every_time():
         o, e = eff.kv8_attention(q, cache, *index)
         x = eff.kv8_weigh_(torch.zeros(2, 4, s.width * 64).to("gcu"), q, e, cache, *index)
         assert all(torch.equal(a.cpu(), b.cpu()) for a, b in ((o, out), (e, lse), (x, w)))
+
+
+def test_without_workspace_sequences_stay_whole(tmp_path):
+    """In a process of its own, where no workspace allocator is registered."""
+    s = Setup([1, 40], [3000, 2000], 8, 2, 128, 32, seed=17).fill()
+    args, got = tmp_path / "args.pt", tmp_path / "got.pt"
+    torch.save([s.q, *s.cache, *(t.cpu() for t in s.index())], args)
+    code = ("import sys, torch\n"
+            "from torch_gcu import _abi\n"
+            "q, *rest = [t.cuda() for t in torch.load(sys.argv[1], weights_only=True)]\n"
+            "out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device='cuda')\n"
+            "_abi.lib().mi_set_workspace_allocator(_abi._ALLOC_FN(), _abi._FREE_FN(), None)\n"
+            "_abi.kv8_attention(out, lse, q, rest[:4], *rest[4:])\n"
+            "torch.save([out.cpu(), lse.cpu()], sys.argv[2])\n")
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
+    r = subprocess.run([sys.executable, "-c", code, str(args), str(got)], env=env, capture_output=True,
+                       text=True, timeout=100)
+    assert r.returncode == 0, r.stderr[-2000:]
+    check_attention(s, *torch.load(got, weights_only=True))
 
 
 def test_bad_pages_and_lengths_raise_and_touch_nothing():

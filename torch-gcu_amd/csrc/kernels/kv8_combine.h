@@ -18,8 +18,9 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
   const Kv8Lanes lanes(a);
   const int lane = lanes.lane;
   bool some = false;
-  const int chunk =
-      lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, RT, KT).work(); });
+  // (the attention kernel's own number: a float of the plan compiled here could
+  // be rounded differently)
+  const int chunk = wave_uniform(*a.chunk);
   for (int b0 = 0; b0 < a.seqs; b0 += 64) {
     const Kv8Seq s = lanes.at(b0);
     some = some || __ballot(s.n > 0 && kv8_cut(s, a.group, RT, KT).parts(chunk) > 1) != 0;
@@ -102,16 +103,23 @@ mi_status_t kv8_launch(Kv8Args& a, K kernel, int threads, hipStream_t s) {
   const int64_t base = kv8_row_tiles_most(a.tokens, a.seqs, a.group, RT) * a.c.heads;
   const int64_t key_tiles = (((int64_t)a.width << a.c.shift) + KT - 1) / KT;
   const int64_t parts = std::max<int64_t>((key_tiles + a.plan.least - 1) / a.plan.least, 1);
-  const bool cut = parts > 1;
+  bool cut = parts > 1;
   // (idle blocks are not free: 8 sequences of 4000 took 19 us with 512 of them,
   // 24 with 4096)
   a.slots = (int)std::max<int64_t>(std::min(base + a.plan.many, base * parts), 1);
   Workspace ws;
   if (cut) {
     const size_t rows = (size_t)a.slots * RT;
-    MI_RETURN_IF(ws.alloc(rows * (D + 2) * sizeof(float), s));
-    a.part_o = (float*)ws.get();
-    a.part_ml = a.part_o + rows * D;
+    if (ws.alloc((rows * (D + 2) + 1) * sizeof(float), s) == MI_OK) {
+      a.part_o = (float*)ws.get();
+      a.part_ml = a.part_o + rows * D;
+      a.chunk = (int*)(a.part_ml + rows * 2);
+    } else {  // whole sequences need none
+      clear_error();
+      cut = false;
+      a.plan.least = 0x40000000;
+      a.slots = (int)std::max<int64_t>(base, 1);
+    }
   }
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.slots), dim3(threads), 0, s, a);
   MI_RETURN_IF(check_launch("kv8_attention"));

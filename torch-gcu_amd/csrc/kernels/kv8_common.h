@@ -41,6 +41,7 @@ struct Kv8Args {
   int slots;         // partials there is room for
   float* part_o;     // [slots][rows of a tile][D], not normalised
   float* part_ml;    // [slots][rows of a tile][2]: max (log2 units), sum
+  int* chunk;        // key tiles of a part, as the attention kernel cut them, for the merge
   IndexFault* fault;
 };
 
@@ -211,6 +212,7 @@ __device__ __forceinline__ bool kv8_item(const Kv8Args& a, int item, Kv8Item* it
   const Kv8Lanes lanes(a);
   const int chunk =
       lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, RT, KT).work(); });
+  if (item == 0 && a.chunk != nullptr && threadIdx.x == 0) *a.chunk = chunk;
   int place;
   const bool found = lanes.find(
       item,
