@@ -179,8 +179,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
       }
       float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                        fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      mx = half_max(row_max(mx));
       if (mx > m_run[nb]) {
         const float corr = __builtin_amdgcn_exp2f(m_run[nb] - mx);
         m_run[nb] = mx;
@@ -250,9 +249,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   // merge the waves: common max, scaled sums, O added in wave order
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    float l = l_run[nb];
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    const float l = half_sum(row_sum(l_run[nb]));
     if (g == 0) {
       ml[wave][16 * nb + c][0] = m_run[nb];
       ml[wave][16 * nb + c][1] = l;

@@ -129,6 +129,33 @@ __device__ __forceinline__ V ld_const(const V* p) {
 // from it stays in scalar registers, and branches on it are scalar.
 __device__ __forceinline__ int wave_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+__device__ __forceinline__ float wave_uniform_f32(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
+// The larger (the sum) of a lane's value and that of the lane 32 (16) from it, by
+// lane swaps instead of a round through LDS.
+template <bool SUM>
+__device__ __forceinline__ float over_halves(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t u0 = r[0], u1 = r[1];  // (a bit cast of a vector's element takes element 0)
+  const float a = __builtin_bit_cast(float, u0), b = __builtin_bit_cast(float, u1);
+  return SUM ? a + b : fmaxf(a, b);
+}
+template <bool SUM>
+__device__ __forceinline__ float over_rows(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t u0 = r[0], u1 = r[1];  // (a bit cast of a vector's element takes element 0)
+  const float a = __builtin_bit_cast(float, u0), b = __builtin_bit_cast(float, u1);
+  return SUM ? a + b : fmaxf(a, b);
+}
+__device__ __forceinline__ float half_max(float x) { return over_halves<false>(x); }
+__device__ __forceinline__ float half_sum(float x) { return over_halves<true>(x); }
+__device__ __forceinline__ float row_max(float x) { return over_rows<false>(x); }
+__device__ __forceinline__ float row_sum(float x) { return over_rows<true>(x); }
+
 // lds_copy16 from an address of each lane's own.
 __device__ __forceinline__ void lds_copy16_at(const void* p, void* lds) {
   const uint32_t m0 = wave_uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);

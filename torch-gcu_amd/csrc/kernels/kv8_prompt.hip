@@ -39,6 +39,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   constexpr int KN = NW == 8 ? KU / 256 : KU / NT;  // a thread's K units
   __shared__ __align__(16) uint16_t kt[2][PKT * D];
   __shared__ __align__(16) uint16_t vt[2][PKT * D];
+  __shared__ __align__(16) float scales[2][8];  // of a tile's 16-key groups: scores', values'
+  __shared__ int absent[2];                     // bit g: group g does not exist
 
   Kv8Item it;
   if (!kv8_item<RT, PKT>(a, blockIdx.x, &it)) return;
@@ -57,6 +59,7 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   const int lo = (int)((int64_t)tiles * it.part / it.parts);
   const int hi = (int)((int64_t)tiles * (it.part + 1) / it.parts);
 
+  const float scale = fabsf(a.scale_log2);
   const int shift = a.c.shift, in_page = (1 << shift) - 1;
   const int* table = a.table + it.seq * a.t_sb;
   const uint8_t* kc = a.c.k + it.head * a.c.k_sh;
@@ -75,6 +78,12 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   u32x4 kr[KN];
   uint32_t vr[8];
   int ke[KN], ve = 0;
+  // one thread a 16-key group brings its scales: they come by the way of the
+  // codes, since scalar loads return out of order and would make every wait for
+  // an LDS read a wait for all of them
+  int se = 0;
+  float s_k = 0.f, s_v = 0.f;
+  bool s_ok = true;
   int v_left = 0;  // of this thread's 8 keys those nearer than this exist
   auto entries = [&](int j) __attribute__((always_inline)) {
     if (has_k) {
@@ -83,6 +92,7 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
         ke[n] = entry_of(j * PKT + (ku + n * (NW == 8 ? 256 : NT)) / (D / 16));
     }
     if (has_v) ve = entry_of(j * PKT + v_key);
+    if (tid < 4) se = entry_of(j * PKT + 16 * tid);
   };
   auto load = [&](int j) __attribute__((always_inline)) {
     const int key0 = j * PKT;
@@ -103,8 +113,23 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) vr[i] = *(const uint32_t*)(vp + (i < 4 ? i : i + 4) * D);
     }
+    if (tid < 4) {
+      const int p = kv8_page(se, a.c.pages);
+      const bool in = key0 + 16 * tid < len;
+      s_ok = in && p >= 0;
+      if (in && p < 0) record_index_fault(a.fault, se, a.c.pages);
+      s_k = ksc[max(p, 0) * a.c.ks_sp];
+      s_v = vsc[max(p, 0) * a.c.vs_sp];
+    }
   };
   auto store = [&](int buf) __attribute__((always_inline)) {
+    if (tid < 4) {
+      const float k = scale * s_k;
+      scales[buf][tid] = k < 0x1p-100f ? 0x1p-100f : k;  // masked scores stay -inf when multiplied by it
+      scales[buf][4 + tid] = s_ok ? s_v : 0.f;
+      const uint64_t gone = __ballot(!s_ok);
+      if (tid == 0) absent[buf] = (int)gone;
+    }
     if (has_k) {
 #pragma unroll
       for (int n = 0; n < KN; ++n) {
@@ -160,7 +185,6 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   for (int t = 0; t < KS; ++t) {
     qf[t] = *(const vec*)(a.q + tok * a.q_st + head * a.q_sh + 16 * t + 8 * half);
   }
-  const float scale = fabsf(a.scale_log2);
   if (a.scale_log2 < 0.f) {  // scales below are positive
 #pragma unroll
     for (int t = 0; t < KS; ++t) qf[t] = -qf[t];
@@ -180,22 +204,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
     if (j + 2 < hi) load(j + 2);
     entries(j + 3);
     if (key0 < w_most) {
-      // scales of the tile's four 16-key groups
-      float sc[4], vs[4];
-      bool ok[4], all = true;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int pos = key0 + 16 * g;
-        const int e = ld_const(table + min(pos >> shift, a.width - 1));
-        const int p = kv8_page(e, a.c.pages);
-        ok[g] = pos < len && p >= 0;
-        all = all && ok[g];
-        if (pos < len && p < 0 && lane == 0) record_index_fault(a.fault, e, a.c.pages);
-        const int64_t page = max(p, 0);
-        const float k = scale * ld_const(ksc + page * a.c.ks_sp);
-        sc[g] = k < 0x1p-100f ? 0x1p-100f : k;  // masked scores stay -inf when multiplied by it
-        vs[g] = ok[g] ? ld_const(vsc + page * a.c.vs_sp) : 0.f;
-      }
+      const f32x4 sc = *(const f32x4*)scales[buf], vs = *(const f32x4*)(scales[buf] + 4);
+      const int gone = wave_uniform(absent[buf]);
       f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
@@ -212,13 +222,13 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
       }
       // accumulator r of half st is key 32 st + 8 (r / 4) + 4 half + r % 4, of
       // the 16-key group 2 st + r / 8
-      if (key0 + PKT > w_least || !all) {
+      if (key0 + PKT > w_least || gone != 0) {
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int key = key0 + 32 * st + 8 * (r >> 2) + 4 * half + (r & 3);
-            s[st][r] = key < lim && ok[2 * st + (r >> 3)] ? s[st][r] : -INFINITY;
+            s[st][r] = key < lim && !(gone >> (2 * st + (r >> 3)) & 1) ? s[st][r] : -INFINITY;
           }
       }
       float mx = -INFINITY;
@@ -229,8 +239,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
         for (int r = 1; r < 8; ++r) x = fmaxf(x, s[g >> 1][8 * (g & 1) + r]);
         mx = fmaxf(mx, x * sc[g]);
       }
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float top = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+      mx = half_max(mx);
+      const float top = wave_uniform_f32(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
       float corr = 1.f;
       if (top > vref) {
         corr = vref * __builtin_amdgcn_rcpf(top);
@@ -248,7 +258,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       float ls[4] = {0.f, 0.f, 0.f, 0.f};
-      const bool plain = vs[0] == vref && vs[1] == vref && vs[2] == vref && vs[3] == vref;
+      const bool plain =
+          wave_uniform(vs[0] == vref && vs[1] == vref && vs[2] == vref && vs[3] == vref) != 0;
       f32x8 p[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g)
@@ -285,7 +296,7 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
     }
   }
 
-  const float l = l_run + __shfl_xor(l_run, 32, 64);
+  const float l = half_sum(l_run);
   if (row >= rows) return;
   const bool whole = it.parts == 1;
   if (!whole && (int)blockIdx.x >= a.slots) return;

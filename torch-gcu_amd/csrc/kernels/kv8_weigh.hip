@@ -294,7 +294,7 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
       v += dpp_f32<0x4E>(v);
       v += dpp_f32<0x141>(v);
       v += dpp_f32<0x140>(v);
-      v += __shfl_xor(v, 16, 64);
+      v = row_sum(v);
       const int key = key0 + 8 * (r >> 2) + 4 * half + (r & 3);
       if (col == r && key < s.len && keys.ok[r >> 3]) out[key] += v;
     }
