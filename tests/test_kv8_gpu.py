@@ -110,6 +110,8 @@ SHAPES = [
     ([300, 5], [1500, 2000], 8, 8, 128, 16),
     ([600], [0], 3, 1, 128, 128),
     ([64, 64], [64, 0], 16, 2, 64, 256),
+    ([1024], [3700], 64, 8, 64, 256),                # 256 blocks of 256 rows
+    ([515, 500], [4000, 3333], 32, 32, 128, 64),     # and rows that do not fill them
 ]
 
 

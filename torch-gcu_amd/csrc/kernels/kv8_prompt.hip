@@ -334,16 +334,30 @@ __global__ __launch_bounds__(64 * NW, 2) void kv8_prompt_kernel(Kv8Args a) {
 
 template <typename T, int D>
 mi_status_t run_prompt(Kv8Args& a, hipStream_t s) {
-  constexpr int NW = 4;
-  // A block per CU where its tiles are few: two share a CU at 2.9 us a tile of
+  const int cus = cu_count();
+  const int64_t tiles = (((int64_t)a.width << a.c.shift) + PKT - 1) / PKT;
+  // blocks, if the sequences' new tokens are about as many in each
+  auto blocks = [&](int nw) {
+    const int64_t some = std::min(a.seqs, a.tokens), rows = (int64_t)a.tokens * a.group;
+    return some > 0 ? some * ((rows / some + 32 * nw - 1) / (32 * nw)) * a.c.heads : 0;
+  };
+  // 256 rows a block halve what is spent on conversions and loads, but one such
+  // block fills a CU: taken for long sequences whose blocks fill seven eighths of
+  // their rounds over the CUs.  us, 256 and 128 rows, 32 query heads on 8: 1 x 2048
+  // tokens behind 14000 (256 blocks) 546 / 603, 2 x 2048 behind 14000 (512) 1042 /
+  // 1154, 4 x 2048 behind 4000 (1024) 732 / 788, 3 x 1500 behind 4000 (576) 474 /
+  // 465, 8 x 1024 behind nothing 137 / 125.
+  const int64_t wide = blocks(8), rounds = (wide + cus - 1) / cus;
+  if (tiles >= 64 && wide > 0 && wide * 8 >= rounds * cus * 7) {
+    a.plan = {cus, 0x40000000, 24, cus};
+    return kv8_launch<T, D, 256, PKT, true>(a, kv8_prompt_kernel<T, D, 8>, 512, s);
+  }
+  // A block per CU where its tiles are few: two share a CU at 2.6 us a tile of
   // each, one alone takes 1.7 to 2, and a part more costs 8 us and its partials
   // (32 sequences of 512, 32 new tokens each: 28 us uncut, 47 in halves; 1 of
   // 16128, 128 new: 89 us with a block per CU, 67 with two).
-  const int cus = cu_count();
-  const int64_t tiles = (((int64_t)a.width << a.c.shift) + PKT - 1) / PKT;
-  const int64_t blocks = kv8_row_tiles_most(a.tokens, a.seqs, a.group, 32 * NW) * a.c.heads;
-  a.plan = {cus, 24, blocks >= cus && tiles <= 24 ? 24 : 4, 2 * cus};
-  return kv8_launch<T, D, 32 * NW, PKT, true>(a, kv8_prompt_kernel<T, D, NW>, 64 * NW, s);
+  a.plan = {cus, 24, blocks(4) >= cus && tiles <= 24 ? 24 : 4, 2 * cus};
+  return kv8_launch<T, D, 128, PKT, true>(a, kv8_prompt_kernel<T, D, 4>, 256, s);
 }
 
 }  // namespace
