@@ -112,6 +112,8 @@ SHAPES = [
     ([64, 64], [64, 0], 16, 2, 64, 256),
     ([1024], [3700], 64, 8, 64, 256),                # 256 blocks of 256 rows
     ([515, 500], [4000, 3333], 32, 32, 128, 64),     # and rows that do not fill them
+    ([40, 1], [100, 33], 80, 1, 128, 64),            # more heads to one than a tile has rows
+    ([70, 33], [200, 0], 14, 2, 64, 32),             # seven heads to one
 ]
 
 

@@ -162,6 +162,12 @@ __device__ __forceinline__ void lds_copy16_at(const void* p, void* lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
 }
 
+// The same, 4 bytes a lane.
+__device__ __forceinline__ void lds_copy4_at(const void* p, void* lds) {
+  const uint32_t m0 = wave_uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+}
+
 // Inclusive sums over the lanes, by DPP within rows of 16 and two row broadcasts.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int scan_step(int v) {

@@ -51,8 +51,10 @@ struct WeighItem {
             &s, &place))
       return false;
     const Kv8Cut cut = kv8_cut(s, a.group, RT, KT);
-    const int n = parts(s, a.group, chunk), part = place % n;
-    head = place / n;
+    // heads first: blocks go to the XCDs in turn, so with 8 heads each L2 holds the
+    // queries of one
+    const int n = parts(s, a.group, chunk), part = place / a.c.heads;
+    head = place % a.c.heads;
     lo = (int)((int64_t)cut.key_tiles * part / n);
     hi = (int)((int64_t)cut.key_tiles * (part + 1) / n);
     rows = cut.rows;
@@ -171,8 +173,8 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
   typedef typename AttnOp<T>::vec vec;
   constexpr int RT = 64, KT = WKT * WNW, P = D / 32, CH = D / 8;
   constexpr int N = RT * CH / (64 * WNW);  // 16-byte pieces of a row tile a thread stages
-  __shared__ __align__(16) uint16_t qs[2][RT * D];
-  __shared__ float ls[2][RT];
+  __shared__ __align__(16) uint16_t qs[3][RT * D];
+  __shared__ __align__(16) float ls[3][RT];
   if (blockIdx.x == 0)
     kv8_report_lengths(a.lengths, a.seqs, a.width << a.c.shift, a.fault);
   WeighItem<RT, KT> it;
@@ -182,51 +184,46 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
   const Kv8Seq s = it.s;
   const int past = s.len - s.n;
   float* out = wt.w + it.seq * wt.sb + it.head * wt.sh;
-  // A row tile goes from global memory straight to LDS, 16 bytes a lane: this
-  // thread copies a piece of rows tid / CH + n RPI, the one that belongs at place
-  // tid % CH of its rows (the XOR swizzle repeats with the rows of a wave's
-  // copies).  Pointers advance from tile to tile (a division per row and tile
-  // would cost more than the products); rows past the last one read the last one.
+  // A tile of up to RT rows is whole tokens' heads, or RT heads of one token where
+  // the group has more: its rows lie at the same offsets from its first one in
+  // every tile, so a lane's addresses cost one addition a tile.
+  const int hp = min(group, RT), tp = RT / hp;
+  struct RowTile {
+    int t, g;  // first token and first head of the group
+  };
+  auto next = [&](RowTile& x) __attribute__((always_inline)) {
+    x.g += RT;
+    if (x.g >= group) x = {x.t + tp, 0};
+  };
+  auto count = [&](const RowTile& x) __attribute__((always_inline)) {
+    return min(tp, s.n - x.t) * min(hp, group - x.g);
+  };
+  // It goes from global memory straight to LDS, 16 bytes a lane: this thread copies
+  // a piece of rows tid / CH + n RPI, the one that belongs at place tid % CH of its
+  // rows (the XOR swizzle repeats with the rows of a wave's copies).  Rows past the
+  // last one read the first one.
   constexpr int RPI = 64 * WNW / CH;
   const int piece = 8 * (tid % CH ^ swz_k_of<D>(tid / CH & 31));
-  struct RowAt {
-    int64_t at;  // offset of the row's token and head
-    int g;       // its head in the group
-  };
-  const int step_t = RT / group, step_g = RT % group;
-  auto row_at = [&](int row, int64_t st, int64_t sh) __attribute__((always_inline)) {
-    return RowAt{(s.first + row / group) * st + (it.head * group + row % group) * sh, row % group};
-  };
-  auto advance = [&](RowAt& x, int64_t st, int64_t sh) __attribute__((always_inline)) {
-    x.at += step_t * st + step_g * sh;
-    if (step_g != 0) {
-      x.g += step_g;
-      if (x.g >= group) {
-        x.g -= group;
-        x.at += st - group * sh;
-      }
-    }
-  };
-  const int64_t q_last = row_at(it.rows - 1, a.q_st, a.q_sh).at;
-  const int64_t l_last = row_at(it.rows - 1, a.lse_st, a.lse_sh).at;
-  RowAt q_at[N], l_at;
-  float lr = 0.f;
-  auto begin = [&](int r0) __attribute__((always_inline)) {
+  const uint16_t* q_at[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) q_at[n] = row_at(r0 + tid / CH + n * RPI, a.q_st, a.q_sh);
-    l_at = row_at(r0 + lane, a.lse_st, a.lse_sh);
-  };
-  auto copy = [&](int r0, int buf) __attribute__((always_inline)) {  // tiles in order after begin()
+  for (int n = 0; n < N; ++n) {
+    const int i = tid / CH + n * RPI;
+    q_at[n] = a.q + (i / hp) * a.q_st + (i % hp) * a.q_sh + piece;
+  }
+  const float* l_at = a.lse + (lane / hp) * a.lse_st + (lane % hp) * a.lse_sh;
+  auto copy = [&](const RowTile& x, int buf) __attribute__((always_inline)) {
+    const int64_t token = s.first + x.t, h = it.head * group + x.g;
+    const int64_t at = token * a.q_st + h * a.q_sh;
+    const int rows = count(x);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      int64_t at = q_at[n].at;
-      if (r0 + RT > it.rows && r0 + tid / CH + n * RPI >= it.rows) at = q_last;
-      lds_copy16_at(a.q + at + piece, qs[buf] + (wave * 64 + n * 64 * WNW) * 8);
-      advance(q_at[n], a.q_st, a.q_sh);
+      const uint16_t* from = q_at[n];
+      if (rows < RT && tid / CH + n * RPI >= rows) from = a.q + piece;
+      lds_copy16_at(from + at, qs[buf] + (wave * 64 + n * 64 * WNW) * 8);
     }
     if (wave == 0) {  // RT == 64: a lane each
-      lr = a.lse[r0 + lane < it.rows ? l_at.at : l_last] * 1.4426950408889634f;
-      advance(l_at, a.lse_st, a.lse_sh);
+      const float* from = rows < RT && lane >= rows ? a.lse : l_at;
+      lds_copy4_at(from + token * a.lse_st + h * a.lse_sh, ls[buf]);
     }
   };
 
@@ -241,25 +238,35 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
       kf[2 * p] = fp8x8_to<T>(x[0], x[1]);
       kf[2 * p + 1] = fp8x8_to<T>(x[2], x[3]);
     }
+    // the lane's own weight: one read and one write, not one for each product
+    const int mine = key0 + 8 * (col >> 2) + 4 * half + (col & 3);
+    const bool owner = col < 16 && mine < s.len && (col < 8 ? keys.ok[0] : keys.ok[1]);
+    const float before = owner ? out[mine] : 0.f;
     f32x16 sum = f32x16{};
-    // rows before `first` see none of the block's keys, from `full` on all of
-    // the wave's
-    const int first = max(0, j * KT - past) * group / RT * RT;
-    const int full = first_row(s, key0 + WKT - 1, group);
+    // the block's first key is seen from its own token on, all keys of the wave by
+    // the tokens from `full` on
+    RowTile now = {max(0, j * KT - past) / tp * tp, 0}, ahead = now;
+    const int full = key0 + WKT - 1 - past;
     __syncthreads();  // the buffers' last readers
-    begin(first);
-    copy(first, 0);
-    int buf = 0;
-    for (int r0 = first; r0 < it.rows; r0 += RT, buf ^= 1) {
-      if (wave == 0) ls[buf][lane] = lr;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies of the tile
+    copy(ahead, 0);
+    next(ahead);
+    if (ahead.t < s.n) copy(ahead, 1);
+    for (int buf = 0; now.t < s.n; next(now), buf = buf == 2 ? 0 : buf + 1) {
+      // this wave's copies of the tile, with those of the next one still on the way
+      if (ahead.t >= s.n) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else if (wave == 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N + 1) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
       __syncthreads();
-      if (r0 + RT < it.rows) copy(r0 + RT, buf ^ 1);
+      if (ahead.t < s.n) next(ahead);
+      if (ahead.t < s.n) copy(ahead, buf == 0 ? 2 : buf - 1);
       if (key0 >= s.len) continue;
+      const int rows = count(now);
 #pragma unroll
       for (int u = 0; u < RT / 32; ++u) {
-        const uint16_t* q = qs[buf] + (32 * u + col) * D;
-        const float lse = ls[buf][32 * u + col];
+        const int row = 32 * u + col;
+        const uint16_t* q = qs[buf] + row * D;
+        // a row that is none weighs nothing
+        const float lse = row < rows ? ls[buf][row] * 1.4426950408889634f : INFINITY;
         f32x16 x = f32x16{};
 #pragma unroll
         for (int p = 0; p < P; ++p) {
@@ -271,22 +278,18 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], keys.sc[r >> 3], -lse));
-        const int row = r0 + 32 * u;
-        if (row >= full && row + 32 <= it.rows) {
+        if (now.t >= full) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) sum[r] += x[r];
         } else {
-          int base = key0 + 4 * half;
-          asm volatile("" : "+v"(base));  // nothing of this branch waits in registers outside it
+          // how many of the lane's keys, from its first one on, the row's token sees
+          const int seen = past + now.t + row / hp - (key0 + 4 * half);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = base + 8 * (r >> 2) + (r & 3);
-            const bool sees = row + col < it.rows && row + col >= first_row(s, key, group);
-            sum[r] += sees ? x[r] : 0.f;
-          }
+          for (int r = 0; r < 16; ++r) sum[r] += 8 * (r >> 2) + (r & 3) <= seen ? x[r] : 0.f;
         }
       }
     }
+    float got = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float v = sum[r];
@@ -295,9 +298,9 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
       v += dpp_f32<0x141>(v);
       v += dpp_f32<0x140>(v);
       v = row_sum(v);
-      const int key = key0 + 8 * (r >> 2) + 4 * half + (r & 3);
-      if (col == r && key < s.len && keys.ok[r >> 3]) out[key] += v;
+      got = col == r ? v : got;
     }
+    if (owner) out[mine] = before + got;
   }
 }
 
