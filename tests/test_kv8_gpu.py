@@ -131,6 +131,31 @@ def test_append_and_attention(new, past, h, hk, d, page, dtype):
     check_attention(s, out, lse)
 
 
+def wide_table(rows, heads, page):
+    """Columns of a block table with which a call of few tokens counts as one of
+    prompts (rows: new tokens x heads of a group, over 64 a sequence)."""
+    return (1 << 23) // (rows * heads * page) + 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("new,past,h,hk,d,page", [
+    ([17, 40], [0, 100], 16, 4, 128, 32),
+    ([33, 130, 1], [70, 0, 500], 8, 2, 128, 64),
+    ([257], [129], 24, 8, 64, 64),
+    ([300, 5], [1500, 2000], 8, 8, 128, 16),
+    ([300, 0, 70], [100, 700, 1], 14, 2, 64, 16),  # seven heads to one, a sequence without new tokens
+    ([600], [0], 3, 1, 128, 128),
+    ([40, 1], [100, 33], 80, 1, 128, 64),
+    ([1, 90, 64], [300, 0, 64], 16, 2, 64, 256),
+    ([3] * 67, [5 * i for i in range(67)], 23, 1, 64, 16),  # more than a wave of sequences
+])
+def test_prompts_of_few_tokens(new, past, h, hk, d, page, dtype):
+    s = Setup(new, past, h, hk, d, page, dtype, seed=len(new) + h,
+              width=wide_table(sum(new) * h // hk, hk, page)).fill()
+    out, lse = eff.kv8_attention(s.q.to("gcu"), s.gcu(), *s.index())
+    check_attention(s, out, lse)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("new,past,h,hk,d,page", SHAPES)
 def test_weigh(new, past, h, hk, d, page, dtype):
@@ -261,10 +286,11 @@ def test_tokens_one_by_one_as_together():
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_non_finite_tokens_reach_only_who_sees_them(bad, dtype):
+@pytest.mark.parametrize("wide", [False, True])
+def test_non_finite_tokens_reach_only_who_sees_them(bad, dtype, wide):
     """Token 50 of 70 has a bad key, token 60 a bad value element: the queries
     before them stay what they were, those after are NaN."""
-    s = Setup([70, 1], [0, 40], 4, 2, 128, 32, dtype, seed=2)
+    s = Setup([70, 1], [0, 40], 4, 2, 128, 32, dtype, seed=2, width=wide_table(142, 2, 32) if wide else 0)
     s.k[50, 1, 3], s.v[60, 0, 100] = bad, bad
     cache, index = s.gcu(), s.index()
     eff.kv8_append(s.k.to("gcu"), s.v.to("gcu"), cache, *index)
@@ -306,6 +332,71 @@ def test_queries_without_keys_and_rows_of_no_sequence():
     assert torch.allclose(w.cpu().double(), want, rtol=1e-4, atol=1e-6)
 
 
+@pytest.mark.parametrize("new,width", [(1, 40), (200, 40), (200, 2000)])
+def test_scales_of_pages_that_are_not_there(new, width):
+    """Table entries behind a sequence's last page name none; page 0, whose
+    scales are NaN, is not the sequence's and must not come in for them."""
+    s = Setup([new], [33], 8, 2, 64, 16, width=width, seed=3)
+    at = s.table[0].index(0) if 0 in s.table[0] else None
+    if at is not None:  # page 0 to the free ones
+        s.table[0][at] = s.free.pop()
+    s.cache = tuple(torch.full_like(t, 0x7F if t.dtype == torch.uint8 else math.nan) for t in s.cache)
+    old = torch.randn(2, 33, 2, 64, generator=gen(4)).to(s.dtype)
+    oracle.append(s.cache, old[0], old[1], s.table, [33], [0, 33])
+    s.fill()
+    assert s.cache[2][0].isnan().all() and s.cache[3][0].isnan().all()
+    out, lse = eff.kv8_attention(s.q.to("gcu"), s.gcu(), *s.index())
+    check_attention(s, out, lse)
+    w = torch.zeros(1, 2, s.width * 16).to("gcu")
+    eff.kv8_weigh_(w, s.q.to("gcu"), lse, s.gcu(), *s.index())
+    assert w.isfinite().all().item()
+
+
+def test_prompts_without_keys_bad_pages_and_starts():
+    """The same of a call of prompts: tokens before position 0, rows of no
+    sequence, a page outside the pool, lengths and starts out of range."""
+    s = Setup([200, 130], [0, 20], 4, 2, 64, 16, pad=5, seed=4, width=wide_table(670, 2, 16)).fill()
+    s.lens[0] = 150  # tokens 0 .. 49 of sequence 0 come before position 0
+    cache, index = s.gcu(), s.index()
+    out, lse = eff.kv8_attention(s.q.to("gcu"), cache, *index)
+    for empty in (slice(0, 50), slice(330, 335)):
+        assert (out[empty] == 0).all().item() and (lse[empty] == -math.inf).all().item()
+    check_attention(s, out, lse)
+    w = torch.zeros(2, 2, s.width * 16).to("gcu")
+    eff.kv8_weigh_(w, s.q.to("gcu"), lse, cache, *index)
+    want = torch.zeros(2, 2, s.width * 16, dtype=torch.float64)
+    oracle.attention(s.q, s.cache, s.table, s.lens, s.starts, s.d ** -0.5, want, lse.cpu())
+    assert torch.allclose(w.cpu().double(), want, rtol=1e-4, atol=1e-6)
+    torch.gcu.synchronize()
+
+    bad = [list(t) for t in s.table]
+    bad[1][2] = s.pages
+    index[0] = s.index(table=bad)[0]
+    got, log = eff.kv8_attention(s.q.to("gcu"), cache, *index)
+    with pytest.raises(IndexError, match=f"index {s.pages} is out of bounds"):
+        torch.gcu.synchronize()
+    assert torch.equal(got[:200].cpu(), out[:200].cpu()) and torch.equal(log[:200].cpu(), lse[:200].cpu())
+    assert got.cpu().isfinite().all()
+    # as if the page's 16 positions did not exist
+    keys = oracle.tokens(s.cache[0][:, 0], s.cache[2][:, 0], s.table[1], s.lens[1])
+    scores = torch.cat([keys[:32], keys[48:]]) @ s.q[329, 0].double() * s.d ** -0.5
+    assert abs(float(log[329, 0]) - float(scores.logsumexp(0))) < 1e-4
+    index = s.index(lens=[s.lens[0], -7])
+    got, log = eff.kv8_attention(s.q.to("gcu"), cache, *index)
+    with pytest.raises(IndexError, match="index -7 is out of bounds"):
+        torch.gcu.synchronize()
+    assert torch.equal(got[:200].cpu(), out[:200].cpu())
+    assert (got[200:] == 0).all().item() and (log[200:] == -math.inf).all().item()
+    index = s.index()
+    for starts in ([5, 2, 335], [0, 1000, 8], [-3, 4, 2 ** 31 - 1], [335, 335, 0], [0, 335, -2 ** 31]):
+        index[2] = torch.tensor(starts, dtype=torch.int32).to("gcu")
+        got, log = eff.kv8_attention(s.q.to("gcu"), cache, *index)
+        torch.gcu.synchronize()
+        assert got.shape == s.q.shape
+        eff.kv8_weigh_(w, s.q.to("gcu"), log, cache, *index)
+        torch.gcu.synchronize()
+
+
 def test_no_sequences_and_no_tokens():
     cache = eff.kv8_cache(2, 2, 64, 16)
     none = torch.zeros(0, dtype=torch.int32).to("gcu")
@@ -345,19 +436,20 @@ def test_strided_inputs_and_cache():
     assert torch.equal(eff.kv8_attention(odd, cache, *index)[0].cpu(), out.cpu())
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("scale", [0.3, 0.0, -0.2])
-def test_scales(scale):
-    s = Setup([1, 40], [300, 100], 8, 2, 64, 16, seed=7).fill()
+def test_scales(scale, wide):
+    s = Setup([1, 40], [300, 100], 8, 2, 64, 16, seed=7, width=wide_table(164, 2, 16) if wide else 0).fill()
     out, lse = torch.ops.torch_gcu.kv8_attention(s.q.to("gcu"), *s.gcu(), *s.index(), scale)
     check_attention(s, out, lse, scale)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
-@pytest.mark.parametrize("new", [1, 40])
-def test_blocks_of_very_different_scales(new, dtype):
+@pytest.mark.parametrize("new,wide", [(1, False), (40, False), (40, True)])
+def test_blocks_of_very_different_scales(new, wide, dtype):
     """Values of 2^-20 in most pages, of 1 in one that the softmax hardly sees, then
     of 2^9: sums stay relative to what they hold."""
-    s = Setup([new], [400], 4, 2, 128, 16, dtype, seed=8).fill()
+    s = Setup([new], [400], 4, 2, 128, 16, dtype, seed=8, width=wide_table(80, 2, 16) if wide else 0).fill()
     for i, p in enumerate(s.table[0]):
         s.cache[3][p] *= 2.0 ** (-20 if i < 12 else -6 if i < 20 else 9 if i == 22 else -20)
         s.cache[2][p] *= 2.0 ** (i % 3)

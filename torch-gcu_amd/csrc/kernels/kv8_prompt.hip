@@ -125,7 +125,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   auto store = [&](int buf) __attribute__((always_inline)) {
     if (tid < 4) {
       const float k = scale * s_k;
-      scales[buf][tid] = k < 0x1p-100f ? 0x1p-100f : k;  // masked scores stay -inf when multiplied by it
+      // masked scores stay -inf when multiplied by it
+      scales[buf][tid] = !s_ok || k < 0x1p-100f ? 0x1p-100f : k;
       scales[buf][4 + tid] = s_ok ? s_v : 0.f;
       const uint64_t gone = __ballot(!s_ok);
       if (tid == 0) absent[buf] = (int)gone;
