@@ -67,6 +67,8 @@ REFUSED = [
     (ALL, "k_cache", lambda t: torch.zeros(3, 2, 64, 16, dtype=torch.uint8).transpose(2, 3), INVALID, "dense"),
     (ALL, "k_cache", lambda t: torch.zeros(3 * 2 * 16 * 64 + 1, dtype=torch.uint8)[1:].view(t.shape), INVALID, "aligned"),
     (ALL, "k_cache", lambda t: t[:1].expand(3, 2, 16, 64), INVALID, "overlap"),
+    (ALL, "k_cache", lambda t: t.as_strided(t.shape, (16 * 64, 16 * 64, 64, 1)), INVALID, "overlap"),
+    (ALL, "k_scale", lambda t: t.as_strided((3, 2), (1, 1)), INVALID, "overlap"),
     (ALL, "k_scale", lambda t: t.double(), INVALID, "float32"),
     (ALL, "v_scale", lambda t: t[:, :1], INVALID, "float32 [pages, heads]"),
     (ALL, "k_scale", lambda t: t[:1].expand(3, 2), INVALID, "overlap"),
@@ -95,6 +97,10 @@ REFUSED = [
     (("weigh", "evict"), "weights", lambda t: t[..., :31].contiguous(), INVALID, "positions"),
     (("weigh", "evict"), "weights", lambda t: t.double(), INVALID, "float32"),
     (("weigh", "evict"), "weights", lambda t: t[:, :1].expand(2, 2, 32), INVALID, "overlap"),
+    (("weigh", "evict"), "weights", lambda t: t.as_strided((2, 2, 32), (32, 32, 1)), INVALID, "overlap"),
+    (("attention",), "out", lambda t: t[:1].expand(t.shape), INVALID, "overlap"),
+    (("attention",), "lse", lambda t: t.as_strided(t.shape, (1, 1)), INVALID, "overlap"),
+    (("evict",), "kept", lambda t: t.as_strided(t.shape, (5, 5, 1)), INVALID, "kept"),
     (("evict",), "keep", lambda n: 0, INVALID, "keep"),
     (("evict",), "recent", lambda n: 5, INVALID, "keep"),
     (("evict",), "sink", lambda n: -1, INVALID, "keep"),
@@ -125,6 +131,20 @@ def test_head_dims_that_have_no_kernel(op, d, status):
 def test_page_sizes(op, page):
     st, message = run(op, call(page=page))
     assert st == INVALID and "page size" in message
+
+
+@pytest.mark.parametrize("ops,one,other,words", [
+    (("append", "evict"), "v_cache", "k_cache", "same memory"),
+    (("append", "evict"), "v_scale", "k_scale", "same memory"),
+    (("evict",), "new_lengths", "lengths", "of their own"),
+    (("evict",), "new_weights", "weights", "of their own"),
+])
+def test_what_is_written_has_memory_of_its_own(ops, one, other, words):
+    for op in ops:
+        a = call()
+        a[one] = a[other]
+        st, message = run(op, a)
+        assert st == INVALID and words in message, (op, st, message)
 
 
 def test_null_cache():

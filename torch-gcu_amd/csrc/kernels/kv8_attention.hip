@@ -362,6 +362,9 @@ extern "C" mi_status_t mi_kv8_attention(const mi_tensor_t* out, const mi_tensor_
   if (out->strides[2] != 1 || out->strides[0] % 8 != 0 || out->strides[1] % 8 != 0 ||
       (uintptr_t)out->data % 16 != 0)
     MI_FAIL(MI_ERR_UNSUPPORTED, "%s: rows of out must be dense and 16-byte aligned", op);
+  MI_CHECK_ARG(kv8_apart(out->sizes[0], out->strides[0], out->sizes[1], out->strides[1], dim) &&
+                   kv8_apart(lse->sizes[0], lse->strides[0], lse->sizes[1], lse->strides[1], 1),
+               "%s: rows of out or lse overlap", op);
   MI_RETURN_IF(kv8_check_seqs(op, block_table, lengths, starts, q->sizes[0], &a));
   MI_CHECK_ARG(std::isfinite(scale), "%s: scale is not finite", op);
   if (a.tokens == 0) return MI_OK;

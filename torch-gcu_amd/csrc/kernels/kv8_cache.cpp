@@ -1,5 +1,7 @@
 // Checks that the entry points of the 8-bit key/value cache share.  They read
 // descriptors only and run before any device call.
+#include <utility>
+
 #include "kv8_common.h"
 
 namespace mi {
@@ -15,6 +17,17 @@ mi_status_t check_ints(const char* op, const mi_tensor_t* t, const char* name, i
   return MI_OK;
 }
 }  // namespace
+
+bool kv8_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t extent) {
+  if (n0 <= 1 && n1 <= 1) return true;
+  if (n0 <= 1) return s1 >= extent;
+  if (n1 <= 1) return s0 >= extent;
+  if (s0 < s1) {
+    std::swap(n0, n1);
+    std::swap(s0, s1);
+  }
+  return s1 >= extent && s0 >= (__int128)(n1 - 1) * s1 + extent;
+}
 
 mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cache* c,
                             int64_t* dim) {
@@ -48,10 +61,8 @@ mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cach
                      t.strides[0] % 16 == 0 && (uintptr_t)t.data % 16 == 0,
                  "%s: a page's head in %s_cache must be dense and 16-byte aligned", op, n);
     // a page or head that shares memory with another would be written twice
-    MI_CHECK_ARG((t.sizes[1] == 1 || t.strides[1] >= p * t.sizes[3]) &&
-                     (t.sizes[0] == 1 || t.strides[0] >= p * t.sizes[3]) &&
-                     (s.sizes[1] == 1 || s.strides[1] >= 1) &&
-                     (s.sizes[0] == 1 || s.strides[0] >= 1),
+    MI_CHECK_ARG(kv8_apart(t.sizes[0], t.strides[0], t.sizes[1], t.strides[1], p * t.sizes[3]) &&
+                     kv8_apart(s.sizes[0], s.strides[0], s.sizes[1], s.strides[1], 1),
                  "%s: pages or heads of the %s cache overlap", op, n);
     MI_CHECK_ARG(t.sizes[0] <= 0x7fffffff && t.sizes[1] <= 65535, "%s: too many pages or heads", op);
   }
@@ -72,6 +83,12 @@ mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cach
   c->shift = 0;
   while ((1 << c->shift) < k->sizes[2]) ++c->shift;
   *dim = k->sizes[3];
+  return MI_OK;
+}
+
+mi_status_t kv8_check_written(const char* op, const Kv8Cache& c) {
+  MI_CHECK_ARG(c.k != c.v && c.k_scale != c.v_scale, "%s: k and v of the cache are the same memory",
+               op);
   return MI_OK;
 }
 
@@ -125,6 +142,16 @@ mi_status_t kv8_check_seqs(const char* op, const mi_tensor_t* table, const mi_te
   return MI_OK;
 }
 
+mi_status_t kv8_check_kept(const char* op, const mi_tensor_t* kept, int64_t keep, const Kv8Args& a) {
+  MI_RETURN_IF(validate(kept, "kept"));
+  MI_CHECK_ARG(kept->dtype == MI_I32 && kept->ndim == 3 && kept->sizes[0] == a.seqs &&
+                   kept->sizes[1] == a.c.heads && kept->sizes[2] == keep &&
+                   (keep == 1 || kept->strides[2] == 1) &&
+                   kv8_apart(kept->sizes[0], kept->strides[0], kept->sizes[1], kept->strides[1], keep),
+               "%s: kept must be int32 [sequences, heads, keep] with dense rows of their own", op);
+  return MI_OK;
+}
+
 mi_status_t kv8_check_weights(const char* op, const mi_tensor_t* w, const char* name,
                               const Kv8Args& a) {
   MI_RETURN_IF(validate(w, name));
@@ -136,8 +163,7 @@ mi_status_t kv8_check_weights(const char* op, const mi_tensor_t* w, const char* 
                op, name, (long long)cap);
   if (w->sizes[2] > 0x7fffffff) MI_FAIL(MI_ERR_TOO_LARGE, "%s: %s has too many positions", op, name);
   // rows that share memory would be added to twice
-  MI_CHECK_ARG((w->sizes[0] <= 1 || w->strides[0] >= w->sizes[2]) &&
-                   (w->sizes[1] <= 1 || w->strides[1] >= w->sizes[2]),
+  MI_CHECK_ARG(kv8_apart(w->sizes[0], w->strides[0], w->sizes[1], w->strides[1], w->sizes[2]),
                "%s: rows of %s overlap", op, name);
   return MI_OK;
 }

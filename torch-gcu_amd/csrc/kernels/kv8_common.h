@@ -293,11 +293,18 @@ __device__ __forceinline__ void kv8_rest(const Kv8Args& a) {
 
 // Host side (kv8_cache.cpp): the cache's own checks, and the tensors that say
 // which sequences a call is about.
+// Whether rows of `extent` elements, n0 x n1 of them at strides s0 and s1, lie one
+// after the other with either index as the outer one.
+bool kv8_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t extent);
 mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cache* c, int64_t* dim);
+// for calls that write it
+mi_status_t kv8_check_written(const char* op, const Kv8Cache& c);
 mi_status_t kv8_check_queries(const char* op, const mi_tensor_t* q, const mi_tensor_t* lse,
                               int64_t dim, Kv8Args* a);
 mi_status_t kv8_check_seqs(const char* op, const mi_tensor_t* table, const mi_tensor_t* lengths,
                            const mi_tensor_t* starts, int64_t tokens, Kv8Args* a);
+// int32 [sequences, heads, keep], dense rows
+mi_status_t kv8_check_kept(const char* op, const mi_tensor_t* kept, int64_t keep, const Kv8Args& a);
 // Attention of many query rows per sequence (kv8_prompt.hip).
 mi_status_t kv8_prompt(Kv8Args& a, int64_t dim, bool f16, hipStream_t s);
 // float32 [sequences, heads, at least the table's positions], dense rows

@@ -270,6 +270,7 @@ extern "C" mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor
   int64_t dim = 0;
   a.group = 1;
   MI_RETURN_IF(kv8_check_cache(op, cache, &a.c, &dim));
+  MI_RETURN_IF(kv8_check_written(op, a.c));
   MI_RETURN_IF(kv8_check_seqs(op, block_table, lengths, nullptr, 0, &a));
   MI_RETURN_IF(kv8_check_weights(op, weights, "weights", a));
   MI_RETURN_IF(kv8_check_weights(op, new_weights, "new_weights", a));
@@ -285,18 +286,16 @@ extern "C" mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor
                    (new_table->sizes[1] <= 1 || new_table->strides[1] == 1),
                "%s: new_table must be int32 [sequences, at least %lld pages] with dense rows", op,
                (long long)pages);
-  MI_RETURN_IF(validate(kept, "kept"));
-  MI_CHECK_ARG(kept->dtype == MI_I32 && kept->ndim == 3 && kept->sizes[0] == a.seqs &&
-                   kept->sizes[1] == a.c.heads && kept->sizes[2] == keep &&
-                   (keep == 1 || kept->strides[2] == 1) &&
-                   (a.seqs <= 1 || kept->strides[0] >= keep) &&
-                   (a.c.heads <= 1 || kept->strides[1] >= keep),
-               "%s: kept must be int32 [sequences, heads, keep] with dense rows of their own", op);
+  MI_RETURN_IF(kv8_check_kept(op, kept, keep, a));
   MI_RETURN_IF(validate(new_lengths, "new_lengths"));
   MI_CHECK_ARG(new_lengths->dtype == MI_I32 && new_lengths->ndim == 1 &&
                    new_lengths->sizes[0] == a.seqs &&
                    (a.seqs <= 1 || new_lengths->strides[0] == 1),
                "%s: new_lengths must be a dense int32 vector of the sequences", op);
+  // blocks read the old ones while others write
+  MI_CHECK_ARG(a.seqs == 0 || (new_lengths->data != lengths->data &&
+                               new_weights->data != weights->data),
+               "%s: new_lengths and new_weights need memory of their own", op);
   if (a.seqs > 32767) MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 32767 sequences", op);
   if (a.seqs == 0) return MI_OK;
   e.w = (const float*)weights->data;
