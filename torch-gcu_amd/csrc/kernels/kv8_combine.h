@@ -96,7 +96,8 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
   }
 }
 
-// Room for the partials of a call whose parts are planned by a.plan, then the attention kernel and, where anything can have been cut,
+// Room for the partials of a call whose parts are planned by a.plan, then the
+// attention kernel and, where anything can have been cut,
 // the merge.
 template <typename T, int D, int RT, int KT, bool LAST_FIRST, typename K>
 mi_status_t kv8_launch(Kv8Args& a, K kernel, int threads, hipStream_t s) {

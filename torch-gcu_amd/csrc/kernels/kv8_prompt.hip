@@ -356,8 +356,9 @@ mi_status_t run_prompt(Kv8Args& a, hipStream_t s) {
   // A block per CU where its tiles are few: two share a CU at 2.6 us a tile of
   // each, one alone takes 1.7 to 2, and a part more costs 8 us and its partials
   // (32 sequences of 512, 32 new tokens each: 28 us uncut, 47 in halves; 1 of
-  // 16128, 128 new: 89 us with a block per CU, 67 with two).
-  a.plan = {cus, 24, blocks(4) >= cus && tiles <= 24 ? 24 : 4, 2 * cus};
+  // 16128, 128 new: 89 us with a block per CU, 67 with two; 16 heads of 64, 4 x up to
+  // 1024 tokens behind 1000: 47 us uncut, 67 in parts).
+  a.plan = {cus, 24, blocks(4) >= cus && tiles <= 32 ? 32 : 4, 2 * cus};
   return kv8_launch<T, D, 128, PKT, true>(a, kv8_prompt_kernel<T, D, 4>, 256, s);
 }
 
