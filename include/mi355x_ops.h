@@ -558,10 +558,11 @@ mi_status_t mi_kv8_weigh(const mi_tensor_t* weights, const mi_tensor_t* q,
 /* Keeps min(keep, lengths[b]) tokens per sequence and head: the first `sink`,
  * the last `recent`, and the others of largest weight (ties: the lower
  * position; NaN counts as no weight), in their order.  They are written to the
- * pages of new_table (int32 [B, >= ceil(keep / page)]), which no block_table
- * row of the call may name; the old pages stay as they were.  kept int32
- * [B, heads, keep] the old positions, then -1; new_lengths int32 [B];
- * new_weights like weights, the kept ones, then 0. */
+ * pages of new_table (int32 [B, >= ceil(keep / page)]), none named twice and
+ * none by a block_table row of the call; the old pages stay as they were.  kept
+ * int32 [B, heads, keep] the old positions, then -1; new_lengths int32 [B];
+ * new_weights like weights, the kept ones, then 0; the last two in memory of
+ * their own. */
 mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor_t* weights,
                          const mi_tensor_t* block_table, const mi_tensor_t* new_table,
                          const mi_tensor_t* lengths, int64_t keep, int64_t recent,

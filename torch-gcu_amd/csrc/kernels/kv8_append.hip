@@ -10,7 +10,9 @@
 // What bounds it: a prompt's bytes (16-bit tokens read, codes written), a
 // decode step's chain of dependent reads (starts, table, token, scale).  One
 // thread block per touched page and head owns that page's scale, so nothing
-// is shared between blocks.
+// is shared between blocks.  8 heads of 128: 11137 tokens of four sequences 18.8
+// us (68 MB, 3.6 TB/s where a large copy reaches 5.0: the chain, and tokens read
+// a second time from the caches), 8 tokens of as many 4.4 us.
 //
 // A token with an infinite or NaN element has NaN codes for its whole key, so
 // that every query that sees it gets NaN, and 0 in place of the bad elements

@@ -2,8 +2,11 @@
 // cache.
 //
 // What bounds it: 4 D flops per query row and key on the matrix instructions,
-// and beside them about as much time of exp2, maxima and sums on the vector
-// unit.  A block takes 32 NW query rows of one k/v head (the group's heads of
+// and beside them more time of exp2, maxima and sums on the vector unit.  32 query
+// heads on 8 of 128: 2048 tokens behind 14000 550 us (916 TFLOP/s where a large
+// product reaches 1426; matrix instructions 37 % of the cycles), 2783 tokens of
+// four sequences behind 359 to 823 86 us (500: 704 blocks on 512 places).
+//   A block takes 32 NW query rows of one k/v head (the group's heads of
 // consecutive tokens), a wave 32 of them, and walks the keys in tiles of 64:
 //   S^T = K Q^T, O^T = V^T P^T (v_mfma_f32_32x32x16), P^T taken from the S^T
 //   accumulators as they stand.

@@ -103,7 +103,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor,
                   scale: Optional[float] = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of new tokens' queries [tokens, heads, head_dim] over the cache,
     each up to its own position (append first): (out, logsumexp float32 [tokens,
-    heads]).  scale defaults to head_dim ** -0.5.  Tokens of no sequence, and
+    heads]), without gradients.  scale defaults to head_dim ** -0.5.  Tokens of no sequence, and
     tokens that see nothing, get 0 and -inf."""
     return torch.ops.torch_gcu.kv8_attention(q, *cache, block_table, lengths, starts, scale)
 
@@ -124,7 +124,7 @@ def kv8_evict(cache: KV8Cache, weights: torch.Tensor, block_table: torch.Tensor,
     """Cut every sequence to `keep` tokens per k/v head: the first `sink`, the
     last `recent` and the others of largest weight (ties: the lower position),
     moved in their order to the pages of new_table (int32 [sequences, ceil(keep /
-    page) or more]), which must not be pages of block_table.  Returns the kept
+    page) or more]), none named twice and none in block_table.  Returns the kept
     positions int32 [sequences, heads, keep] (then -1), the new lengths and the
     kept tokens' weights (shape of weights, then 0).  The old pages are the
     caller's again; queries keep using their true positions for RoPE."""
