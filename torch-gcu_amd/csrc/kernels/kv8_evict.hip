@@ -12,8 +12,8 @@
 // subnormal under a larger scale (half a step of 2^-9 of the new scale).  What
 // bounds the pair: the latency of the selection's passes for few sequences, the
 // gathered bytes for many.  8 heads of 128: 16 sequences of 4000 to 16000 cut to
-// 2000 tokens, 20 us for the selection and 24 for the moves (131 MB, 5.4 TB/s);
-// 1 of 1000 cut to 250, 8.6 and 4.
+// 2000 tokens, 18 us for the selection and 24 for the moves (131 MB, 5.4 TB/s);
+// 1 of 1000 cut to 250, 8.2 and 4.
 #include <algorithm>
 
 #include "kv8_common.h"
@@ -35,6 +35,7 @@ struct Kv8Evict {
   int keep, recent, sink;
 };
 
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // Larger weight, larger integer; -0 as 0, NaN below every number but above 0,
@@ -81,21 +82,21 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
     if (held) return *(const u32x4*)(ranks + i);
     return u32x4{rank_at(i), rank_at(i + 1), rank_at(i + 2), rank_at(i + 3)};
   };
+  // all of a thread's loads in flight at once, and the histograms cleared meanwhile
+  float x[SELN / SELT];
   if (held && want > 0) {
-    // all of a thread's loads in flight at once
-    float x[SELN / SELT];
 #pragma unroll
-    for (int k = 0; k < SELN / SELT; ++k) {
-      const int i = k * SELT + tid;
-      x[k] = w[min(i, len - 1)];
-    }
+    for (int k = 0; k < SELN / SELT; ++k) x[k] = w[min(k * SELT + tid, len - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ((int*)hist)[i * SELT + tid] = 0;
+  if (held && want > 0) {
 #pragma unroll
     for (int k = 0; k < SELN / SELT; ++k) {
       const int i = k * SELT + tid;
       if (k * SELT < len) ranks[i] = i >= lo && i < hi ? rank_of(x[k]) : 0u;
     }
   }
-  for (int i = tid; i < 4 * 256 * 4; i += SELT) (&hist[0][0][0])[i] = 0;
   __syncthreads();
   uint32_t prefix = 0, mask = 0;
   int ties = want;  // how many of the candidates at the threshold stay
@@ -141,6 +142,11 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
     if (!cut) return i + 4 <= len ? 15 : i < len ? (1 << (len - i)) - 1 : 0;
     const u32x4 u = want > 0 && i < len ? ranks_at(i) : u32x4{};
     int r = 0;
+    if (want > 0 && wave_uniform(i) >= lo && wave_uniform(i) + 256 <= hi) {  // all of the wave's
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r |= (u[k] > prefix ? 1 << k : 0) | (u[k] == prefix ? 16 << k : 0);
+      return r;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const bool forced = i + k < lo || (i + k >= hi && i + k < len);
@@ -159,7 +165,8 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
     __syncthreads();
 #pragma unroll 1
     for (int k = 0; k < chunks; ++k) {
-      const int scan = wave_scan(packed(kinds(r0 + 4 * (k * SELT + tid))));
+      const int own = 4 * (k * SELT + tid), x = kinds(r0 + own), scan = wave_scan(packed(x));
+      *(i32x2*)(ranks + own) = i32x2{x, scan};  // in place of the lane's four ranks
       if (lane == 63) counts[k * (SELT / 64) + wave] = scan;
     }
     __syncthreads();
@@ -167,9 +174,10 @@ __global__ __launch_bounds__(SELT) void kv8_select_kernel(Kv8Args a, Kv8Evict e)
     const int all = __builtin_amdgcn_readlane(upto, 63);
 #pragma unroll 1
     for (int k = 0; k < chunks; ++k) {
-      const int i = r0 + 4 * (k * SELT + tid), x = kinds(i), n = packed(x);
-      const int before =
-          __builtin_amdgcn_readlane(upto - mine, k * (SELT / 64) + wave) + wave_scan(n) - n;
+      const int own = 4 * (k * SELT + tid), i = r0 + own;
+      const i32x2 got = *(const i32x2*)(ranks + own);
+      const int x = got[0], n = packed(x);
+      const int before = __builtin_amdgcn_readlane(upto - mine, k * (SELT / 64) + wave) + got[1] - n;
       // ties before this position, of which those under `ties` stay
       int tie_at = tied + (int)((uint32_t)before >> 16);
       int at = done + (before & 0xffff) + min(tie_at, ties) - min(tied, ties);
