@@ -257,6 +257,21 @@ int main() {
     }
     assert(items <= plan.many + heads * kv8_row_tiles_most(tokens, seqs, group, rt));
     assert(touched <= kv8_touched_most(tokens, seqs, 4));
+    // rounds hold each tile of each sequence once, the farthest-seeing ones first
+    int longest = 0;
+    for (int b = 0; b < seqs; ++b) if (all[b].n > 0 && all[b].len > longest) longest = all[b].len;
+    for (int b = 0; b < seqs && b < 64; ++b) {
+      const Kv8Cut c = kv8_cut(all[b], group, rt, kt);
+      const Kv8Rounds r(all[b], c, longest, group, rt);
+      assert(r.off >= 0 && r.tiles == c.row_tiles && !r.in(-1) && r.before(0) == 0);
+      int seen = 0;
+      for (int k = r.off > 3 ? r.off - 3 : 0; k < r.off + r.tiles + 3; ++k) {
+        assert(r.before(k) == seen);
+        seen += r.in(k);
+        if (r.in(k)) assert(k - r.off >= 0 && k - r.off < c.row_tiles);
+      }
+      assert(seen == c.row_tiles);
+    }
   }
   for (unsigned u = 0; u < 0x7f800000u; u += 12345) {
     float x;

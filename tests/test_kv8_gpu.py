@@ -190,6 +190,7 @@ EVICT = [
     ([700, 2500, 1025], 600, 0, 0, 2, 128, 16),       # by weight alone
     ([3000], 1, 0, 0, 4, 64, 256),
     ([4097, 2048, 1024], 1023, 100, 1, 2, 128, 128),
+    ([40000, 16385, 16384], 9000, 300, 4, 1, 64, 256),  # longer than what a block holds
 ]
 
 

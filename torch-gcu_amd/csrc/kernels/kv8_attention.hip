@@ -55,7 +55,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   __shared__ float ml[NW][RT][3];
 
   Kv8Item it;
-  if (!kv8_item<RT, RKT>(a, blockIdx.x, &it)) return;
+  if (!kv8_item<RT, RKT, false>(a, blockIdx.x, &it)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int group = a.group, rows = it.cut.rows, row0 = it.tile * RT, len = it.s.len;

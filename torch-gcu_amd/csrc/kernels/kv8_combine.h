@@ -33,6 +33,7 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
     // the sequence that token t is of, and the items before it
     int64_t before = 0;
     bool found = false;
+    int where = 0;
     Kv8Seq s{};
     for (int b0 = 0; b0 < a.seqs && !found; b0 += 64) {
       const Kv8Seq mine = lanes.at(b0);
@@ -42,6 +43,7 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
       if (hit != 0) {
         const int l = __builtin_ctzll(hit);
         found = true;
+        where = l;
         s = Kv8Lanes::pick(mine, l);
         before += __builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l);
       } else {
@@ -54,8 +56,17 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
     if (parts == 1) continue;
     const int row = (t - s.first) * a.group + h % a.group;
     const int tile = LAST_FIRST ? c.row_tiles - 1 - row / RT : row / RT;
-    const int64_t item = before + ((int64_t)tile * a.c.heads + h / a.group) * parts;
-    if (item < 0 || item + parts > a.slots) continue;
+    int64_t item = before + ((int64_t)tile * a.c.heads + h / a.group) * parts;
+    int64_t step = 1;  // from a part to the next
+    if (LAST_FIRST && Kv8RoundItems::apply(a)) {
+      const Kv8RoundItems all = Kv8RoundItems::of<RT, KT>(a, lanes.head, chunk);
+      const int k = tile + __builtin_amdgcn_readlane(all.rounds.off, where);
+      const int n = all.rounds.in(k) ? all.parts : 0;
+      const int first = all.before(k) + __builtin_amdgcn_readlane(wave_scan(n) - n, where);
+      step = a.c.heads;
+      item = (int64_t)first * step + h / a.group;
+    }
+    if (item < 0 || item + (parts - 1) * step >= a.slots) continue;
     typedef float f2 __attribute__((ext_vector_type(2)));
     const f2* pm = (const f2*)a.part_ml + item * RT + row % RT;
     const float* po = a.part_o + (item * RT + row % RT) * D + lane * E;
@@ -66,7 +77,7 @@ __global__ __launch_bounds__(256) void kv8_combine_kernel(Kv8Args a) {
       f2 ml[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t p = min(p0 + u, parts - 1);
+        const int64_t p = min(p0 + u, parts - 1) * step;
         v[u] = *(const fe*)(po + p * RT * D);
         ml[u] = pm[p * RT];
         if (p0 + u >= parts) ml[u] = f2{-INFINITY, 0.f};

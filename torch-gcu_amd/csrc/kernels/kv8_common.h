@@ -168,18 +168,21 @@ __device__ __forceinline__ void lds_copy4_at(const void* p, void* lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(p), "{m0}"(m0) : "memory");
 }
 
-// Inclusive sums over the lanes, by DPP within rows of 16 and two row broadcasts.
-template <int CTRL, int ROWS>
+// Inclusive sums (or maxima of numbers that are not negative) over the lanes, by
+// DPP within rows of 16 and two row broadcasts.
+template <bool MAX, int CTRL, int ROWS>
 __device__ __forceinline__ int scan_step(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+  const int x = __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+  return MAX ? max(v, x) : v + x;
 }
+template <bool MAX = false>
 __device__ __forceinline__ int wave_scan(int v) {
-  v = scan_step<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
-  v = scan_step<0x112, 0xF>(v);
-  v = scan_step<0x114, 0xF>(v);
-  v = scan_step<0x118, 0xF>(v);
-  v = scan_step<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-  return scan_step<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+  v = scan_step<MAX, 0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v = scan_step<MAX, 0x112, 0xF>(v);
+  v = scan_step<MAX, 0x114, 0xF>(v);
+  v = scan_step<MAX, 0x118, 0xF>(v);
+  v = scan_step<MAX, 0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return scan_step<MAX, 0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
 // The call's sequences, a lane each, 64 at a time; the first 64 stay in
@@ -232,6 +235,31 @@ struct Kv8Lanes {
   }
 };
 
+__device__ __forceinline__ int wave_last(int x) { return __builtin_amdgcn_readlane(x, 63); }
+
+// The items of Kv8Rounds: a wave's lanes hold a sequence each.
+struct Kv8RoundItems {
+  Kv8Rounds rounds;
+  int parts, end;  // parts of the lane's sequence; one past the last round, of all
+
+  template <int RT, int KT>
+  static __device__ __forceinline__ Kv8RoundItems of(const Kv8Args& a, const Kv8Seq& s, int chunk) {
+    const Kv8Cut c = kv8_cut(s, a.group, RT, KT);
+    const int longest = wave_last(wave_scan<true>(c.row_tiles > 0 ? s.len : 0));
+    const Kv8Rounds r(s, c, longest, a.group, RT);
+    const int end = wave_last(wave_scan<true>(r.tiles > 0 ? r.off + r.tiles : 0));
+    return {r, c.row_tiles > 0 ? c.parts(chunk) : 0, end};
+  }
+  // (a single sequence's items are in that order anyway)
+  static __device__ __forceinline__ bool apply(const Kv8Args& a) {
+    return a.seqs > 1 && a.seqs <= 64;
+  }
+  // items of a head in rounds 0 .. k - 1, of all sequences
+  __device__ __forceinline__ int before(int k) const {
+    return wave_last(wave_scan(rounds.before(k) * parts));
+  }
+};
+
 // One block's share of a call over query rows and keys: row tile `tile` of k/v
 // head `head` of sequence `seq`, part `part` of its `parts` of keys.
 struct Kv8Item {
@@ -240,13 +268,42 @@ struct Kv8Item {
   int seq, head, tile, part, parts;
 };
 
-template <int RT, int KT>
+// FARTHEST: in the order of Kv8Rounds, with tiles counted from the sequence's end:
+// blocks start in the order of their items, and what starts last should be short
+// (32 query heads on 8 of 128: 4 x up to 1024 tokens behind up to 1000 86 -> 82 us,
+// 32 x up to 64 behind up to 1800 70 -> 62; finding the item takes 1 us more, which
+// calls without a second round of blocks lose: 4 x up to 512 behind up to 1500, 16
+// heads on 4 of 64, 42 -> 44).
+template <int RT, int KT, bool FARTHEST>
 __device__ __forceinline__ bool kv8_item(const Kv8Args& a, int item, Kv8Item* it) {
   const Kv8Lanes lanes(a);
   const int chunk =
       lanes.chunk([&](const Kv8Seq& s) { return kv8_cut(s, a.group, RT, KT).work(); });
   if (item == 0 && a.chunk != nullptr && threadIdx.x == 0) *a.chunk = chunk;
   int place;
+  if (FARTHEST && Kv8RoundItems::apply(a)) {
+    const Kv8RoundItems all = Kv8RoundItems::of<RT, KT>(a, lanes.head, chunk);
+    const int want = item / a.c.heads;  // items of a round hold every head
+    int lo = 0, hi = all.end;           // the round: before(lo) <= want < before(lo + 1)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (all.before(mid) <= want) lo = mid;
+      else hi = mid;
+    }
+    const int n = all.rounds.in(lo) ? all.parts : 0, upto = wave_scan(n);
+    const int rest = want - all.before(lo);
+    const uint64_t hit = __ballot(upto > rest);
+    if (rest < 0 || hit == 0) return false;
+    const int l = __builtin_ctzll(hit);
+    it->seq = wave_uniform(l);
+    it->s = Kv8Lanes::pick(lanes.head, l);
+    it->cut = kv8_cut(it->s, a.group, RT, KT);
+    it->parts = __builtin_amdgcn_readlane(all.parts, l);
+    it->part = rest - (__builtin_amdgcn_readlane(upto, l) - it->parts);
+    it->head = item % a.c.heads;
+    it->tile = lo - __builtin_amdgcn_readlane(all.rounds.off, l);
+    return true;
+  }
   const bool found = lanes.find(
       item,
       [&](const Kv8Seq& s) {

@@ -66,6 +66,21 @@ MI_HD Kv8Cut kv8_cut(const Kv8Seq& s, int group, int rt, int kt) {
   return c;
 }
 
+// Row tiles of up to 64 sequences by how far their last tokens see, the farthest
+// first: round k takes of each sequence the tile whose end lies about k tiles'
+// tokens before the longest sequence's end, if it has one.
+struct Kv8Rounds {
+  int off;    // the round of the sequence's last tile
+  int tiles;
+  MI_HD Kv8Rounds(const Kv8Seq& s, const Kv8Cut& c, int longest, int group, int rt) {
+    const int step = rt / group > 1 ? rt / group : 1;  // tokens of a row tile
+    tiles = c.row_tiles;
+    off = tiles > 0 ? (longest - s.len) / step : 0;
+  }
+  MI_HD int before(int k) const { return kv8_clamp(k - off, 0, tiles); }  // tiles in rounds 0 .. k - 1
+  MI_HD bool in(int k) const { return k >= off && k - off < tiles; }
+};
+
 // How the key tiles of a call are cut into parts: `few` parts in all, or `many`
 // where a part would be longer than `wide` tiles, none shorter than `least`.
 struct Kv8Plan {

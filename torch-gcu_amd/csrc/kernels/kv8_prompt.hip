@@ -3,9 +3,9 @@
 //
 // What bounds it: 4 D flops per query row and key on the matrix instructions,
 // and beside them more time of exp2, maxima and sums on the vector unit.  32 query
-// heads on 8 of 128: 2048 tokens behind 14000 550 us (916 TFLOP/s where a large
+// heads on 8 of 128: 2048 tokens behind 14000 546 us (924 TFLOP/s where a large
 // product reaches 1426; matrix instructions 37 % of the cycles), 2783 tokens of
-// four sequences behind 359 to 823 86 us (500: 704 blocks on 512 places).
+// four sequences behind 359 to 823 82 us (527: 704 blocks on 512 places).
 //   A block takes 32 NW query rows of one k/v head (the group's heads of
 // consecutive tokens), a wave 32 of them, and walks the keys in tiles of 64:
 //   S^T = K Q^T, O^T = V^T P^T (v_mfma_f32_32x32x16), P^T taken from the S^T
@@ -46,8 +46,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   __shared__ int absent[2];                     // bit g: group g does not exist
 
   Kv8Item it;
-  if (!kv8_item<RT, PKT>(a, blockIdx.x, &it)) return;
-  it.tile = it.cut.row_tiles - 1 - it.tile;  // the longest rows first
+  if (!kv8_item<RT, PKT, true>(a, blockIdx.x, &it)) return;
+  it.tile = it.cut.row_tiles - 1 - it.tile;  // the farthest-seeing rows first
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5, col = lane & 31;
