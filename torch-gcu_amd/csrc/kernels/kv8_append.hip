@@ -10,9 +10,9 @@
 // What bounds it: a prompt's bytes (16-bit tokens read, codes written), a
 // decode step's chain of dependent reads (starts, table, token, scale).  One
 // thread block per touched page and head owns that page's scale, so nothing
-// is shared between blocks.  8 heads of 128: 11137 tokens of four sequences 18.8
-// us (68 MB, 3.6 TB/s where a large copy reaches 5.0: the chain, and tokens read
-// a second time from the caches), 8 tokens of as many 4.4 us.
+// is shared between blocks.  8 heads of 128: 11137 tokens of four sequences 17.7
+// us (68 MB, 3.9 TB/s where a large copy reaches 5.0), 8 tokens of as many
+// sequences 4.4 us.
 //
 // A token with an infinite or NaN element has NaN codes for its whole key, so
 // that every query that sees it gets NaN, and 0 in place of the bad elements
@@ -32,21 +32,26 @@ struct Kv8New {
 };
 
 template <typename T>
-__device__ __forceinline__ void widen8(const uint16_t* p, float* x) {
+__device__ __forceinline__ void widen8(u32x4 p, float* x) {
   union {
     u32x4 w;
     uint16_t e[8];
   } u;
-  u.w = *(const u32x4*)p;
+  u.w = p;
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = Num<T>::load(u.e[i]);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
+// U 16-byte pieces of the page's keys and as many of its values a thread, in
+// registers between the maximum and the codes; NT threads, so that pages of 256
+// tokens have as many in flight (11137 tokens of 8 heads of 128, us: in registers,
+// and read a second time for the codes, pages of 16 18.6 / 22.0, of 64 17.7 / 18.8,
+// of 256 24.2 / 37.7).
+template <typename T, int D, int U, int NT>
+__global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, Kv8New x) {
   constexpr int CH = D / 8;  // 8-element pieces of a token's row
   __shared__ int bad[256];   // tokens of the page with a non-finite element
-  __shared__ float most[2][4];
+  __shared__ float most[2][NT / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int cap = a.width << a.c.shift, shift = a.c.shift, size = 1 << shift;
   if (blockIdx.x == 0 && blockIdx.y == 0) {
@@ -78,22 +83,34 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
   float* scales[2] = {(float*)a.c.k_scale + page * a.c.ks_sp + head * a.c.ks_sh,
                       (float*)a.c.v_scale + page * a.c.vs_sp + head * a.c.vs_sh};
 
-  for (int i = threadIdx.x; i < size; i += 256) bad[i] = 0;
-  __syncthreads();
+  const int n = (hi - lo) * CH;
+  u32x4 r[2][U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (NT * u < n) {
+      const int i = min((int)threadIdx.x + NT * u, n - 1), slot = lo + i / CH, c = i % CH;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) r[w][u] = *(const u32x4*)(src[w] + slot * st[w] + 8 * c);
+    }
+  const float was[2] = {*scales[0], *scales[1]};
+  for (int i = threadIdx.x; i < size; i += NT) bad[i] = 0;
+  __syncthreads();  // and every thread has read the scales
   float am[2] = {0.f, 0.f};
-  for (int i = threadIdx.x + lo * CH; i < hi * CH; i += 256) {
-    const int slot = i / CH, c = i % CH;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float e[8];
-      widen8<T>(src[w] + slot * st[w] + 8 * c, e);
+  for (int u = 0; u < U; ++u)
+    if (NT * u < n) {
+      const int slot = lo + min((int)threadIdx.x + NT * u, n - 1) / CH;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (kv8_finite(e[j])) am[w] = fmaxf(am[w], fabsf(e[j]));
-        else bad[slot] = 1;  // every writer writes the same
+      for (int w = 0; w < 2; ++w) {
+        float e[8];
+        widen8<T>(r[w][u], e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (kv8_finite(e[j])) am[w] = fmaxf(am[w], fabsf(e[j]));
+          else bad[slot] = 1;  // every writer writes the same
+        }
       }
     }
-  }
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     am[w] = wave_fmax(am[w]);
@@ -102,14 +119,16 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const float m = fmaxf(fmaxf(most[w][0], most[w][1]), fmaxf(most[w][2], most[w][3]));
-    const float before = *scales[w];
+    float m = most[w][0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, most[w][i]);
+    const float before = was[w];
     // a page starts anew with its first slot, whatever scale it had
     float scale = kv8_scale_of(m);
     if (lo > 0) scale = fmaxf(scale, before);
     if (lo > 0 && scale != before) {
       const float ratio = before / scale;
-      for (int i = threadIdx.x; i < lo * (D / 16); i += 256) {
+      for (int i = threadIdx.x; i < lo * (D / 16); i += NT) {
         u32x4* p = (u32x4*)dst[w] + i;
         u32x4 v = *p;
 #pragma unroll
@@ -118,10 +137,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
       }
     }
     const float inv = 1.0f / scale;
-    for (int i = threadIdx.x + lo * CH; i < hi * CH; i += 256) {
-      const int slot = i / CH, c = i % CH;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = threadIdx.x + NT * u, slot = lo + i / CH, c = i % CH;
+      if (i >= n) continue;
       float e[8];
-      widen8<T>(src[w] + slot * st[w] + 8 * c, e);
+      widen8<T>(r[w][u], e);
       const bool nan = w == 0 && bad[slot] != 0;
       f32x4 p[2];
 #pragma unroll
@@ -131,7 +152,6 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8Args a, Kv8New x) {
       }
       *(u32x2*)(dst[w] + slot * D + 8 * c) = u32x2{f32x4_to_fp8(p[0]), f32x4_to_fp8(p[1])};
     }
-    __syncthreads();  // every thread has read the scale
     if (threadIdx.x == 0) *scales[w] = scale;
   }
 }
@@ -171,13 +191,21 @@ extern "C" mi_status_t mi_kv8_append(const mi_kv8_cache_t* cache, const mi_tenso
                  v->strides[0], v->strides[1]};
   const dim3 grid((unsigned)kv8_touched_most(a.tokens, a.seqs, a.c.shift), (unsigned)a.c.heads);
   hipStream_t s = (hipStream_t)stream;
-  if (k->dtype == MI_BF16 && dim == 128)
-    hipLaunchKernelGGL((kv8_append_kernel<BF16, 128>), grid, dim3(256), 0, s, a, x);
-  else if (k->dtype == MI_BF16)
-    hipLaunchKernelGGL((kv8_append_kernel<BF16, 64>), grid, dim3(256), 0, s, a, x);
-  else if (dim == 128)
-    hipLaunchKernelGGL((kv8_append_kernel<F16, 128>), grid, dim3(256), 0, s, a, x);
-  else
-    hipLaunchKernelGGL((kv8_append_kernel<F16, 64>), grid, dim3(256), 0, s, a, x);
+  auto launch = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a, x);
+  };
+  auto run = [&](auto type, auto width) {
+    typedef decltype(type) T;
+    constexpr int D = decltype(width)::value;
+    const int64_t pieces = (int64_t)(D / 8) << a.c.shift;
+    if (pieces <= 512) launch(kv8_append_kernel<T, D, 2, 256>, 256);
+    else if (pieces <= 1024) launch(kv8_append_kernel<T, D, 4, 256>, 256);
+    else if (pieces <= 2048) launch(kv8_append_kernel<T, D, 4, 512>, 512);
+    else if constexpr (D == 128) launch(kv8_append_kernel<T, D, 4, 1024>, 1024);
+  };
+  const std::integral_constant<int, 128> wide;
+  const std::integral_constant<int, 64> narrow;
+  if (k->dtype == MI_BF16) dim == 128 ? run(BF16{}, wide) : run(BF16{}, narrow);
+  else dim == 128 ? run(F16{}, wide) : run(F16{}, narrow);
   return check_launch(op);
 }
