@@ -330,14 +330,19 @@ mi_status_t run_rows(Kv8Args& a, hipStream_t s) {
   // enough that the last ones to end count (32 sequences of 4000 to 16000: 130 ->
   // 119 us).  A part is at least a tile per wave, and short sequences stay whole,
   // since the merge is a launch of 4 us: up to 1024 positions (1 of 300: 13 -> 8
-  // us), or 2048 where there is a pair for each CU (32 x 8 of 2000: 29 -> 25).
+  // us), or 4096 where a row tile and head for each block fill seven eighths of
+  // their rounds over the CUs (32 x 8 of 4000: 52 -> 45, of 1000 to 4000 43 -> 37,
+  // 56 x 8 of 3000 69 -> 63; but 40 x 8 of 4000 62 -> 76, of 2000 38 -> 40).
   const int cus = cu_count();
   const int64_t tiles = (((int64_t)a.width << a.c.shift) + RKT - 1) / RKT;
-  const int64_t pairs = kv8_row_tiles_most(a.tokens, a.seqs, a.group, 16 * NB) * a.c.heads;
-  const int whole = pairs >= cus ? 8 * NW : 4 * NW;
+  // if the sequences' new tokens are about as many in each
+  const int64_t some = std::min(a.seqs, a.tokens), rows = (int64_t)a.tokens * a.group;
+  const int64_t blocks = some > 0 ? some * ((rows / some + 16 * NB - 1) / (16 * NB)) * a.c.heads : 0;
+  const int64_t rounds = (blocks + cus - 1) / cus;
+  const int whole = blocks > 0 && blocks * 8 >= rounds * cus * 7 ? 16 * NW : 4 * NW;
   a.plan = {2 * cus, 64, tiles <= whole ? whole : NW, 4 * cus};
   // one row tile a sequence: its codes are read once
-  if ((int64_t)a.tokens * a.group <= (int64_t)16 * NB * std::min(a.seqs, a.tokens))
+  if (rows <= 16 * NB * some)
     return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW, true>, 64 * NW, s);
   return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW, false>, 64 * NW, s);
 }
