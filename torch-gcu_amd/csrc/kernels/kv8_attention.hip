@@ -340,7 +340,11 @@ mi_status_t run_rows(Kv8Args& a, hipStream_t s) {
   const int64_t blocks = some > 0 ? some * ((rows / some + 16 * NB - 1) / (16 * NB)) * a.c.heads : 0;
   const int64_t rounds = (blocks + cus - 1) / cus;
   const int whole = blocks > 0 && blocks * 8 >= rounds * cus * 7 ? 16 * NW : 4 * NW;
-  a.plan = {2 * cus, 64, tiles <= whole ? whole : NW, 4 * cus};
+  // each sequence's last part is half a one on the average: room for them, or a few
+  // blocks start when the others end (12 x 8 of 4000: 29 -> 24 us, 16 x 8 of 4000 to
+  // 8000 40 -> 35; 24 x 16 of 2000, more than the CUs: 34 -> 39)
+  const int few = 2 * cus - (blocks < cus ? (int)blocks / 2 : 0);
+  a.plan = {few, 64, tiles <= whole ? whole : NW, 4 * cus};
   // one row tile a sequence: its codes are read once
   if (rows <= 16 * NB * some)
     return kv8_launch<T, D, 16 * NB, RKT, false>(a, kv8_rows_kernel<T, D, NB, NW, true>, 64 * NW, s);
