@@ -114,6 +114,8 @@ SHAPES = [
     ([515, 500], [4000, 3333], 32, 32, 128, 64),     # and rows that do not fill them
     ([40, 1], [100, 33], 80, 1, 128, 64),            # more heads to one than a tile has rows
     ([70, 33], [200, 0], 14, 2, 64, 32),             # seven heads to one
+    ([90, 70], [1500, 1000], 16, 8, 64, 32),         # blocks of 128 keys for most of the CUs
+    ([40], [9000], 80, 1, 64, 256),                  # the same, of more heads to one than a tile has rows
 ]
 
 

@@ -156,15 +156,16 @@ __device__ __forceinline__ float half_sum(float x) { return over_halves<true>(x)
 __device__ __forceinline__ float row_max(float x) { return over_rows<false>(x); }
 __device__ __forceinline__ float row_sum(float x) { return over_rows<true>(x); }
 
-// lds_copy16 from an address of each lane's own.
-__device__ __forceinline__ void lds_copy16_at(const void* p, void* lds) {
-  const uint32_t m0 = wave_uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+// lds_copy16 from an address of each lane's own to m0 (of lds_place) and on.
+__device__ __forceinline__ uint32_t lds_place(void* lds) {
+  return wave_uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+}
+__device__ __forceinline__ void lds_copy16_at(const void* p, uint32_t m0) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(m0) : "memory");
 }
 
 // The same, 4 bytes a lane.
-__device__ __forceinline__ void lds_copy4_at(const void* p, void* lds) {
-  const uint32_t m0 = wave_uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+__device__ __forceinline__ void lds_copy4_at(const void* p, uint32_t m0) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(p), "{m0}"(m0) : "memory");
 }
 

@@ -15,7 +15,7 @@
 //     lane adds its 16 keys' weights over all rows of its column before the 32
 //     columns are added at the end.
 // 32 query heads on 8 of 128: 8 sequences of 4000, a token each 10 us (34.9 MB, 3.5
-// TB/s); 2 of 4333, 333 tokens each 41 us (553 TFLOP/s: an exp2 and two more vector
+// TB/s); 2 of 4333, 333 tokens each 40 us (567 TFLOP/s: an exp2 and two more vector
 // instructions a score take twice the products' time, and 544 blocks are two a CU
 // and three on some).
 #include <algorithm>
@@ -172,13 +172,16 @@ __global__ __launch_bounds__(64 * WNW, 4) void kv8_weigh_rows_kernel(Kv8Args a, 
   }
 }
 
-template <typename T, int D>
+// RS waves share 32 keys, each with its part of a tile's rows.
+template <typename T, int D, int RS>
 __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a, Kv8Weights wt) {
   typedef typename AttnOp<T>::vec vec;
-  constexpr int RT = 64, KT = WKT * WNW, P = D / 32, CH = D / 8;
+  constexpr int RT = RS == 4 ? 128 : 64, KT = WKT * WNW / RS, P = D / 32, CH = D / 8;
+  constexpr int U = RT / 32 / RS;  // a wave's halves of 32 rows
   constexpr int N = RT * CH / (64 * WNW);  // 16-byte pieces of a row tile a thread stages
   __shared__ __align__(16) uint16_t qs[3][RT * D];
   __shared__ __align__(16) float ls[3][RT];
+  __shared__ float part[WNW][WKT];
   if (blockIdx.x == 0)
     kv8_report_lengths(a.lengths, a.seqs, a.width << a.c.shift, a.fault);
   WeighItem<RT, KT> it;
@@ -214,25 +217,31 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
     const int i = tid / CH + n * RPI;
     q_at[n] = a.q + (i / hp) * a.q_st + (i % hp) * a.q_sh + piece;
   }
-  const float* l_at = a.lse + (lane / hp) * a.lse_st + (lane % hp) * a.lse_sh;
+  const bool has_l = wave < RT / 64;  // a lane each
+  const float* l_at = a.lse + (tid / hp) * a.lse_st + (tid % hp) * a.lse_sh;
+  // places in LDS once: a cast of the pointers in the loop costs more than the copies
+  const uint32_t q_to = lds_place(qs[0]) + wave * 64 * 16, l_to = lds_place(ls[0]) + wave * 64 * 4;
   auto copy = [&](const RowTile& x, int buf) __attribute__((always_inline)) {
     const int64_t token = s.first + x.t, h = it.head * group + x.g;
     const int64_t at = token * a.q_st + h * a.q_sh;
+    const int64_t l = token * a.lse_st + h * a.lse_sh;
+    const uint32_t to = q_to + buf * RT * D * 2;
     const int rows = count(x);
+    if (rows == RT) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const uint16_t* from = q_at[n];
-      if (rows < RT && tid / CH + n * RPI >= rows) from = a.q + piece;
-      lds_copy16_at(from + at, qs[buf] + (wave * 64 + n * 64 * WNW) * 8);
-    }
-    if (wave == 0) {  // RT == 64: a lane each
-      const float* from = rows < RT && lane >= rows ? a.lse : l_at;
-      lds_copy4_at(from + token * a.lse_st + h * a.lse_sh, ls[buf]);
+      for (int n = 0; n < N; ++n) lds_copy16_at(q_at[n] + at, to + n * 64 * WNW * 16);
+      if (has_l) lds_copy4_at(l_at + l, l_to + buf * RT * 4);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        lds_copy16_at((tid / CH + n * RPI < rows ? q_at[n] : a.q + piece) + at,
+                      to + n * 64 * WNW * 16);
+      if (has_l) lds_copy4_at((tid < rows ? l_at : a.lse) + l, l_to + buf * RT * 4);
     }
   };
 
   for (int j = it.lo; j < it.hi; ++j) {
-    const int key0 = j * KT + wave * WKT;
+    const int key0 = j * KT + wave / RS * WKT;
     const WeighKeys keys(a, s, it.seq, it.head, min(key0, s.len - 1), D);
     const uint8_t* kp = a.c.k + (col < 16 ? keys.at[0] : keys.at[1]) + (col & 15) * D + 16 * half;
     vec kf[2 * P];
@@ -244,7 +253,8 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
     }
     // the lane's own weight: one read and one write, not one for each product
     const int mine = key0 + 8 * (col >> 2) + 4 * half + (col & 3);
-    const bool owner = col < 16 && mine < s.len && (col < 8 ? keys.ok[0] : keys.ok[1]);
+    const bool owner = wave % RS == 0 && col < 16 && mine < s.len &&
+                       (col < 8 ? keys.ok[0] : keys.ok[1]);
     const float before = owner ? out[mine] : 0.f;
     f32x16 sum = f32x16{};
     // the block's first key is seen from its own token on, all keys of the wave by
@@ -258,7 +268,7 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
     for (int buf = 0; now.t < s.n; next(now), buf = buf == 2 ? 0 : buf + 1) {
       // this wave's copies of the tile, with those of the next one still on the way
       if (ahead.t >= s.n) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      else if (wave == 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N + 1) : "memory");
+      else if (wave < RT / 64) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N + 1) : "memory");
       else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
       __syncthreads();
       if (ahead.t < s.n) next(ahead);
@@ -266,8 +276,8 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
       if (key0 >= s.len) continue;
       const int rows = count(now);
 #pragma unroll
-      for (int u = 0; u < RT / 32; ++u) {
-        const int row = 32 * u + col;
+      for (int u = 0; u < U; ++u) {
+        const int row = 32 * (wave % RS * U + u) + col;
         const uint16_t* q = qs[buf] + row * D;
         // a row that is none weighs nothing
         const float lse = row < rows ? ls[buf][row] * 1.4426950408889634f : INFINITY;
@@ -304,6 +314,13 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
       v = row_sum(v);
       got = col == r ? v : got;
     }
+    if constexpr (RS > 1) {  // added in the order of the rows' parts
+      if (col < 16) part[wave][16 * half + col] = got;
+      __syncthreads();
+      if (wave % RS == 0 && col < 16)
+#pragma unroll
+        for (int i = 1; i < RS; ++i) got += part[wave + i][16 * half + col];
+    }
     if (owner) out[mine] = before + got;
   }
 }
@@ -316,8 +333,21 @@ mi_status_t run_weigh(Kv8Args& a, const Kv8Weights& w, hipStream_t s) {
   const bool few = (int64_t)a.tokens * a.group <= (int64_t)32 * some;
   a.plan = {4 * cu_count(), 0, 1, 4 * cu_count()};
   const dim3 grid((unsigned)(a.plan.many + some * a.c.heads));
+  const int64_t keys = (int64_t)a.width << a.c.shift, tile = WKT * WNW;
+  const int64_t blocks = some * a.c.heads * ((keys + tile - 1) / tile);
   if (few) hipLaunchKernelGGL((kv8_weigh_rows_kernel<T, D>), grid, block, 0, s, a, w);
-  else hipLaunchKernelGGL((kv8_weigh_prompt_kernel<T, D>), grid, block, 0, s, a, w);
+  // A block walks all rows, and where the blocks of 128 keys leave CUs idle, smaller
+  // ones with waves that share the rows walk faster, at twice (four times) the
+  // copies.  us, one, two and four waves to 32 keys, 32 query heads on 8 of 128: 64
+  // tokens behind 500 (40 blocks of 128 keys) 9.6 / 8.9 / 8.9, 333 behind 1000 (88)
+  // 25.5 / 21.3 / 29, behind 4000 (272) 28.5 / 27.4 / 67, 2 x 333 behind 4000 (544) 42
+  // / 65 / 122; 5 heads on one of 64, 5 x 301 behind 721 (40) 27.5 / 21.2 / 14.4.
+  else if (4 * blocks <= cu_count())
+    hipLaunchKernelGGL((kv8_weigh_prompt_kernel<T, D, 4>), grid, block, 0, s, a, w);
+  else if (blocks <= cu_count())
+    hipLaunchKernelGGL((kv8_weigh_prompt_kernel<T, D, 2>), grid, block, 0, s, a, w);
+  else
+    hipLaunchKernelGGL((kv8_weigh_prompt_kernel<T, D, 1>), grid, block, 0, s, a, w);
   return check_launch("kv8_weigh");
 }
 
