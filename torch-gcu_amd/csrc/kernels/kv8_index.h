@@ -39,6 +39,15 @@ MI_HD Kv8Seq kv8_seq(int start, int next, int length, int tokens, int cap) {
 // The page that a table entry names, or -1 if the cache has no such page.
 MI_HD int kv8_page(int entry, int pages) { return entry >= 0 && entry < pages ? entry : -1; }
 
+// Where the 16 keys from `pos` (a multiple of 16) on are loaded from: their own
+// place, or behind the end of a sequence of `len` >= 1 the place of its last 16.
+// Pages hold a multiple of 16, so the 16 slots from the result on lie in one page,
+// and that page is one of the sequence's.
+MI_HD int kv8_group_at(int pos, int len) {
+  const int last = (len - 1) & ~15;
+  return pos < last ? pos : last;
+}
+
 // One past the last position that new token i of a sequence sees: its own
 // position is len - n + i.  0 when nothing is visible.
 MI_HD int kv8_limit(const Kv8Seq& s, int i) {

@@ -78,12 +78,12 @@ struct WeighKeys {
     const int* table = a.table + seq * a.t_sb;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int pos = key0 + 16 * t;
-      const int entry = ld_const(table + min(pos >> a.c.shift, a.width - 1));
+      const bool in = key0 + 16 * t < s.len;
+      const int pos = kv8_group_at(key0 + 16 * t, s.len);
+      const int entry = ld_const(table + (pos >> a.c.shift));
       const int p = kv8_page(entry, a.c.pages);
-      ok[t] = pos < s.len && p >= 0;
-      if (pos < s.len && p < 0 && (threadIdx.x & 63) == 0)
-        record_index_fault(a.fault, entry, a.c.pages);
+      ok[t] = in && p >= 0;
+      if (in && p < 0 && (threadIdx.x & 63) == 0) record_index_fault(a.fault, entry, a.c.pages);
       const int64_t page = max(p, 0);  // read instead, and nothing of it used
       at[t] = page * a.c.k_sp + head * a.c.k_sh + (pos & ((1 << a.c.shift) - 1)) * D;
       sc[t] = a.scale_log2 * ld_const(a.c.k_scale + page * a.c.ks_sp + head * a.c.ks_sh);
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
 
   for (int j = it.lo; j < it.hi; ++j) {
     const int key0 = j * KT + wave / RS * WKT;
-    const WeighKeys keys(a, s, it.seq, it.head, min(key0, s.len - 1), D);
+    const WeighKeys keys(a, s, it.seq, it.head, key0, D);
     const uint8_t* kp = a.c.k + (col < 16 ? keys.at[0] : keys.at[1]) + (col & 15) * D + 16 * half;
     vec kf[2 * P];
 #pragma unroll
