@@ -181,6 +181,7 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
   constexpr int N = RT * CH / (64 * WNW);  // 16-byte pieces of a row tile a thread stages
   __shared__ __align__(16) uint16_t qs[3][RT * D];
   __shared__ __align__(16) float ls[3][RT];
+  __shared__ __align__(16) uint16_t none[D];  // the query of a row that is none
   __shared__ float part[WNW][WKT];
   if (blockIdx.x == 0)
     kv8_report_lengths(a.lengths, a.seqs, a.width << a.c.shift, a.fault);
@@ -189,6 +190,7 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_uniform(tid >> 6);
   const int half = lane >> 5, col = lane & 31, group = a.group;
   const Kv8Seq s = it.s;
+  if (tid < CH) *(u32x4*)(none + 8 * tid) = u32x4{};  // the loop's first barriers lie before its readers
   const int past = s.len - s.n;
   float* out = wt.w + it.seq * wt.sb + it.head * wt.sh;
   // A tile of up to RT rows is whole tokens' heads, or RT heads of one token where
@@ -278,8 +280,9 @@ __global__ __launch_bounds__(64 * WNW, 3) void kv8_weigh_prompt_kernel(Kv8Args a
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int row = 32 * (wave % RS * U + u) + col;
-        const uint16_t* q = qs[buf] + row * D;
-        // a row that is none weighs nothing
+        // a row that is none weighs nothing; its place in the tile holds another
+        // row's query, and one that is not finite would be no 0 even with this lse
+        const uint16_t* q = row < rows ? qs[buf] + row * D : none;
         const float lse = row < rows ? ls[buf][row] * 1.4426950408889634f : INFINITY;
         f32x16 x = f32x16{};
 #pragma unroll
