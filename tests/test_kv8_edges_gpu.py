@@ -5,10 +5,15 @@ import pytest
 import torch
 
 import torch_gcu  # noqa: F401
+from oracle import kv8 as oracle
 from test_kv8_gpu import Setup
 
 pytestmark = pytest.mark.gpu
 eff = torch.gcu.efficient if hasattr(torch, "gcu") else None
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32).to("gcu")
 
 
 # ---- accumulated weights ------------------------------------------------------
@@ -37,3 +42,36 @@ def test_a_bad_query_weighs_on_the_keys_that_it_sees(group, blocks, bad):
         assert got[0].isfinite().all()
         assert torch.equal(got[1][0, 0, at:], got[0][0, 0, at:])
         assert torch.equal(got[1][0, 1], got[0][0, 1])  # the other k/v head
+
+
+# ---- eviction -----------------------------------------------------------------
+
+
+def same_pages(cache, want, pages):
+    for got, want in zip(cache, want):
+        got, want = got.cpu()[pages], want[pages]
+        if got.dtype == torch.uint8:  # 0 and -0 are one number
+            got, want = (torch.where(x == 0x80, 0, x.int()) for x in (got, want))
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("small", [0.0, 1e-30])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 256)])
+def test_zero_tokens_of_a_page_with_a_large_scale(d, page, small):
+    """Tokens of zeros, kept from a page whose other tokens are large, alone or with
+    tokens of another page that are very small."""
+    n, hk, keep = page + 8, 2, 10
+    s = Setup([0], [n], hk, hk, d, page, seed=1, spare=3)
+    x = torch.zeros(2, n, hk, d, dtype=torch.bfloat16)
+    x[:, 8:page] = 1e9  # the first 8 tokens of page 0 are zero
+    x[:, page:] = small
+    s.cache = tuple(torch.zeros_like(t) for t in s.cache)
+    oracle.append(s.cache, x[0], x[1], s.table, [n], [0, n])
+    w = torch.zeros(1, hk, s.width * page)
+    w[..., :7], w[..., page: page + 3] = 2.0, 1.0
+    fresh = [[s.free[0]]]
+    cache, index = s.gcu(), s.index()
+    kept, left, _ = eff.kv8_evict(cache, w.to("gcu"), index[0], i32(fresh), index[1], keep, 0, 0)
+    k, m, _ = oracle.evict(s.cache, w, s.table, fresh, [n], keep, 0, 0)
+    assert torch.equal(kept.cpu(), k) and left.cpu().tolist() == m
+    same_pages(cache, s.cache, list(range(s.pages)))

@@ -257,7 +257,10 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8Args a, Kv8Evict e) {
   for (int u = 0; u < U; ++u) {
     const int i = tid + 256 * u;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) v[u][w] = f32x4_to_fp8(fp8x4_to_f32(v[u][w]) * (sc[u] * inv));
+    for (int w = 0; w < 4; ++w) {
+      // one scale after the other: their product can be infinite where the code is 0
+      v[u][w] = f32x4_to_fp8(fp8x4_to_f32(v[u][w]) * sc[u] * inv);
+    }
     if (i < n * CH) *(u32x4*)(dst + (i / CH) * D + 16 * (i % CH)) = v[u];
   }
   if (tid == 0) ((float*)scales)[page * ssp] = scale;
