@@ -75,3 +75,32 @@ def test_zero_tokens_of_a_page_with_a_large_scale(d, page, small):
     k, m, _ = oracle.evict(s.cache, w, s.table, fresh, [n], keep, 0, 0)
     assert torch.equal(kept.cpu(), k) and left.cpu().tolist() == m
     same_pages(cache, s.cache, list(range(s.pages)))
+
+
+def test_kept_tokens_of_a_page_that_is_not_there_are_zeros():
+    """Whatever the scale of the page that is read in its stead."""
+    d, page, hk = 64, 16, 2
+    s = Setup([0], [40], hk, hk, d, page, seed=2, spare=6)
+    if 0 in s.table[0]:
+        s.table[0][s.table[0].index(0)] = s.free.pop()
+    s.cache = tuple(torch.zeros_like(t) for t in s.cache)
+    x = torch.randn(2, 40, hk, d, generator=torch.Generator().manual_seed(3)).bfloat16()
+    oracle.append(s.cache, x[0], x[1], s.table, [40], [0, 40])
+    for t in s.cache[2:]:
+        t[0] = math.nan
+    bad = [list(s.table[0])]
+    bad[0][1] = s.pages
+    w = torch.zeros(1, hk, s.width * page)
+    w[..., 10:30] = 1.0  # six of page 0, and 14 of the page that is not there
+    fresh = [[p for p in s.free if p][:2]]
+    cache = s.gcu()
+    eff.kv8_evict(cache, w.to("gcu"), s.index(table=bad)[0], i32(fresh), i32([40]), 20, 0, 0)
+    with pytest.raises(IndexError, match=f"index {s.pages} is out of bounds"):
+        torch.gcu.synchronize()
+    gone = s.table[0][1]
+    for t in s.cache[:2]:
+        t[gone] = 0
+    for t in s.cache[2:]:
+        t[gone] = 1.0
+    oracle.evict(s.cache, w, s.table, fresh, [40], 20, 0, 0)
+    same_pages(cache, s.cache, fresh[0])

@@ -236,7 +236,10 @@ __global__ __launch_bounds__(256) void kv8_move_kernel(Kv8Args a, Kv8Evict e) {
     const int64_t old = max(p, 0);
     v[u] = *(const u32x4*)(codes + old * sp + (pos & (size - 1)) * D + 16 * (i % CH));
     sc[u] = scales[old * ssp];
-    if (p < 0) v[u] = u32x4{};  // a page that is not there: zeros
+    if (p < 0) {  // a page that is not there: zeros, whatever the scale of the one read instead
+      v[u] = u32x4{};
+      sc[u] = 1.f;
+    }
   }
   float am = 0.f;
 #pragma unroll
