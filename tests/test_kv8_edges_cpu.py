@@ -3,6 +3,10 @@ its kernels load keys from."""
 import os
 import subprocess
 
+import torch
+
+from torch_gcu import _abi
+
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 KERNELS = os.path.join(REPO, "torch-gcu_amd", "csrc", "kernels")
 
@@ -47,3 +51,11 @@ def test_keys_are_loaded_from_inside_a_page(tmp_path):
                     "-I", KERNELS, str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_rope_of_no_tokens_is_no_error():
+    """Nor is it taken for one where there are positions to rotate by."""
+    q, k = torch.zeros(0, 4, 64, dtype=torch.bfloat16), torch.zeros(0, 2, 64, dtype=torch.bfloat16)
+    for positions, status in ((torch.zeros(0, dtype=torch.int64), 0), (torch.zeros(3, dtype=torch.int64), 1)):
+        a = [_abi.desc(t) for t in (q, k, q, k, positions)]
+        assert _abi.lib().mi_rope(*a, 1e4, None) == status, _abi.lib().mi_last_error()

@@ -480,7 +480,9 @@ mi_status_t mi_rope(const mi_tensor_t* q_out, const mi_tensor_t* k_out, const mi
                     mi_stream_t stream_) {
   clear_error();
   hipStream_t stream = (hipStream_t)stream_;
-  MI_CHECK_ARG(q != nullptr && q->data != nullptr, "rope: q is required");
+  // (no tokens have no memory)
+  MI_CHECK_ARG(q != nullptr && (q->data != nullptr || (q->ndim == 3 && q->sizes[0] == 0)),
+               "rope: q is required");
   MI_RETURN_IF(validate(q, "q"));
   MI_RETURN_IF(validate(positions, "positions"));
   MI_CHECK_ARG(positions->ndim == 1, "rope: positions must be 1-D");
@@ -489,6 +491,8 @@ mi_status_t mi_rope(const mi_tensor_t* q_out, const mi_tensor_t* k_out, const mi
   MI_CHECK_ARG(theta > 0.0, "rope: theta must be positive");
   MI_CHECK_ARG(q->ndim == 3, "rope: q must be [tokens, heads, head_dim]");
   const int64_t tokens = positions->sizes[0];
+  MI_CHECK_ARG(q->sizes[0] == tokens, "rope: q has %lld tokens, positions has %lld",
+               (long long)q->sizes[0], (long long)tokens);
   const int64_t D = q->sizes[2];
   MI_CHECK_ARG(D % 2 == 0, "rope: head_dim must be even");
   const int esz = dtype_size(q->dtype);
