@@ -7,6 +7,7 @@ import torch
 import torch_gcu  # noqa: F401
 from oracle import kv8 as oracle
 from test_kv8_gpu import Setup
+from torch_gcu.utils import decoder_layer as dl
 
 pytestmark = pytest.mark.gpu
 eff = torch.gcu.efficient if hasattr(torch, "gcu") else None
@@ -104,3 +105,18 @@ def test_kept_tokens_of_a_page_that_is_not_there_are_zeros():
         t[gone] = 1.0
     oracle.evict(s.cache, w, s.table, fresh, [40], 20, 0, 0)
     same_pages(cache, s.cache, fresh[0])
+
+
+# ---- the decoder layer ----------------------------------------------------------
+
+
+def test_decoder_layer_without_new_tokens():
+    cfg = dl.LayerConfig(vocab=100, hidden=256, heads=4, head_dim=64, ffn=512)
+    w = {n: t.to("gcu") for n, t in dl.init_weights(cfg, 3).items()}
+    for n in ("wk", "wv"):
+        w[n] = w[n][:128].contiguous()
+    cache = eff.kv8_cache(4, 2, 64, 32)
+    ids = torch.zeros(0, dtype=torch.int64).to("gcu")
+    out, q, lse = dl.forward_cached(w, ids, cfg, cache, i32([[0, 1]]), i32([5]), i32([0, 0]), ids)
+    assert out.shape == (0, 256) and q.shape == (0, 4, 64) and lse.shape == (0, 4)
+    assert all((t.cpu() == 0).all() for t in cache)

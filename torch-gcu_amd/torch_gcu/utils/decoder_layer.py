@@ -149,8 +149,8 @@ def forward_cached(weights: dict, ids: torch.Tensor, cfg: LayerConfig, cache,
     x = F.embedding(ids, weights["embed"])
     h = _rms_norm(x, weights["attn_norm"], cfg.eps)
     q = F.linear(h, weights["wq"]).view(T, H, D)
-    k = F.linear(h, weights["wk"]).view(T, -1, D)
-    v = F.linear(h, weights["wv"]).view(T, -1, D)
+    k = F.linear(h, weights["wk"]).view(T, weights["wk"].shape[0] // D, D)
+    v = F.linear(h, weights["wv"]).view(T, weights["wv"].shape[0] // D, D)
     _rope_(q, k, pos, cfg.theta)
     eff.kv8_append(k, v, cache, block_table, lengths, starts)
     a, lse = eff.kv8_attention(q, cache, block_table, lengths, starts)
