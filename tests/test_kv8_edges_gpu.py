@@ -1,4 +1,6 @@
-"""Edges of the 8-bit key/value cache on the GPU."""
+"""Edges of the 8-bit key/value cache on the GPU: queries that are not finite beside
+rows that pad a tile, pages of very different scales, tokens that are zero, and
+tolerances that go by each row's own values."""
 import math
 
 import pytest
@@ -6,11 +8,13 @@ import torch
 
 import torch_gcu  # noqa: F401
 from oracle import kv8 as oracle
-from test_kv8_gpu import Setup
+from test_kv8_gpu import F, SHAPES, Setup, wide_table
 from torch_gcu.utils import decoder_layer as dl
 
 pytestmark = pytest.mark.gpu
 eff = torch.gcu.efficient if hasattr(torch, "gcu") else None
+DTYPES = [torch.bfloat16, torch.float16]
+IDS = ["bf16", "f16"]
 
 
 def i32(x):
@@ -105,6 +109,106 @@ def test_kept_tokens_of_a_page_that_is_not_there_are_zeros():
         t[gone] = 1.0
     oracle.evict(s.cache, w, s.table, fresh, [40], 20, 0, 0)
     same_pages(cache, s.cache, fresh[0])
+
+
+# ---- attention ----------------------------------------------------------------
+
+
+def bounds(s, scale):
+    """(want, tolerance) of the output: each row by its own keys.  With u = eps / 2 of
+    the type: a score is an fp32 sum of exact products, off by at most e_j = (D + 8) F
+    times its sum of |q k| scale, and 2^-21 for the exp2 unit and log2(e); so a weight
+    p_j by p_j (e_j + sum_i p_i e_i).  A weight is rounded to the type: by u, or in f16
+    under its normal range by 2^-25 of the row's largest weight (and never by more than
+    itself).  The sum over n keys
+    is off by n F of the sum of magnitudes, the output rounded by u (2^-25 in f16)."""
+    f16, u = s.dtype == torch.float16, torch.finfo(s.dtype).eps / 2
+    hk = s.cache[0].shape[1]
+    T, H, D = s.q.shape
+    want, tol = (torch.zeros(T, H, D, dtype=torch.float64) for _ in range(2))
+    for b, total in enumerate(s.lens):
+        span = slice(s.starts[b], s.starts[b + 1])
+        n = span.stop - span.start
+        if n == 0 or total == 0:
+            continue
+        see = torch.arange(total)[None] <= torch.arange(total - n, total)[:, None]
+        for h in range(H):
+            g = h // (H // hk)
+            k, v = (oracle.tokens(s.cache[i][:, g], s.cache[i + 2][:, g], s.table[b], total) for i in (0, 1))
+            q = s.q[span, h].double()
+            x = torch.where(see, (q @ k.t()) * scale, -math.inf)
+            p = torch.softmax(x, 1).nan_to_num(nan=0.0)  # a row that sees nothing: 0
+            e = (D + 8) * F * (q.abs() @ k.abs().t()) * abs(scale) + 2.0 ** -21
+            off = p * (e + (p * e).sum(1, keepdim=True) + u + see.sum(1, keepdim=True) * F)
+            if f16:
+                off = off + torch.minimum(2.0 ** -25 * p.amax(1, keepdim=True), p)
+            want[span, h] = p @ v
+            tol[span, h] = off @ v.abs() + u * want[span, h].abs()
+    tol += 2.0 ** -25 if f16 else 1e-37
+    return want, tol
+
+
+def check(s, out):
+    want, tol = bounds(s, s.d ** -0.5)
+    off = (out.cpu().double() - want).abs() / tol
+    assert not off.isnan().any(), "NaN"
+    assert off.max() <= 1, f"{off.max()} of the tolerance, in row {int(off.amax((1, 2)).argmax())}"
+
+
+def attend(s):
+    out, _ = eff.kv8_attention(s.q.to("gcu"), s.gcu(), *s.index())
+    return out
+
+
+def larger(s, page, ratio):
+    for _ in range(2):  # 2^130 is no float32
+        s.cache[3][page] *= 2.0 ** (ratio // 2)
+
+
+def width_for(s_new, group, hk, page, wide):
+    return wide_table(sum(s_new) * group, hk, page) if wide else 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("new,past,h,hk,d,page", [SHAPES[i] for i in (1, 3, 6, 8, 10, 12, 13, 17)])
+def test_each_row_by_its_own_values(new, past, h, hk, d, page, dtype):
+    s = Setup(new, past, h, hk, d, page, dtype, seed=5).fill()
+    check(s, attend(s))
+    for i in range(s.pages):
+        s.cache[3][i] *= 2.0 ** (i % 5)
+    check(s, attend(s))
+
+
+@pytest.mark.parametrize("dtype,ratio", [(torch.float16, 4), (torch.float16, 14), (torch.float16, 20),
+                                         (torch.float16, 30), (torch.bfloat16, 20), (torch.bfloat16, 130)])
+@pytest.mark.parametrize("new,wide", [(1, False), (8, False), (90, False)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_large_page_of_no_weight(d, new, wide, dtype, ratio):
+    """A page whose values are larger by 2^ratio, and whose scores are so low that the
+    softmax gives it nothing: the others' weights keep their bits."""
+    s = Setup([new], [600], 4, 2, d, 16, dtype, seed=d + new, width=width_for([new], 2, 2, 16, wide))
+    s.q[..., 0] = 1024.0
+    s.fill()
+    low = [s.table[0][10], s.table[0][27]]
+    for p in s.table[0]:  # channel 0 of the keys decides alone
+        s.cache[0][p, ..., 0] = 0xFE if p in low else 0  # -448
+    s.cache[3][:] *= 2.0 ** (-60 if dtype == torch.bfloat16 else 0)
+    for p in low:
+        larger(s, p, ratio)
+    check(s, attend(s))
+
+
+@pytest.mark.parametrize("dtype,ratio", [(torch.float16, 10), (torch.float16, 20), (torch.float16, 28),
+                                         (torch.bfloat16, 20), (torch.bfloat16, 130)])
+@pytest.mark.parametrize("wide", [False])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_in_front_of_a_large_page(d, wide, dtype, ratio):
+    """Queries that end before a page of large values, in the same tile of keys."""
+    s = Setup([100], [100], 4, 2, d, 16, dtype, seed=d, width=width_for([100], 2, 2, 16, wide)).fill()
+    large = 12 if dtype == torch.float16 else 70  # times 2^large, the others 2^ratio less
+    s.cache[3][:] *= 2.0 ** (large - ratio)
+    larger(s, s.table[0][9], ratio)
+    check(s, attend(s))
 
 
 # ---- the decoder layer ----------------------------------------------------------

@@ -18,9 +18,8 @@
 //                 K nor V passes through LDS.
 //
 // The scales multiply scores (K) and weights (V) in fp32: one scalar per 16
-// keys, since a page holds a multiple of 16.  P is rounded to the input type;
-// for f16 the weights are taken relative to the largest V scale met, or small
-// scales would push them under f16's range.
+// keys, since a page holds a multiple of 16.  P is rounded to the input type; for
+// f16 as Kv8F16 says.
 //
 // Work: kv8_plan cuts each sequence's keys into parts so that all sequences
 // together make a few blocks per CU, whatever their lengths; the device reads
@@ -135,23 +134,28 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[nb][i] = f32x4{};
   }
-  float vref = 0x1p-126f;  // f16: the largest V scale met; o holds sums over it
+  float vref = 0x1p-126f;  // f16: o holds sums over it
 
   auto compute = [&](int j, RowsTile<D>& x) __attribute__((always_inline)) {
     const bool edge = j * RKT + RKT > least || !x.ok[0] || !x.ok[1];
     float vs[2] = {x.ok[0] ? x.vs[0] : 0.f, x.ok[1] ? x.vs[1] : 0.f};
+    bool apart[2] = {false, false};
     if constexpr (F) {
-      const float top = fmaxf(vs[0], vs[1]);
+      const float top = wave_uniform_f32(Kv8F16::ref(fmaxf(vs[0], vs[1])));
       if (top > vref) {
-        const float r = vref / top;
+        const float r = wave_uniform_f32(vref * __builtin_amdgcn_rcpf(top));
         vref = top;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int i = 0; i < DT; ++i) o[nb][i] *= r;
       }
-      vs[0] /= vref;
-      vs[1] /= vref;
+      const float inv = __builtin_amdgcn_rcpf(vref);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        vs[t] = wave_uniform_f32(vs[t] * inv);
+        apart[t] = Kv8F16::apart(vs[t]);
+      }
     }
     vec kf[2][KS];
 #pragma unroll
@@ -159,7 +163,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
 #pragma unroll
       for (int k = 0; k < KS; ++k)
         kf[t][k] = fp8x8_to<T>(x.k[t][k >> 1][2 * (k & 1)], x.k[t][k >> 1][2 * (k & 1) + 1]);
-    vec pk[NB];
+    f32x8 p[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       f32x8 s;
@@ -182,6 +186,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
       float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                        fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
       mx = half_max(row_max(mx));
+      if constexpr (F) mx = ceilf(mx);
       if (mx > m_run[nb]) {
         const float corr = __builtin_amdgcn_exp2f(m_run[nb] - mx);
         m_run[nb] = mx;
@@ -189,17 +194,31 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[nb][i] *= corr;
       }
-      const float m_use = m_run[nb] == -INFINITY ? 0.f : m_run[nb];
-      f32x8 p;
+      const float m_use = m_run[nb] == -INFINITY ? 0.f : F ? m_run[nb] - Kv8F16::BITS : m_run[nb];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(s[i] - m_use);
-        l_run[nb] += e;
-        p[i] = e * vs[i >> 2];
+        p[nb][i] = __builtin_amdgcn_exp2f(s[i] - m_use);
+        l_run[nb] += p[nb][i];
       }
-      pk[nb] = __builtin_convertvector(p, vec);
     }
-    if (j * RKT + RKT > len || !x.ok[0] || !x.ok[1]) {
+    // d = 4 w + 2 h and the next of the lane's 8 keys, as operands
+    auto values = [&](int w, int h, vec* vf) __attribute__((always_inline)) {
+      union {
+        typename Fp8To<T>::pair p[4];
+        vec v;
+      } u[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // the two bytes of keys 2 q and 2 q + 1, side by side
+        const uint32_t e = __builtin_amdgcn_perm(x.v[2 * q + 1][w], x.v[2 * q][w],
+                                                 h == 0 ? 0x05010400u : 0x07030602u);
+        u[0].p[q] = Fp8To<T>::template cvt<false>(e);
+        u[1].p[q] = Fp8To<T>::template cvt<true>(e);
+      }
+      vf[0] = u[0].v;
+      vf[1] = u[1].v;
+    };
+    if (j * RKT + RKT > len || !x.ok[0] || !x.ok[1] || apart[0] || apart[1]) {
       // what lies behind the last token, or on a page that is not there, may
       // hold anything, NaN codes too: 0 x NaN must not come in
 #pragma unroll
@@ -209,29 +228,49 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
         for (int w = 0; w < W; ++w)
           x.v[i][w] = key < len && x.ok[i >> 2] ? x.v[i][w] : 0u;
       }
-    }
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      union {
-        typename Fp8To<T>::pair p[4];
-        vec v;
-      } vf[4];
+      for (int t = 0; t < 2; ++t) {
+        if (!apart[t]) continue;
+        // 16 keys by themselves, the other half's weights as 0
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        // bytes 0, 1 (then 2, 3) of keys 2 q and 2 q + 1, side by side
-        const uint32_t e0 = __builtin_amdgcn_perm(x.v[2 * q + 1][w], x.v[2 * q][w], 0x05010400u);
-        const uint32_t e1 = __builtin_amdgcn_perm(x.v[2 * q + 1][w], x.v[2 * q][w], 0x07030602u);
-        vf[0].p[q] = Fp8To<T>::template cvt<false>(e0);
-        vf[1].p[q] = Fp8To<T>::template cvt<true>(e0);
-        vf[2].p[q] = Fp8To<T>::template cvt<false>(e1);
-        vf[3].p[q] = Fp8To<T>::template cvt<true>(e1);
+        for (int nb = 0; nb < NB; ++nb) {
+          f32x8 half = f32x8{};
+#pragma unroll
+          for (int i = 4 * t; i < 4 * t + 4; ++i) half[i] = p[nb][i];
+          const vec pk = __builtin_convertvector(half, vec);
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              vec vf[2];
+              values(w, h, vf);
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                o[nb][4 * w + 2 * h + e] += Mma16<T>::mma(vf[e], pk, f32x4{}) * vs[t];
+            }
+        }
+        vs[t] = 0.f;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-          o[nb][4 * w + e] = Mma16<T>::mma(vf[e].v, pk[nb], o[nb][4 * w + e]);
     }
+    vec pk[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[nb][i] *= vs[i >> 2];
+      pk[nb] = __builtin_convertvector(p[nb], vec);
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        vec vf[2];
+        values(w, h, vf);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            o[nb][4 * w + 2 * h + e] = Mma16<T>::mma(vf[e], pk[nb], o[nb][4 * w + 2 * h + e]);
+      }
   };
 
   // this wave's tiles lo + wave, then every NW-th, their table entries one step
@@ -251,7 +290,8 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   // merge the waves: common max, scaled sums, O added in wave order
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    const float l = half_sum(row_sum(l_run[nb]));
+    float l = half_sum(row_sum(l_run[nb]));
+    if constexpr (F) l *= Kv8F16::UNIT;
     if (g == 0) {
       ml[wave][16 * nb + c][0] = m_run[nb];
       ml[wave][16 * nb + c][1] = l;
@@ -270,7 +310,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
     for (int w = 0; w < NW; ++w)
       l[nb] += ml[w][16 * nb + c][1] * __builtin_amdgcn_exp2f(ml[w][16 * nb + c][0] - mu);
     float own = __builtin_amdgcn_exp2f(m_run[nb] - mu);
-    if constexpr (F) own *= vref;
+    if constexpr (F) own *= vref * Kv8F16::UNIT;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll

@@ -101,6 +101,25 @@ struct Mma16<F16> {
   }
 };
 
+// How softmax weights become f16 operands that lose no more than the rounding to
+// f16 does, whatever scales the values have.  A weight is e = 2^(score - m), with m
+// the running maximum rounded up to a whole number, so at most 1; it is kept as
+// 2^15 e (with m whole the subtraction in the exponent stays exact), which takes
+// f16's range of 2^-25 to 2^-40.  Sums over keys are relative to the largest V scale
+// met, up to 2^8 (fp32 then holds them for all scales that are written), and a
+// weight may be multiplied by its V scale over that before it is rounded, as long as
+// the quotient takes no more than the 15 bits.  Where it does, the 16 keys' product
+// has an accumulator of its own that is multiplied in fp32: a page of large values
+// that a row does not see, or gives no weight, so costs the others' weights nothing.
+struct Kv8F16 {
+  static constexpr float BITS = 15.f, UNIT = 0x1p-15f;
+  static __device__ __forceinline__ float ref(float top) { return fminf(top, 0x1p8f); }
+  // (just over 1 may be a quotient's rounding, and 2^15 x 1.5 still is an f16)
+  static __device__ __forceinline__ bool apart(float f) {
+    return f > 1.5f || (f < UNIT && f > 0.f);
+  }
+};
+
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Four codes to floats and back (to nearest, ties to even; the caller has
 // scaled to |x| <= 448, NaN becomes the NaN code).
