@@ -170,9 +170,12 @@ def width_for(s_new, group, hk, page, wide):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("wide", [False, True])  # the kernel of few rows, and that of prompts
 @pytest.mark.parametrize("new,past,h,hk,d,page", [SHAPES[i] for i in (1, 3, 6, 8, 10, 12, 13, 17)])
-def test_each_row_by_its_own_values(new, past, h, hk, d, page, dtype):
-    s = Setup(new, past, h, hk, d, page, dtype, seed=5).fill()
+def test_each_row_by_its_own_values(new, past, h, hk, d, page, wide, dtype):
+    if wide and sum(new) * h // hk <= 64 * len(new):
+        pytest.skip("few rows at any width")
+    s = Setup(new, past, h, hk, d, page, dtype, seed=5, width=width_for(new, h // hk, hk, page, wide)).fill()
     check(s, attend(s))
     for i in range(s.pages):
         s.cache[3][i] *= 2.0 ** (i % 5)
@@ -181,7 +184,7 @@ def test_each_row_by_its_own_values(new, past, h, hk, d, page, dtype):
 
 @pytest.mark.parametrize("dtype,ratio", [(torch.float16, 4), (torch.float16, 14), (torch.float16, 20),
                                          (torch.float16, 30), (torch.bfloat16, 20), (torch.bfloat16, 130)])
-@pytest.mark.parametrize("new,wide", [(1, False), (8, False), (90, False)])
+@pytest.mark.parametrize("new,wide", [(1, False), (8, False), (90, False), (90, True)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_a_large_page_of_no_weight(d, new, wide, dtype, ratio):
     """A page whose values are larger by 2^ratio, and whose scores are so low that the
@@ -200,7 +203,7 @@ def test_a_large_page_of_no_weight(d, new, wide, dtype, ratio):
 
 @pytest.mark.parametrize("dtype,ratio", [(torch.float16, 10), (torch.float16, 20), (torch.float16, 28),
                                          (torch.bfloat16, 20), (torch.bfloat16, 130)])
-@pytest.mark.parametrize("wide", [False])
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("d", [64, 128])
 def test_rows_in_front_of_a_large_page(d, wide, dtype, ratio):
     """Queries that end before a page of large values, in the same tile of keys."""

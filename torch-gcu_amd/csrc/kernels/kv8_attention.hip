@@ -19,7 +19,7 @@
 //
 // The scales multiply scores (K) and weights (V) in fp32: one scalar per 16
 // keys, since a page holds a multiple of 16.  P is rounded to the input type; for
-// f16 as Kv8F16 says.
+// f16 as Kv8Weight says.
 //
 // Work: kv8_plan cuts each sequence's keys into parts so that all sequences
 // together make a few blocks per CU, whatever their lengths; the device reads
@@ -48,7 +48,8 @@ struct RowsTile {
 template <typename T, int D, int NB, int NW, bool ONCE>
 __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   typedef typename AttnOp<T>::vec vec;
-  constexpr bool F = std::is_same<T, F16>::value;
+  typedef Kv8Weight<T> Wt;
+  constexpr bool F = Wt::F;
   constexpr int RT = 16 * NB, KS = D / 32, DT = D / 16, W = D / 64;
   __shared__ float red[NW * NB * DT * 4 * 64];
   __shared__ float ml[NW][RT][3];
@@ -141,7 +142,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
     float vs[2] = {x.ok[0] ? x.vs[0] : 0.f, x.ok[1] ? x.vs[1] : 0.f};
     bool apart[2] = {false, false};
     if constexpr (F) {
-      const float top = wave_uniform_f32(Kv8F16::ref(fmaxf(vs[0], vs[1])));
+      const float top = wave_uniform_f32(Wt::ref(fmaxf(vs[0], vs[1])));
       if (top > vref) {
         const float r = wave_uniform_f32(vref * __builtin_amdgcn_rcpf(top));
         vref = top;
@@ -154,7 +155,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         vs[t] = wave_uniform_f32(vs[t] * inv);
-        apart[t] = Kv8F16::apart(vs[t]);
+        apart[t] = Wt::apart(vs[t]);
       }
     }
     vec kf[2][KS];
@@ -186,7 +187,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
       float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                        fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
       mx = half_max(row_max(mx));
-      if constexpr (F) mx = ceilf(mx);
+      mx = Wt::top(mx);
       if (mx > m_run[nb]) {
         const float corr = __builtin_amdgcn_exp2f(m_run[nb] - mx);
         m_run[nb] = mx;
@@ -194,7 +195,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[nb][i] *= corr;
       }
-      const float m_use = m_run[nb] == -INFINITY ? 0.f : F ? m_run[nb] - Kv8F16::BITS : m_run[nb];
+      const float m_use = Wt::offset(m_run[nb]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[nb][i] = __builtin_amdgcn_exp2f(s[i] - m_use);
@@ -290,8 +291,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
   // merge the waves: common max, scaled sums, O added in wave order
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    float l = half_sum(row_sum(l_run[nb]));
-    if constexpr (F) l *= Kv8F16::UNIT;
+    const float l = half_sum(row_sum(l_run[nb])) * Wt::UNIT;
     if (g == 0) {
       ml[wave][16 * nb + c][0] = m_run[nb];
       ml[wave][16 * nb + c][1] = l;
@@ -310,7 +310,7 @@ __device__ __forceinline__ void rows_item(const Kv8Args& a) {
     for (int w = 0; w < NW; ++w)
       l[nb] += ml[w][16 * nb + c][1] * __builtin_amdgcn_exp2f(ml[w][16 * nb + c][0] - mu);
     float own = __builtin_amdgcn_exp2f(m_run[nb] - mu);
-    if constexpr (F) own *= vref * Kv8F16::UNIT;
+    if constexpr (F) own *= vref * Wt::UNIT;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll

@@ -101,22 +101,33 @@ struct Mma16<F16> {
   }
 };
 
-// How softmax weights become f16 operands that lose no more than the rounding to
-// f16 does, whatever scales the values have.  A weight is e = 2^(score - m), with m
-// the running maximum rounded up to a whole number, so at most 1; it is kept as
-// 2^15 e (with m whole the subtraction in the exponent stays exact), which takes
-// f16's range of 2^-25 to 2^-40.  Sums over keys are relative to the largest V scale
-// met, up to 2^8 (fp32 then holds them for all scales that are written), and a
-// weight may be multiplied by its V scale over that before it is rounded, as long as
-// the quotient takes no more than the 15 bits.  Where it does, the 16 keys' product
-// has an accumulator of its own that is multiplied in fp32: a page of large values
-// that a row does not see, or gives no weight, so costs the others' weights nothing.
-struct Kv8F16 {
-  static constexpr float BITS = 15.f, UNIT = 0x1p-15f;
-  static __device__ __forceinline__ float ref(float top) { return fminf(top, 0x1p8f); }
-  // (just over 1 may be a quotient's rounding, and 2^15 x 1.5 still is an f16)
+// How softmax weights become 16-bit operands that lose no more than a rounding to
+// the type does, whatever scales the values have.  Sums over keys are relative to
+// the largest V scale met (up to MOST, so that fp32 holds them beside the smallest
+// one), and a weight may be multiplied by its V scale over that before it is rounded,
+// while the quotient leaves the type's range as it is.  Where it does not, the 16
+// keys' product has an accumulator of its own that is multiplied in fp32: a page of
+// large values that a row does not see, or gives no weight, so costs the other
+// weights nothing.
+//   f16: a weight is e = 2^(score - m), with m the running maximum rounded up to a
+// whole number, so at most 1; it is kept as 2^15 e (with m whole the subtraction in
+// the exponent stays exact), which takes the least f16 of 2^-25 to 2^-40, and the
+// quotient may take those 15 bits again.
+//   bf16 has fp32's range: quotients down to 2^-60 leave weights from 2^-66 on whole.
+template <typename T>
+struct Kv8Weight {
+  static constexpr bool F = std::is_same<T, F16>::value;
+  static constexpr float BITS = F ? 15.f : 0.f, UNIT = F ? 0x1p-15f : 1.f;
+  static constexpr float MOST = F ? 0x1p8f : 0x1p60f, LEAST = F ? UNIT : 0x1p-60f;
+  // the running maximum for a new largest score (base 2), and what is subtracted
+  static __device__ __forceinline__ float top(float mx) { return F ? ceilf(mx) : mx; }
+  static __device__ __forceinline__ float offset(float m) {
+    return m == -INFINITY ? 0.f : F ? m - BITS : m;
+  }
+  static __device__ __forceinline__ float ref(float scale) { return fminf(scale, MOST); }
+  // (f16: just over 1 may be a quotient's rounding, and 2^15 x 1.5 still is a number)
   static __device__ __forceinline__ bool apart(float f) {
-    return f > 1.5f || (f < UNIT && f > 0.f);
+    return (F && f > 1.5f) || (f < LEAST && f > 0.f);
   }
 };
 

@@ -17,7 +17,7 @@
 // fragment reads conflict.  One barrier a tile.
 // A key's scale multiplies its scores inside the exponent's FMA (one scalar per
 // 16 keys); a value's scale multiplies the weights, and only where it differs
-// from the largest one met so far, which the accumulators are relative to.
+// from the one that the accumulators are relative to (Kv8Weight).
 #include <algorithm>
 
 #include "kv8_combine.h"
@@ -35,6 +35,7 @@ __device__ __forceinline__ int swz_vt(int d) {
 template <typename T, int D, int NW>
 __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   typedef typename AttnOp<T>::vec vec;
+  typedef Kv8Weight<T> Wt;
   constexpr int RT = 32 * NW, NT = 64 * NW;
   constexpr int KS = D / 16, DT = D / 32;
   constexpr int VU = D / 4 * 8;              // V units: 4 d of 8 keys
@@ -43,7 +44,9 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
   __shared__ __align__(16) uint16_t kt[2][PKT * D];
   __shared__ __align__(16) uint16_t vt[2][PKT * D];
   __shared__ __align__(16) float scales[2][8];  // of a tile's 16-key groups: scores', values'
-  __shared__ int absent[2];                     // bit g: group g does not exist
+  // of a tile: the largest V scale and the least that is not 0, the scale of all
+  // groups or -1, and as an int, bit g: group g does not exist
+  __shared__ __align__(16) float about[2][4];
 
   Kv8Item it;
   if (!kv8_item<RT, PKT, true>(a, blockIdx.x, &it)) return;
@@ -130,9 +133,17 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
       const float k = scale * s_k;
       // masked scores stay -inf when multiplied by it
       scales[buf][tid] = !s_ok || k < 0x1p-100f ? 0x1p-100f : k;
-      scales[buf][4 + tid] = s_ok ? s_v : 0.f;
-      const uint64_t gone = __ballot(!s_ok);
-      if (tid == 0) absent[buf] = (int)gone;
+      const float v = s_ok ? s_v : 0.f;
+      scales[buf][4 + tid] = v;
+      const int gone = (int)__ballot(!s_ok);
+      const bool even = __ballot(v == wave_uniform_f32(v)) == 15;
+      float large = fmaxf(v, dpp_f32<0xB1>(v));
+      large = fmaxf(large, dpp_f32<0x4E>(large));
+      float least = v > 0.f ? v : large;
+      least = fminf(least, dpp_f32<0xB1>(least));
+      least = fminf(least, dpp_f32<0x4E>(least));
+      if (tid == 0)
+        *(f32x4*)about[buf] = f32x4{large, least, even ? v : -1.f, __builtin_bit_cast(float, gone)};
     }
     if (has_k) {
 #pragma unroll
@@ -175,7 +186,7 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
-  float vref = 0x1p-126f;  // the largest V scale met; o holds sums over it
+  float vref = 0x1p-126f;  // o holds sums over it
 
   if (lo < hi) {
     entries(lo);
@@ -209,7 +220,9 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
     entries(j + 3);
     if (key0 < w_most) {
       const f32x4 sc = *(const f32x4*)scales[buf], vs = *(const f32x4*)(scales[buf] + 4);
-      const int gone = wave_uniform(absent[buf]);
+      const f32x4 ab = *(const f32x4*)about[buf];
+      const float large = ab[0], least = ab[1], even = ab[2], bits = ab[3];
+      const int gone = wave_uniform(__builtin_bit_cast(int, bits));
       f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
       for (int t = 0; t < KS; ++t) {
@@ -243,8 +256,8 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
         for (int r = 1; r < 8; ++r) x = fmaxf(x, s[g >> 1][8 * (g & 1) + r]);
         mx = fmaxf(mx, x * sc[g]);
       }
-      mx = half_max(mx);
-      const float top = wave_uniform_f32(fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3])));
+      mx = Wt::top(half_max(mx));
+      const float top = wave_uniform_f32(Wt::ref(large));
       float corr = 1.f;
       if (top > vref) {
         corr = vref * __builtin_amdgcn_rcpf(top);
@@ -260,10 +273,9 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[i][r] *= corr;
       }
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      const float m_use = Wt::offset(m_run);
       float ls[4] = {0.f, 0.f, 0.f, 0.f};
-      const bool plain =
-          wave_uniform(vs[0] == vref && vs[1] == vref && vs[2] == vref && vs[3] == vref) != 0;
+      const bool plain = wave_uniform(even == vref) != 0;
       f32x8 p[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g)
@@ -277,8 +289,26 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
       if (!plain) {
         float inv = __builtin_amdgcn_rcpf(vref);
         asm volatile("" : "+v"(inv));  // the products below stay in this branch
+        f32x4 f = vs * inv;
+        if (wave_uniform(Wt::apart(least * inv) || Wt::apart(large * inv))) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) p[g] *= vs[g] * inv;
+          for (int g = 0; g < 4; ++g) {
+            if (!wave_uniform(Wt::apart(f[g]))) continue;
+            const vec own = __builtin_convertvector(p[g], vec);  // the 16 keys by themselves
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+              const int d = 32 * i + col;
+              const vec vf = *(const vec*)(vt[buf] + d * PKT + 8 * ((2 * g + half) ^ swz_vt<D>(d)));
+              const f32x16 x = AttnOp<T>::mma(vf, own, f32x16{});
+#pragma unroll
+              for (int r = 0; r < 16; ++r) o[i][r] = __builtin_fmaf(x[r], f[g], o[i][r]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            f[g] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) p[g] *= f[g];
       }
       vec pk[4];
 #pragma unroll
@@ -300,12 +330,12 @@ __device__ __forceinline__ void prompt_item(const Kv8Args& a) {
     }
   }
 
-  const float l = half_sum(l_run);
+  const float l = half_sum(l_run) * Wt::UNIT;
   if (row >= rows) return;
   const bool whole = it.parts == 1;
   if (!whole && (int)blockIdx.x >= a.slots) return;
   const int64_t at = (int64_t)blockIdx.x * RT + 32 * wave + col;
-  const float f = whole ? (l == 0.f ? 0.f : vref / l) : vref;
+  const float unit = vref * Wt::UNIT, f = whole ? (l == 0.f ? 0.f : unit / l) : unit;
 #pragma unroll
   for (int i = 0; i < DT; ++i)
 #pragma unroll
