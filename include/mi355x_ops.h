@@ -497,7 +497,9 @@ mi_status_t mi_layer_norm_backward(const mi_tensor_t* grad_input,
  *   k, v              uint8   [pages, heads, page, head_dim]; head_dim 64 or
  *                     128, page a power of two from 16 to 256; a page's head
  *                     dense and 16-byte aligned, pages and heads at any
- *                     non-overlapping strides
+ *                     non-overlapping strides; for the calls that write them k
+ *                     and v (and the two scales) share no memory, but may lie
+ *                     among each other in one pool with the same strides
  *   k_scale, v_scale  float32 [pages, heads]
  *
  * A call is about sequences b = 0 .. B - 1:

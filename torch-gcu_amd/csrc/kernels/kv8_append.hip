@@ -170,7 +170,7 @@ extern "C" mi_status_t mi_kv8_append(const mi_kv8_cache_t* cache, const mi_tenso
   int64_t dim = 0;
   a.group = 1;
   MI_RETURN_IF(kv8_check_cache(op, cache, &a.c, &dim));
-  MI_RETURN_IF(kv8_check_written(op, a.c));
+  MI_RETURN_IF(kv8_check_written(op, a.c, dim));
   MI_RETURN_IF(validate(k, "k"));
   MI_RETURN_IF(validate(v, "v"));
   for (const mi_tensor_t* t : {k, v}) {

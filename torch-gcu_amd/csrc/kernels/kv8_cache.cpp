@@ -29,6 +29,33 @@ bool kv8_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t extent) {
   return s1 >= extent && s0 >= (__int128)(n1 - 1) * s1 + extent;
 }
 
+bool kv8_disjoint(const Kv8Rows& a, const Kv8Rows& b, int64_t extent) {
+  const __int128 a0 = (uintptr_t)a.data, b0 = (uintptr_t)b.data;
+  auto end = [&](const Kv8Rows& x, __int128 at) {
+    return at + (__int128)(x.n0 - 1) * x.s0 + (__int128)(x.n1 - 1) * x.s1 + extent;
+  };
+  if (a.n0 < 1 || a.n1 < 1 || b.n0 < 1 || b.n1 < 1 || end(a, a0) <= b0 || end(b, b0) <= a0)
+    return true;
+  // rows of one lie among those of the other: with the same strides they meet where
+  // some steps of the two make up the distance, to less than a row
+  if (a.n0 != b.n0 || a.n1 != b.n1 || (a.n0 > 1 && a.s0 != b.s0) || (a.n1 > 1 && a.s1 != b.s1))
+    return false;
+  int64_t few = a.n0, step = a.s0, many = a.n1, stride = a.s1;
+  if (few > many) {
+    std::swap(few, many);
+    std::swap(step, stride);
+  }
+  for (int64_t i = 1 - few; i < few; ++i) {
+    const __int128 left = b0 - a0 - (__int128)i * step;
+    const __int128 near = many > 1 && stride > 0 ? left / stride : 0;
+    for (__int128 j = near - 1; j <= near + 1; ++j) {
+      const __int128 off = left - j * stride;
+      if (j > -many && j < many && off > -extent && off < extent) return false;
+    }
+  }
+  return true;
+}
+
 mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cache* c,
                             int64_t* dim) {
   MI_CHECK_ARG(cache != nullptr, "%s: cache is NULL", op);
@@ -86,9 +113,14 @@ mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cach
   return MI_OK;
 }
 
-mi_status_t kv8_check_written(const char* op, const Kv8Cache& c) {
-  MI_CHECK_ARG(c.k != c.v && c.k_scale != c.v_scale, "%s: k and v of the cache are the same memory",
-               op);
+mi_status_t kv8_check_written(const char* op, const Kv8Cache& c, int64_t dim) {
+  const int64_t n = sizeof(float);
+  const Kv8Rows k{c.k, c.pages, c.k_sp, c.heads, c.k_sh};
+  const Kv8Rows v{c.v, c.pages, c.v_sp, c.heads, c.v_sh};
+  const Kv8Rows ks{c.k_scale, c.pages, n * c.ks_sp, c.heads, n * c.ks_sh};
+  const Kv8Rows vs{c.v_scale, c.pages, n * c.vs_sp, c.heads, n * c.vs_sh};
+  MI_CHECK_ARG(kv8_disjoint(k, v, dim << c.shift) && kv8_disjoint(ks, vs, n),
+               "%s: k and v of the cache are the same memory", op);
   return MI_OK;
 }
 

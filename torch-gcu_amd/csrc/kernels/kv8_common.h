@@ -385,8 +385,16 @@ __device__ __forceinline__ void kv8_rest(const Kv8Args& a) {
 // after the other with either index as the outer one.
 bool kv8_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t extent);
 mi_status_t kv8_check_cache(const char* op, const mi_kv8_cache_t* cache, Kv8Cache* c, int64_t* dim);
+// Rows of `extent` bytes at two strides, in bytes, and whether no row of one tensor
+// shares memory with one of another.  They may lie among each other where their
+// strides are the same (k and v by turns in one pool).
+struct Kv8Rows {
+  const void* data;
+  int64_t n0, s0, n1, s1;
+};
+bool kv8_disjoint(const Kv8Rows& a, const Kv8Rows& b, int64_t extent);
 // for calls that write it
-mi_status_t kv8_check_written(const char* op, const Kv8Cache& c);
+mi_status_t kv8_check_written(const char* op, const Kv8Cache& c, int64_t dim);
 mi_status_t kv8_check_queries(const char* op, const mi_tensor_t* q, const mi_tensor_t* lse,
                               int64_t dim, Kv8Args* a);
 mi_status_t kv8_check_seqs(const char* op, const mi_tensor_t* table, const mi_tensor_t* lengths,

@@ -286,7 +286,7 @@ extern "C" mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor
   int64_t dim = 0;
   a.group = 1;
   MI_RETURN_IF(kv8_check_cache(op, cache, &a.c, &dim));
-  MI_RETURN_IF(kv8_check_written(op, a.c));
+  MI_RETURN_IF(kv8_check_written(op, a.c, dim));
   MI_RETURN_IF(kv8_check_seqs(op, block_table, lengths, nullptr, 0, &a));
   MI_RETURN_IF(kv8_check_weights(op, weights, "weights", a));
   MI_RETURN_IF(kv8_check_weights(op, new_weights, "new_weights", a));
@@ -309,8 +309,12 @@ extern "C" mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor
                    (a.seqs <= 1 || new_lengths->strides[0] == 1),
                "%s: new_lengths must be a dense int32 vector of the sequences", op);
   // blocks read the old ones while others write
-  MI_CHECK_ARG(a.seqs == 0 || (new_lengths->data != lengths->data &&
-                               new_weights->data != weights->data),
+  auto rows = [](const mi_tensor_t* t) {
+    return Kv8Rows{t->data, t->sizes[0], 4 * t->strides[0], t->sizes[1], 4 * t->strides[1]};
+  };
+  MI_CHECK_ARG(kv8_disjoint({new_lengths->data, 1, 0, 1, 0}, {lengths->data, 1, 0, 1, 0},
+                            4 * (int64_t)a.seqs) &&
+                   kv8_disjoint(rows(new_weights), rows(weights), 4 * weights->sizes[2]),
                "%s: new_lengths and new_weights need memory of their own", op);
   if (a.seqs > 32767) MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 32767 sequences", op);
   if (a.seqs == 0) return MI_OK;
