@@ -513,7 +513,8 @@ mi_status_t mi_layer_norm_backward(const mi_tensor_t* grad_input,
  * bounds is touched whatever they hold: a length outside [0, W page] makes the
  * sequence empty, a page outside the pool is not written and not seen, starts
  * are clamped to the tokens; the first two are recorded for
- * mi_index_fault_take.  Only entries for positions below lengths[b] are read. */
+ * mi_index_fault_take.  What block_table holds for positions from lengths[b] on
+ * is of no account. */
 typedef struct {
   mi_tensor_t k;
   mi_tensor_t v;
@@ -539,7 +540,9 @@ mi_status_t mi_kv8_append(const mi_kv8_cache_t* cache, const mi_tensor_t* k,
  * log of the softmax sums.  A token that sees nothing has out 0 and lse -inf.
  * q and out bf16 or f16 [tokens, H, head_dim].  Rows of no sequence are left as
  * they were, or with fill_rest set to 0 and -inf.  fp32 scores, sums and
- * accumulation; softmax weights are rounded to q's type.  Partial sums of cut
+ * accumulation; softmax weights are rounded to q's type (f16: under its normal
+ * range by at most 2^-25 of the row's largest), whatever scales the values have.
+ * Partial sums of cut
  * sequences take workspace; nothing is cut when there is none. */
 mi_status_t mi_kv8_attention(const mi_tensor_t* out, const mi_tensor_t* lse,
                              const mi_tensor_t* q, const mi_kv8_cache_t* cache,
@@ -561,7 +564,8 @@ mi_status_t mi_kv8_weigh(const mi_tensor_t* weights, const mi_tensor_t* q,
  * the last `recent`, and the others of largest weight (ties: the lower
  * position; NaN counts as no weight), in their order.  They are written to the
  * pages of new_table (int32 [B, >= ceil(keep / page)]), none named twice and
- * none by a block_table row of the call; the old pages stay as they were.  kept
+ * none by a block_table row of the call; the old pages stay as they were, and
+ * tokens of a page outside the pool become zeros.  kept
  * int32 [B, heads, keep] the old positions, then -1; new_lengths int32 [B];
  * new_weights like weights, the kept ones, then 0; the last two in memory of
  * their own. */

@@ -26,8 +26,8 @@
 // the lengths, so a captured call follows them.  A block's waves take 32-key
 // tiles in turn, never wait for each other, and are merged through LDS; parts
 // are merged by kv8_combine_kernel in a fixed order.  32 query heads on 8 of 128:
-// 32 sequences of 4000 to 16000 118 us (648 MB, 5.5 TB/s), 8 of 4000 15 us and
-// the merge's 4 (65.7 MB, 3.4 TB/s together), 1 of 301 7 us.
+// 32 sequences of 4000 to 16000 118 us (648 MB, 5.5 TB/s), 8 of 4000 16 us and
+// the merge's 4 (65.7 MB, 3.3 TB/s together), 1 of 301 7 us.
 #include <algorithm>
 
 #include "kv8_combine.h"
@@ -366,7 +366,9 @@ __global__ __launch_bounds__(64 * NW, 4) void kv8_rows_kernel(Kv8Args a) {
 template <typename T, int D>
 mi_status_t run_rows(Kv8Args& a, hipStream_t s) {
   constexpr int NB = 1, NW = 8;
-  // Two blocks of eight waves per CU, and twice as many parts where they are long
+  // (The rules here and in mi_kv8_attention go by the table's width, since the host
+  // does not know the lengths; the times are those of tables as wide as the longest
+  // sequence.)  Two blocks of eight waves per CU, and twice as many parts where they are long
   // enough that the last ones to end count (32 sequences of 4000 to 16000: 130 ->
   // 119 us).  A part is at least a tile per wave, and short sequences stay whole,
   // since the merge is a launch of 4 us: up to 1024 positions (1 of 300: 13 -> 8

@@ -13,7 +13,7 @@
 // bounds the pair: the latency of the selection's passes for few sequences, the
 // gathered bytes for many.  8 heads of 128: 16 sequences of 4000 to 16000 cut to
 // 2000 tokens, 18 us for the selection and 24 for the moves (131 MB, 5.4 TB/s);
-// 1 of 1000 cut to 250, 8.2 and 4.
+// 1 of 1000 cut to 250, 8.7 and 4.
 #include <algorithm>
 
 #include "kv8_common.h"

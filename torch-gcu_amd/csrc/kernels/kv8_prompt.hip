@@ -1,11 +1,13 @@
 // Attention of many query rows per sequence (pieces of prompts) over the 8-bit
 // cache.
 //
-// What bounds it: 4 D flops per query row and key on the matrix instructions,
-// and beside them more time of exp2, maxima and sums on the vector unit.  32 query
-// heads on 8 of 128: 2048 tokens behind 14000 546 us (924 TFLOP/s where a large
-// product reaches 1426; matrix instructions 37 % of the cycles), 2783 tokens of
-// four sequences behind 359 to 823 82 us (527: 704 blocks on 512 places).
+// What bounds it: 4 D flops per query row and key on the matrix instructions, and
+// more time of exp2, maxima and sums on the vector unit, one after the other: the
+// barrier of a tile keeps a SIMD's waves in the same phase.  32 query heads on 8 of
+// 128: 2048 tokens behind 14000 546 us (924 TFLOP/s where a large product reaches
+// 1426; matrix instructions 4.8e5 and vector ones 6.5e5 cycles a SIMD of 1.15e6),
+// 2783 tokens of four sequences behind 359 to 823 82 us (527: 704 blocks on 512
+// places).
 //   A block takes 32 NW query rows of one k/v head (the group's heads of
 // consecutive tokens), a wave 32 of them, and walks the keys in tiles of 64:
 //   S^T = K Q^T, O^T = V^T P^T (v_mfma_f32_32x32x16), P^T taken from the S^T
@@ -386,7 +388,8 @@ mi_status_t run_prompt(Kv8Args& a, hipStream_t s) {
     a.plan = {cus, 0x40000000, 24, cus};
     return kv8_launch<T, D, 256, PKT, true>(a, kv8_prompt_kernel<T, D, 8>, 512, s);
   }
-  // A block per CU where its tiles are few: two share a CU at 2.6 us a tile of
+  // (tiles of the table's width, as wide as the longest sequence in these times)  A
+  // block per CU where its tiles are few: two share a CU at 2.6 us a tile of
   // each, one alone takes 1.7 to 2, and a part more costs 8 us and its partials
   // (32 sequences of 512, 32 new tokens each: 28 us uncut, 47 in halves; 1 of
   // 16128, 128 new: 89 us with a block per CU, 67 with two; 16 heads of 64, 4 x up to

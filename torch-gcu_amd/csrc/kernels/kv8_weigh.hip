@@ -15,7 +15,8 @@
 //     lane adds its 16 keys' weights over all rows of its column before the 32
 //     columns are added at the end.
 // 32 query heads on 8 of 128: 8 sequences of 4000, a token each 10 us (34.9 MB, 3.5
-// TB/s); 2 of 4333, 333 tokens each 40 us (567 TFLOP/s: an exp2 and two more vector
+// TB/s: no load of a wave's next codes is in flight while a tile is computed); 2 of
+// 4333, 333 tokens each 40.5 us (560 TFLOP/s: an exp2 and two more vector
 // instructions a score take twice the products' time, and 544 blocks are two a CU
 // and three on some).
 #include <algorithm>
@@ -339,7 +340,8 @@ mi_status_t run_weigh(Kv8Args& a, const Kv8Weights& w, hipStream_t s) {
   const int64_t keys = (int64_t)a.width << a.c.shift, tile = WKT * WNW;
   const int64_t blocks = some * a.c.heads * ((keys + tile - 1) / tile);
   if (few) hipLaunchKernelGGL((kv8_weigh_rows_kernel<T, D>), grid, block, 0, s, a, w);
-  // A block walks all rows, and where the blocks of 128 keys leave CUs idle, smaller
+  // (by the table's width, as wide as the longest sequence in these times)  A block
+  // walks all rows, and where the blocks of 128 keys leave CUs idle, smaller
   // ones with waves that share the rows walk faster, at twice (four times) the
   // copies.  us, one, two and four waves to 32 keys, 32 query heads on 8 of 128: 64
   // tokens behind 500 (40 blocks of 128 keys) 9.6 / 8.9 / 8.9, 333 behind 1000 (88)
