@@ -169,12 +169,13 @@ def width_for(s_new, group, hk, page, wide):
     return wide_table(sum(s_new) * group, hk, page) if wide else 0
 
 
+BY_ROW = [(False, *SHAPES[i]) for i in (1, 3, 6, 8, 10, 12, 13, 17)]  # by the kernel of few rows
+BY_ROW += [(True, *SHAPES[i]) for i in (10, 12, 13, 17)]  # by that of prompts
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-@pytest.mark.parametrize("wide", [False, True])  # the kernel of few rows, and that of prompts
-@pytest.mark.parametrize("new,past,h,hk,d,page", [SHAPES[i] for i in (1, 3, 6, 8, 10, 12, 13, 17)])
-def test_each_row_by_its_own_values(new, past, h, hk, d, page, wide, dtype):
-    if wide and sum(new) * h // hk <= 64 * len(new):
-        pytest.skip("few rows at any width")
+@pytest.mark.parametrize("wide,new,past,h,hk,d,page", BY_ROW)
+def test_each_row_by_its_own_values(wide, new, past, h, hk, d, page, dtype):
     s = Setup(new, past, h, hk, d, page, dtype, seed=5, width=width_for(new, h // hk, hk, page, wide)).fill()
     check(s, attend(s))
     for i in range(s.pages):
