@@ -80,13 +80,13 @@ SHARED = [
     # offset of v, strides: pages or heads of one on those of the other
     (0, None), (16, None), (1008, None), (1024, None), (2048, None), (3 * 2048 - 16, None),
     (1008, (4096, 2048, 64, 1)), (2048, (4096, 2048, 64, 1)), (4096 + 2048, (4096, 2048, 64, 1)),
-    (3072 + 16, (6144, 2048, 64, 1)), (1024, (1024, 4096, 64, 1)),
+    (1040, (6144, 2048, 64, 1)), (1024, (1024, 4096, 64, 1)),
 ]
 APART = [
     (3 * 2048, None), (1024, (4096, 2048, 64, 1)),          # behind, by turns head by head
     (2048, (4096, 1024, 64, 1)),                            # page by page
     (5120, (4096, 2048, 64, 1)),                            # a page later, the odd heads
-    (3072, (1024, 6144, 64, 1)),                            # heads outside pages
+    (4096, (1024, 8192, 64, 1)),                            # heads outside pages
 ]
 
 
