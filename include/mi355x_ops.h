@@ -576,6 +576,56 @@ mi_status_t mi_kv8_evict(const mi_kv8_cache_t* cache, const mi_tensor_t* weights
                          const mi_tensor_t* new_lengths,
                          const mi_tensor_t* new_weights, mi_stream_t stream);
 
+/* ---- linear layers in 8-bit floating point -----------------------------------
+ * No counterpart in the reference.  A matrix is held as e4m3 codes with
+ * power-of-two scales, one byte each: an element is code * 2^(byte - 127).
+ *
+ *   codes   uint8 [rows, columns], dense along columns
+ *   scales  uint8, of activations [rows, ceil(columns / 128)], one for each 128
+ *           columns of a row; of weights [ceil(rows / 128), ceil(columns / 128)],
+ *           one for each block of 128 x 128
+ *
+ * What is written has the smallest scale s >= 2^-110 with amax <= 448 s over the
+ * group's finite elements, and a code to nearest, ties to even; an element that
+ * is infinite or NaN becomes NaN.  Reading takes any byte (255 is NaN).  A NaN in
+ * a row of activations makes NaN of that row of the product, one in a weight's
+ * row of that column, and of nothing else.  Outputs share no memory with other
+ * tensors of the call unless said. */
+typedef struct {
+  mi_tensor_t codes;
+  mi_tensor_t scales;
+} mi_fp8_t;
+
+/* Activations x [rows, columns] (bf16, f16 or f32), and a weight, to codes and
+ * scales of theirs. */
+mi_status_t mi_fp8_quantize(const mi_fp8_t* out, const mi_tensor_t* x, mi_stream_t stream);
+mi_status_t mi_fp8_quantize_weight(const mi_fp8_t* out, const mi_tensor_t* weight, mi_stream_t stream);
+
+/* total = x + residual in the type of both, y = total * rsqrt(mean(total^2) +
+ * eps) * weight over rows of x [rows, columns] (bf16, f16 or f32), fp32 math; y as
+ * activations in out.  residual NULL: total is x, and nothing is written to total
+ * (which may be NULL); total may be x or the residual itself.  weight of x's type,
+ * a dense vector, or NULL. */
+mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const mi_tensor_t* x,
+                            const mi_tensor_t* residual, const mi_tensor_t* weight, double eps,
+                            mi_stream_t stream);
+
+/* out = x weight^T (+ bias) (+ residual), rounded once to out's type (bf16 or
+ * f16): x activations [M, K], weight [N, K], bias a dense vector of out's type or
+ * float32, residual of out's type, which may be out itself.  The products go
+ * through the scaled e4m3 matrix instructions and add up in fp32; one instruction
+ * adds 8 neighbours of K at a time with 13 bits below the largest of them, which
+ * is off by 1.5e-5 of a sum of normal numbers, a sixth of f16's rounding.  Rows of
+ * codes that are not 16-byte aligned are copied to workspace first; K is cut in
+ * slices, added in a fixed order, where tiles are few. */
+mi_status_t mi_fp8_linear(const mi_tensor_t* out, const mi_fp8_t* x, const mi_fp8_t* weight,
+                          const mi_tensor_t* bias, const mi_tensor_t* residual, mi_stream_t stream);
+
+/* out = silu(x w_gate^T) * (x w_up^T) as activations, computed in fp32 from the
+ * products' sums and rounded once, to the codes. */
+mi_status_t mi_fp8_linear_silu_mul(const mi_fp8_t* out, const mi_fp8_t* x, const mi_fp8_t* w_gate,
+                                   const mi_fp8_t* w_up, mi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -316,6 +316,17 @@ TORCH_LIBRARY(torch_gcu, m) {
       "kv8_evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale, "
       "Tensor weights, Tensor block_table, Tensor new_table, Tensor lengths, int keep, int recent, "
       "int sink=0) -> (Tensor, Tensor, Tensor)");
+  m.def("fp8_quantize(Tensor x) -> (Tensor, Tensor)");
+  m.def("fp8_quantize_weight(Tensor weight) -> (Tensor, Tensor)");
+  m.def(
+      "rms_norm_fp8(Tensor x, Tensor? weight, float eps=1e-06, Tensor? residual=None) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def(
+      "fp8_linear(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, Tensor? bias=None, "
+      "Tensor? residual=None, ScalarType? dtype=None) -> Tensor");
+  m.def(
+      "fp8_linear_silu_mul(Tensor x, Tensor x_scales, Tensor w_gate, Tensor gate_scales, Tensor w_up, "
+      "Tensor up_scales) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(torch_gcu, PrivateUse1, m) {
@@ -331,4 +342,9 @@ TORCH_LIBRARY_IMPL(torch_gcu, PrivateUse1, m) {
   m.impl("kv8_attention", TORCH_FN(torch_gcu::efficient::kv8_attention));
   m.impl("kv8_weigh_", TORCH_FN(torch_gcu::efficient::kv8_weigh_));
   m.impl("kv8_evict", TORCH_FN(torch_gcu::efficient::kv8_evict));
+  m.impl("fp8_quantize", TORCH_FN(torch_gcu::efficient::fp8_quantize));
+  m.impl("fp8_quantize_weight", TORCH_FN(torch_gcu::efficient::fp8_quantize_weight));
+  m.impl("rms_norm_fp8", TORCH_FN(torch_gcu::efficient::rms_norm_fp8));
+  m.impl("fp8_linear", TORCH_FN(torch_gcu::efficient::fp8_linear));
+  m.impl("fp8_linear_silu_mul", TORCH_FN(torch_gcu::efficient::fp8_linear_silu_mul));
 }

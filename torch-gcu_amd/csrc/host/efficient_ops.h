@@ -45,5 +45,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> kv8_evict(
     const at::Tensor& weights, const at::Tensor& block_table, const at::Tensor& new_table,
     const at::Tensor& lengths, int64_t keep, int64_t recent, int64_t sink);
 
+// linear layers in 8-bit floating point (fp8_ops.cpp)
+std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x);
+std::tuple<at::Tensor, at::Tensor> fp8_quantize_weight(const at::Tensor& weight);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_fp8(const at::Tensor& x,
+                                                            const std::optional<at::Tensor>& weight,
+                                                            double eps,
+                                                            const std::optional<at::Tensor>& residual);
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
+                      const at::Tensor& weight_scales, const std::optional<at::Tensor>& bias,
+                      const std::optional<at::Tensor>& residual, std::optional<at::ScalarType> dtype);
+std::tuple<at::Tensor, at::Tensor> fp8_linear_silu_mul(const at::Tensor& x, const at::Tensor& x_scales,
+                                                       const at::Tensor& w_gate,
+                                                       const at::Tensor& gate_scales,
+                                                       const at::Tensor& w_up,
+                                                       const at::Tensor& up_scales);
+
 }  // namespace efficient
 }  // namespace torch_gcu

@@ -1,0 +1,82 @@
+// Shared by the kernels of linear layers in 8-bit floating point: rows of e4m3
+// codes with a power-of-two scale for each 128 columns, weights with one for each
+// 128 x 128 block; a scale is its biased exponent, 2^(byte - 127), which is what the
+// scaled matrix instructions take.
+#pragma once
+
+#include <algorithm>
+#include <cmath>
+
+#include "gemm_common.h"
+
+namespace mi {
+
+constexpr int kFp8Group = 128;
+
+// One operand as a kernel reads (or writes) it: rows of codes and of scale bytes,
+// dense along columns.
+struct Fp8Mat {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t ld, sld;  // row strides, in bytes
+};
+
+inline int64_t fp8_groups(int64_t n) { return (n + kFp8Group - 1) / kFp8Group; }
+
+// Checks of the entry points (fp8_check.cpp); they read descriptors only.
+// codes uint8 [rows, cols] and scales uint8 [rows or its blocks, column groups],
+// dense along columns; written: rows of its own.
+mi_status_t fp8_check(const char* op, const char* name, const mi_fp8_t* t, bool weight, bool written,
+                      Fp8Mat* m);
+// [rows, cols] with unit column stride, of a 16-bit type (or float32 with f32)
+mi_status_t fp8_check_wide(const char* op, const char* name, const mi_tensor_t* t, bool f32);
+// INVALID where an output shares memory with another tensor of the call
+mi_status_t fp8_check_apart(const char* op, const char* name, const mi_tensor_t* out,
+                            const char* other_name, const mi_tensor_t* other);
+
+namespace {
+
+typedef uint32_t f8_u32x2 __attribute__((ext_vector_type(2)));
+constexpr uint32_t kFp8AbsMask = 0x7fffffffu, kFp8Inf = 0x7f800000u;
+
+// The scale byte of a group whose largest finite magnitude has these float bits:
+// the smallest power of two s >= 2^-110 with amax <= 448 s.  448 is 1.75 x 2^8, so the
+// exponent is amax's less 8, and one more where its mantissa is over 1.75.  (2^-110
+// keeps 1 / s and every product of it ordinary floats; the least is the 8-bit cache's.)
+__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax) {
+  const int e = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(e, 127 - 110);
+}
+// 1 / s, exact
+__device__ __forceinline__ float fp8_inverse(uint32_t byte) {
+  return __uint_as_float((254u - byte) << 23);
+}
+// The bits of |x| where x is finite, else 0: the largest of them is the largest
+// finite magnitude (floats that are not negative order as their bits do).
+__device__ __forceinline__ uint32_t fp8_finite_bits(float x) {
+  const uint32_t b = __float_as_uint(x) & kFp8AbsMask;
+  return b < kFp8Inf ? b : 0u;
+}
+// Four values times a power of two as codes, to nearest, ties to even; what is not
+// finite becomes NaN (e4m3 has no infinity).  The caller's scale keeps the finite ones
+// within 448.
+__device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
+  auto f = [&](float x) __attribute__((always_inline)) {
+    return (__float_as_uint(x) & kFp8Inf) == kFp8Inf ? NAN : x * inv;
+  };
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(f(a), f(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f(c), f(d), r, true);
+}
+
+// The largest over each row of 16 lanes, in all of them.
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  auto step = [&](uint32_t o) __attribute__((always_inline)) { v = v > o ? v : o; };
+  step((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));
+  step((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));
+  return v;
+}
+
+}  // namespace
+}  // namespace mi

@@ -1,0 +1,422 @@
+// The tile kernel of 8-bit floating point products, by block shapes (fp8_linear.hip
+// chooses one).
+#pragma once
+
+#include "fp8_common.h"
+#include "gemm_dl.h"
+
+namespace mi {
+
+struct Fp8Gemm {
+  Fp8Mat x, w, w2;     // activations [M][K], weight [N][K]; w2: the up weight of a gate
+  void* out;           // [M][ldc] bf16 or f16
+  int64_t ldc;
+  const void* bias;
+  int bias_dtype;
+  const uint16_t* res;
+  int64_t ldr;
+  Fp8Mat codes;        // a gate's output
+  float* part;         // [2 of a gate][slices][M][ldp] sums of K slices
+  int64_t ldp;
+  int M, N, K;
+  int f16;             // out, residual and 16-bit bias are f16
+  int tiles_m, tiles_n;
+};
+
+namespace {
+
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+
+// acc += a b^T over 128 of K: lane l holds 32 bytes of row l % 16 of each operand
+// (the same 32 of the 128 in both) and ends up with rows 4 (l / 16) + 0 .. 3 of
+// column l % 16.  A scale multiplies a lane's 32 products; here the four lanes of a
+// row give the same one.  (Format 0 is e4m3.)
+__device__ __forceinline__ f32x4_t mma_fp8(i32x8_t a, i32x8_t b, f32x4_t c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+
+// A byte a lane, from an address of its own, to a 32-bit word a lane at lds on (the
+// counterpart of lds_copy16).
+__device__ __forceinline__ void lds_copy_byte(const uint8_t* p, void* lds) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
+  asm volatile("s_nop 0\n\tglobal_load_lds_ubyte %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+}
+
+// silu(g) u and the largest finite magnitude's bits so far
+__device__ __forceinline__ float gate_of(float g, float u, uint32_t* most) {
+  const float y = silu_mul_f32(g, u);
+  *most = max(*most, fp8_finite_bits(y));
+  return y;
+}
+
+constexpr int F8_OUT = 0, F8_PART = 1, F8_GATE = 2, F8_GATE_PART = 3;
+
+// WM x WN waves of TM x TN outputs each, K steps of 128 through a ring of STAGES.
+template <int WM_, int WN_, int TM_, int TN_, int STAGES_>
+struct F8Cfg {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, STAGES = STAGES_;
+  static constexpr int NW = WM * WN, NT = 64 * NW, BM = WM * TM, BN = WN * TN;
+  static constexpr int FM = TM / 16, FN = TN / 16;
+  static constexpr int RB = FN < 4 ? FN : 4;  // weight fragments held
+  static constexpr int NQA = BM / 8 / NW, NQB = BN / 8 / NW;  // 1 KiB wave copies a step
+  static constexpr int NSB = (BM + BN) / 64, NQS = (NSB + NW - 1) / NW;
+  static constexpr int LPW = NQA + NQB + NQS;
+  static constexpr int TA = BM * 128, TB = BN * 128, TS = (BM + BN) * 4, STAGE = TA + TB + TS;
+  static constexpr int HC = TN < 64 ? TN : 64, EP = HC + 4;  // columns of an epilogue pass
+  static constexpr int CP = 128 + 16;                         // a gate's staged code rows
+  static constexpr size_t cmax(size_t a, size_t b) { return a > b ? a : b; }
+  static constexpr size_t LDS_BYTES =
+      cmax((size_t)STAGES * STAGE, cmax((size_t)NW * TM * EP * 4, (size_t)BM * CP + (size_t)WN * BM * 4));
+  static_assert(LDS_BYTES <= 160 * 1024 && NQA >= 1 && NQB >= 1 && FN % RB == 0, "shape");
+};
+
+template <class C, int EPI>
+__global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
+  constexpr int WN = C::WN, TM = C::TM, TN = C::TN, BM = C::BM, BN = C::BN, FM = C::FM, FN = C::FN;
+  constexpr int RB = C::RB, NQA = C::NQA, NQB = C::NQB, NQS = C::NQS, LPW = C::LPW, STAGES = C::STAGES;
+  constexpr int TA = C::TA, TB = C::TB, STAGE = C::STAGE, GROUP_M = 4;
+  constexpr bool GATE = EPI == F8_GATE || EPI == F8_GATE_PART;
+  constexpr bool SPLIT = EPI == F8_PART || EPI == F8_GATE_PART;
+  static_assert(EPI != F8_GATE || BN == 256, "a block holds whole groups of a gate's output");
+  extern __shared__ __align__(16) char smem[];
+  // XCD-aware tile order (blocks go round the 8 XCDs in turn), then groups of
+  // GROUP_M row panels, so the tiles an XCD runs together share panels
+  int tm, tn;
+  {
+    const int total = p.tiles_m * p.tiles_n;
+    int id = blockIdx.x;
+    if (total % 8 == 0) id = (id % 8) * (total / 8) + id / 8;
+    const int group = id / (GROUP_M * p.tiles_n), first = group * GROUP_M;
+    const int size = min(p.tiles_m - first, GROUP_M), in_group = id - group * GROUP_M * p.tiles_n;
+    tm = first + in_group % size;
+    tn = in_group / size;
+  }
+  const int M = p.M, N = p.N, K = p.K;
+  const int m0 = tm * BM, n0 = tn * (GATE ? BN / 2 : BN);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  int KT = K / 128, k_first = 0;
+  if constexpr (SPLIT) {
+    const int S = gridDim.y, s = blockIdx.y, base = KT / S, rem = KT % S;
+    k_first = s * base + min(s, rem);
+    KT = base + (s < rem ? 1 : 0);
+  }
+  // The weight row of row r of the B tile.  A gate's wave holds TN / 2 columns of
+  // the gate and the same of up, so a lane has both products of an output.
+  auto b_row = [&](int r) __attribute__((always_inline)) {
+    return GATE ? n0 + r / TN * (TN / 2) + r % (TN / 2) : n0 + r;
+  };
+  auto b_up = [&](int r) __attribute__((always_inline)) { return GATE && r % TN >= TN / 2; };
+  const uint8_t* A = p.x.codes + (int64_t)m0 * p.x.ld;
+  const uint8_t* B[2] = {p.w.codes + (int64_t)n0 * p.w.ld, GATE ? p.w2.codes + (int64_t)n0 * p.w2.ld : nullptr};
+  // byte offsets of a lane's 16 bytes of each copy (8 rows of 128 bytes), which fit 32
+  // bits; rows past the matrix read its last one and feed outputs that are not stored.
+  // LDS chunk c of row r holds the row's chunk dl_swz(r, c).
+  uint32_t ao[NQA], bo[NQB];
+#pragma unroll
+  for (int q = 0; q < NQA; ++q) {
+    const int r = (wave * NQA + q) * 8 + lane / 8;
+    ao[q] = (uint32_t)((min(m0 + r, M - 1) - m0) * p.x.ld + 16 * dl_swz(r, lane % 8));
+  }
+#pragma unroll
+  for (int q = 0; q < NQB; ++q) {
+    const int r = (wave * NQB + q) * 8 + lane / 8;
+    bo[q] = (uint32_t)((min(b_row(r), N - 1) - n0) * (b_up(r) ? p.w2.ld : p.w.ld) + 16 * dl_swz(r, lane % 8));
+  }
+  // the scale byte of row r of the two tiles (the B tile's behind the A tile's), at K step 0
+  auto scale_at = [&](int r) __attribute__((always_inline)) -> const uint8_t* {
+    if (r < BM) return p.x.scales + (int64_t)min(m0 + r, M - 1) * p.x.sld;
+    const int64_t n = min(b_row(r - BM), N - 1) / kFp8Group;
+    return b_up(r - BM) ? p.w2.scales + n * p.w2.sld : p.w.scales + n * p.w.sld;
+  };
+  const uint8_t* so[NQS];
+#pragma unroll
+  for (int q = 0; q < NQS; ++q) so[q] = scale_at((wave * NQS + q) % C::NSB * 64 + lane);
+  // copy q of K step kt (of this slice) into stage st
+  auto issue_one = [&](int st, int kt, int q) __attribute__((always_inline)) {
+    char* s = smem + st * STAGE;
+    const int64_t k = (int64_t)(k_first + kt) * 128;
+    if (q < NQA) {
+      lds_copy16(A + k, ao[q], s + (wave * NQA + q) * 1024);
+    } else if (q < NQA + NQB) {
+      const int c = wave * NQB + q - NQA;
+      lds_copy16((b_up(c * 8) ? B[1] : B[0]) + k, bo[q - NQA], s + TA + c * 1024);
+    } else {
+      const int c = (wave * NQS + q - NQA - NQB) % C::NSB;
+      lds_copy_byte(so[q - NQA - NQB] + k_first + kt, s + TA + TB + c * 256);
+    }
+  };
+  auto issue = [&](int st, int kt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < LPW; ++q) issue_one(st, kt, q);
+  };
+  // fragments: lane l reads row l % 16, chunks l / 16 and 4 + l / 16
+  const int row = lane & 15;
+  const int ro0 = row * 128 + 16 * dl_swz(row, lane >> 4), ro1 = row * 128 + 16 * dl_swz(row, 4 + (lane >> 4));
+  auto fragment = [&](const char* t) __attribute__((always_inline)) {
+    const u32x4_t lo = *(const u32x4_t*)(t + ro0), hi = *(const u32x4_t*)(t + ro1);
+    return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+  // acc[j][i]: outputs m = 16 i + l % 16, n = 16 j + 4 (l / 16) + 0 .. 3 of the wave's
+  f32x4_t acc[FN][FM];
+#pragma unroll
+  for (int j = 0; j < FN; ++j)
+#pragma unroll
+    for (int i = 0; i < FM; ++i) acc[j][i] = f32x4_t{};
+  i32x8_t af[FM], bf[RB];
+  int sa[FM], sb[2], sa_next[FM], sb_next[2];
+  auto read_a = [&](int st, int i) __attribute__((always_inline)) {
+    af[i] = fragment(smem + st * STAGE + (wm * TM + 16 * i) * 128);
+  };
+  auto read_b = [&](int st, int j) __attribute__((always_inline)) {
+    bf[j % RB] = fragment(smem + st * STAGE + TA + (wn * TN + 16 * j) * 128);
+  };
+  auto read_scales = [&](int st) __attribute__((always_inline)) {
+    const int* s = (const int*)(smem + st * STAGE + TA + TB);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sa_next[i] = s[wm * TM + 16 * i + row];
+#pragma unroll
+    for (int h = 0; h < (GATE ? 2 : 1); ++h) sb_next[h] = s[BM + wn * TN + h * (TN / 2)];
+  };
+  auto take_scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sa[i] = sa_next[i];
+    sb[0] = sb_next[0];
+    if constexpr (GATE) sb[1] = sb_next[1];
+  };
+  auto mfma_one = [&](int j, int i) __attribute__((always_inline)) {
+    acc[j][i] = mma_fp8(bf[j % RB], af[i], acc[j][i], sb[GATE && j >= FN / 2 ? 1 : 0], sa[i]);
+  };
+  auto first_reads = [&](int st) __attribute__((always_inline)) {
+    read_scales(st);
+#pragma unroll
+    for (int j = 0; j < RB - 1; ++j) read_b(st, j);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) read_a(st, i);
+    take_scales();
+  };
+  // One K step over stage st, a row of MFMAs (one weight fragment) at a time.  The weight
+  // fragment RB - 1 rows on is read at each row's start, the activations' of the next
+  // step during the last row, each behind its last use.  From row JB on the reads are
+  // the next step's: before it, that step's copies have to have landed, and behind the
+  // barrier no wave reads stage st again, so that its refill starts there.
+  constexpr int JB = FN - RB + 1, SLOTS = (FN - JB) * FM, PER = (LPW + SLOTS - 1) / SLOTS;
+  auto step = [&](int st, int kt, auto issue_c, auto next_c) __attribute__((always_inline)) {
+    constexpr bool ISSUE = decltype(issue_c)::value, NEXT = decltype(next_c)::value;
+    const int nst = st + 1 == STAGES ? 0 : st + 1;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      if (j == JB && NEXT) {
+        if (ISSUE) wait_vmcnt<(STAGES - 2) * LPW>();
+        else wait_vmcnt<0>();
+        __syncthreads();
+        read_scales(nst);
+      }
+      if (j + RB - 1 < FN) read_b(st, j + RB - 1);
+      else if (NEXT) read_b(nst, j + RB - 1 - FN);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        mfma_one(j, i);
+        if (j == FN - 1 && NEXT) read_a(nst, i);
+        if (j >= JB && ISSUE)
+#pragma unroll
+          for (int u = 0; u < PER; ++u) {
+            const int q = ((j - JB) * FM + i) * PER + u;
+            if (q < LPW) issue_one(st, kt + STAGES, q);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (NEXT) take_scales();
+  };
+
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < KT) issue(s, s);
+  if (K % 128 != 0 && (!SPLIT || blockIdx.y + 1 == gridDim.y)) {
+    // the last K % 128 columns first, zeros behind them, through the last stage
+    typedef u64x2_t __attribute__((aligned(1))) u64x2_u;
+    const int kt0 = K / 128;
+    char* t = smem + (STAGES - 1) * STAGE;
+#pragma unroll
+    for (int q = 0; q < NQA + NQB; ++q) {
+      const int c = q < NQA ? wave * NQA + q : wave * NQB + q - NQA, r = c * 8 + lane / 8;
+      const int chunk = dl_swz(r, lane % 8), k = kt0 * 128 + 16 * chunk;
+      const uint8_t* base = q < NQA ? A + ao[q] : (b_up(c * 8) ? B[1] : B[0]) + bo[q - NQA];
+      base -= 16 * chunk;  // the row's start
+      u64x2_t v;
+      if (K >= 16) {
+        v = shift_down(*(const u64x2_u*)(base + min(k, K - 16)), max(0, k - (K - 16)));
+      } else {
+        v = u64x2_t{};
+        for (int e = 0; e < 16; ++e)
+          if (k + e < K) v[e >> 3] |= (uint64_t)base[k + e] << (8 * (e & 7));
+      }
+      *(u64x2_t*)(t + (q < NQA ? 0 : TA) + c * 1024 + lane * 16) = v;
+    }
+#pragma unroll
+    for (int q = 0; q < NQS; ++q)
+      ((int*)(t + TA + TB))[(wave * NQS + q) % C::NSB * 64 + lane] = so[q][kt0];
+    __syncthreads();
+    read_scales(STAGES - 1);
+    take_scales();
+#pragma unroll
+    for (int i = 0; i < FM; ++i) read_a(STAGES - 1, i);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      read_b(STAGES - 1, j);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) mfma_one(j, i);
+    }
+    __syncthreads();
+  }
+  if (STAGES - 1 < KT) issue(STAGES - 1, STAGES - 1);
+  if (KT > 0) {
+    if (STAGES <= KT) wait_vmcnt<(STAGES - 1) * LPW>();
+    else wait_vmcnt<0>();
+    __syncthreads();
+    first_reads(0);
+    int st = 0, kt = 0;
+    const std::true_type yes;
+    const std::false_type no;
+    for (; kt < KT - STAGES; ++kt) {
+      step(st, kt, yes, yes);
+      st = st + 1 == STAGES ? 0 : st + 1;
+    }
+    for (; kt < KT - 1; ++kt) {
+      step(st, kt, no, yes);
+      st = st + 1 == STAGES ? 0 : st + 1;
+    }
+    step(st, kt, no, no);
+  }
+
+  const int mw = m0 + wm * TM;
+  if constexpr (SPLIT) {
+    // (ldp is a multiple of 4, so a run that starts inside the row fits)
+    const int64_t set = (int64_t)gridDim.y * M * p.ldp;
+    float* part = p.part + (int64_t)blockIdx.y * M * p.ldp;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = wn * TN + 16 * j, n = b_row(r) + 4 * (lane >> 4), m = mw + 16 * i + row;
+        if (m < M && n < N) *(f32x4_t*)(part + (b_up(r) ? set : 0) + (int64_t)m * p.ldp + n) = acc[j][i];
+      }
+    return;
+  }
+  __syncthreads();  // every wave is done with the stages
+  if constexpr (EPI == F8_GATE) {
+    uint32_t* most = (uint32_t*)(smem + BM * C::CP);  // [WN][BM]
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      uint32_t mx = 0;
+#pragma unroll
+      for (int j = 0; j < FN / 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int n = n0 + wn * (TN / 2) + 16 * j + 4 * (lane >> 4) + e;
+          const float g = acc[j][i][e], u = n < N ? acc[j + FN / 2][i][e] : 0.f;
+          acc[j][i][e] = gate_of(n < N ? g : 0.f, u, &mx);
+        }
+      mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, 64));
+      mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, 64));
+      if (lane < 16) most[wn * BM + wm * TM + 16 * i + row] = mx;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int r = wm * TM + 16 * i + row;
+      uint32_t mx = most[r];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) mx = max(mx, most[w * BM + r]);
+      const uint32_t byte = fp8_scale_byte(mx);
+      const float inv = fp8_inverse(byte);
+#pragma unroll
+      for (int j = 0; j < FN / 2; ++j)
+        *(uint32_t*)(smem + r * C::CP + wn * (TN / 2) + 16 * j + 4 * (lane >> 4)) =
+            fp8_codes4(acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3], inv);
+      if (wn == 0 && lane < 16 && m0 + r < M)
+        p.codes.scales[(int64_t)(m0 + r) * p.codes.sld + tn] = (uint8_t)byte;
+    }
+    __syncthreads();
+    const bool vec = p.codes.ld % 16 == 0 && (uintptr_t)p.codes.codes % 16 == 0;
+    for (int id = threadIdx.x; id < BM * 8; id += C::NT) {
+      const int r = id >> 3, c = (id & 7) * 16, n = n0 + c;
+      if (m0 + r >= M || n >= N) continue;
+      const u32x4_t v = *(const u32x4_t*)(smem + r * C::CP + c);
+      uint8_t* dst = p.codes.codes + (int64_t)(m0 + r) * p.codes.ld + n;
+      if (vec && n + 15 < N) {
+        *(u32x4_t*)dst = v;
+      } else {
+        for (int e = 0; e < 16 && n + e < N; ++e) dst[e] = (uint8_t)(v[e >> 2] >> (8 * (e & 3)));
+      }
+    }
+    return;
+  }
+  // out = acc (+ bias) (+ residual), rounded once: HC columns of the wave's tile at a
+  // time through LDS, for whole row segments
+  constexpr int HC = C::HC, EP = C::EP, LPR = HC / 8, RPI = 64 / LPR;
+  float* es = (float*)smem + wave * TM * EP;
+  typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
+  uint16_t* out = (uint16_t*)p.out;
+  const bool vec_out = p.ldc % 8 == 0 && (uintptr_t)out % 16 == 0;
+  const bool vec_res = p.ldr % 8 == 0 && (uintptr_t)p.res % 16 == 0;
+  auto wide = [&](uint16_t v) __attribute__((always_inline)) { return p.f16 ? f16_to_f32(v) : bf16_to_f32(v); };
+#pragma unroll
+  for (int h = 0; h < TN / HC; ++h) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < HC / 16; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        *(f32x4_t*)(es + (16 * i + row) * EP + 16 * j + 4 * (lane >> 4)) = acc[h * (HC / 16) + j][i];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int c = (lane % LPR) * 8, n = n0 + wn * TN + h * HC + c;
+    float bias[8] = {};
+    if (p.bias != nullptr)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int at = min(n + e, N - 1);
+        bias[e] = p.bias_dtype == MI_F32 ? ((const float*)p.bias)[at] : wide(((const uint16_t*)p.bias)[at]);
+      }
+#pragma unroll 4
+    for (int it = 0; it < TM / RPI; ++it) {
+      const int r = it * RPI + lane / LPR, m = mw + r;
+      if (m >= M || n >= N) continue;
+      const f32x4_t lo = *(const f32x4_t*)(es + r * EP + c), hi = *(const f32x4_t*)(es + r * EP + c + 4);
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) + bias[e];
+      if (p.res != nullptr) {
+        const uint16_t* src = p.res + (int64_t)m * p.ldr + n;
+        if (vec_res && n + 7 < N) {
+          const u16x8_t v = *(const u16x8_t*)src;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] += wide(v[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < N) y[e] += wide(src[e]);
+        }
+      }
+      u16x8_t v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p.f16 ? f32_to_f16(y[e]) : f32_to_bf16(y[e]);
+      uint16_t* dst = out + (int64_t)m * p.ldc + n;
+      if (vec_out && n + 7 < N) {
+        *(u16x8_t*)dst = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < N) dst[e] = v[e];
+      }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace mi

@@ -1,0 +1,418 @@
+// Activations and weights to e4m3 codes with a power-of-two scale for each 128
+// columns of a row, or each 128 x 128 block; and the root-mean-square norm, with the
+// residual's addition before it, whose output goes straight to such codes.
+//
+// A scale is the smallest power of two s >= 2^-110 with amax <= 448 s: e4m3 is a
+// floating type, so a power of two costs none of its precision, division by it is
+// exact, and the matrix instructions multiply by it for free.
+//
+// What bounds them: HBM, each element read once and its code written.  A lane holds
+// 8 neighbouring elements, so 16 lanes are a group and its maximum four DPP steps; a
+// row stays in registers between the sum of squares, the maxima and the codes.
+#include "fp8_common.h"
+
+namespace mi {
+namespace {
+
+constexpr int QUANT = 0, NORM = 1, NORM_RES = 2;
+
+struct RowsArgs {
+  const void* x;
+  const void* res;
+  const void* weight;
+  void* total;
+  int64_t x_ld, res_ld, total_ld;  // row strides, in elements
+  Fp8Mat out;
+  int64_t rows;
+  int cols;
+  float eps;
+};
+
+// Eight neighbouring elements as they lie in memory.
+template <typename T>
+struct Eight {
+  typedef typename Num<T>::storage St;
+  static constexpr int W = sizeof(St) * 2;  // 32-bit words
+  union {
+    uint32_t w[W];
+    St e[8];
+  };
+  __device__ __forceinline__ float get(int i) const { return Num<T>::load(e[i]); }
+  // VEC: the row is 16-byte aligned and its length a multiple of 8
+  template <bool VEC>
+  static __device__ __forceinline__ Eight load(const void* row, int col, int cols) {
+    Eight r;
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < W / 4; ++i) {
+        const u32x4_t v = *((const u32x4_t*)((const St*)row + min(col, cols - 8)) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r.w[4 * i + j] = col < cols ? v[j] : 0u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const St v = ((const St*)row)[min(col + i, cols - 1)];
+        r.e[i] = col + i < cols ? v : (St)0;
+      }
+    }
+    return r;
+  }
+  template <bool VEC>
+  __device__ __forceinline__ void store(void* row, int col, int cols) const {
+    if constexpr (VEC) {
+      if (col < cols)
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i)
+          *((u32x4_t*)((St*)row + col) + i) = u32x4_t{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < cols) ((St*)row)[col + i] = e[i];
+    }
+  }
+};
+
+// The scale byte of a group that `lanes` lanes hold 8 elements of each (most: the
+// largest |bits| over the group, whatever it holds), and the codes of this lane's.
+// Groups that hold an infinity or a NaN look at their finite elements again.
+template <typename Max>
+__device__ __forceinline__ f8_u32x2 codes_of(const float* y, uint32_t most, Max group_max,
+                                             uint32_t* byte) {
+  if (most >= kFp8Inf) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, fp8_finite_bits(y[i]));
+    *byte = fp8_scale_byte(group_max(m));
+    const float inv = fp8_inverse(*byte);
+    return f8_u32x2{fp8_codes4(y[0], y[1], y[2], y[3], inv), fp8_codes4(y[4], y[5], y[6], y[7], inv)};
+  }
+  *byte = fp8_scale_byte(most);
+  const float inv = fp8_inverse(*byte);
+  f8_u32x2 r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h] * inv, y[4 * h + 1] * inv, 0, false);
+    r[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2] * inv, y[4 * h + 3] * inv, c, true);
+  }
+  return r;
+}
+
+__device__ __forceinline__ uint32_t largest_bits(const float* y) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(y[i]) & kFp8AbsMask);
+  return m;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, f8_u32x2 c) {
+  if constexpr (VEC) {
+    if (col < cols) *(f8_u32x2*)(row + col) = c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < cols) row[col + i] = (uint8_t)(c[i >> 2] >> (8 * (i & 3)));
+  }
+}
+
+// TPR threads a row, VPL x 8 elements a thread in registers; VPL 0: rows of any
+// length, read again for the codes (the total from where it was written).
+template <typename T, int KIND, int TPR, int VPL, bool VEC>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
+  typedef Eight<T> E;
+  typedef typename E::St St;
+  constexpr int STEP = TPR * 8, N = VPL > 0 ? VPL : 1;
+  __shared__ float red[4];
+  const int t = threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (TPR < 256 && row >= a.rows) return;
+  const int cols = a.cols;
+  const St* x = (const St*)a.x + row * a.x_ld;
+  const St* res = KIND == NORM_RES ? (const St*)a.res + row * a.res_ld : nullptr;
+  St* total = KIND == NORM_RES ? (St*)a.total + row * a.total_ld : nullptr;
+  uint8_t* codes = a.out.codes + row * a.out.ld;
+  uint8_t* scales = a.out.scales + row * a.out.sld;
+  E v[N], r[N];
+  auto load = [&](int i, int col) __attribute__((always_inline)) {
+    v[i] = E::template load<VEC>(x, col, cols);
+    if constexpr (KIND == NORM_RES) r[i] = E::template load<VEC>(res, col, cols);
+  };
+  float ss = 0.f;
+  auto add_up = [&](int i, int col) __attribute__((always_inline)) {
+    if constexpr (KIND == NORM_RES) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i].e[j] = Num<T>::store(v[i].get(j) + r[i].get(j));
+      v[i].template store<VEC>(total, col, cols);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(v[i].get(j), v[i].get(j), ss);
+  };
+  if constexpr (VPL > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) load(i, t * 8 + i * STEP);
+    if constexpr (KIND != QUANT)
+#pragma unroll
+      for (int i = 0; i < N; ++i) add_up(i, t * 8 + i * STEP);
+  } else if constexpr (KIND != QUANT) {
+    for (int c = t * 8; c < cols; c += STEP) {
+      load(0, c);
+      add_up(0, c);
+    }
+  }
+  float norm = 1.f;
+  if constexpr (KIND != QUANT) {
+    ss = wave_sum(ss);
+    if constexpr (TPR == 256) {
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
+      __syncthreads();
+      ss = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    norm = 1.0f / __builtin_sqrtf(ss / (float)cols + a.eps);
+  }
+  auto finish = [&](const E& s, int col) __attribute__((always_inline)) {
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = KIND == QUANT ? s.get(j) : s.get(j) * norm;
+    if (KIND != QUANT && a.weight != nullptr) {
+      const E w = E::template load<VEC>(a.weight, col, cols);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] *= w.get(j);
+    }
+    // (0 x an infinite norm is NaN: what lies behind the row's end stays 0)
+    if (col >= cols) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = 0.f;
+    } else if (!VEC) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = col + j < cols ? y[j] : 0.f;
+    }
+    uint32_t byte;
+    const f8_u32x2 c = codes_of(y, row16_max(largest_bits(y)), row16_max, &byte);
+    store_codes<VEC>(codes, col, cols, c);
+    if ((t & 15) == 0 && col < cols) scales[col / kFp8Group] = (uint8_t)byte;
+  };
+  if constexpr (VPL > 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) finish(v[i], t * 8 + i * STEP);
+  } else {
+    // whole rows of 16 lanes take part in a group's maximum
+    for (int c = t * 8; c / kFp8Group * kFp8Group < cols; c += STEP)
+      finish(E::template load<VEC>(KIND == NORM_RES ? total : x, c, cols), c);
+  }
+}
+
+// A block of 256 threads to a 128 x 128 block of the weight, 8 rows a thread.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void fp8_weight_kernel(const void* w, int64_t ld, int64_t rows, int cols,
+                                                         Fp8Mat out) {
+  typedef Eight<T> E;
+  typedef typename E::St St;
+  __shared__ uint32_t red[4];
+  const int col = blockIdx.x * kFp8Group + (threadIdx.x & 15) * 8;
+  const int64_t row0 = (int64_t)blockIdx.y * kFp8Group + (threadIdx.x >> 4);
+  E v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = E::template load<VEC>((const St*)w + min(row0 + 16 * i, rows - 1) * ld, col, cols);
+  auto block_max = [&](uint32_t m) __attribute__((always_inline)) {
+    m = row16_max(m);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    return max(max(red[0], red[1]), max(red[2], red[3]));
+  };
+  // (rows past the end read the last one again, which is in the block)
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i].get(j)) & kFp8AbsMask);
+  most = block_max(most);
+  if (most >= kFp8Inf) {  // the same for the whole block
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, fp8_finite_bits(v[i].get(j)));
+    most = block_max(most);
+  }
+  const uint32_t byte = fp8_scale_byte(most);
+  const float inv = fp8_inverse(byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = row0 + 16 * i;
+    if (row >= rows) break;
+    const f8_u32x2 c = {fp8_codes4(v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3), inv),
+                        fp8_codes4(v[i].get(4), v[i].get(5), v[i].get(6), v[i].get(7), inv)};
+    store_codes<VEC>(out.codes + row * out.ld, col, cols, c);
+  }
+  if (threadIdx.x == 0) out.scales[blockIdx.y * out.sld + blockIdx.x] = (uint8_t)byte;
+}
+
+// 16-byte accesses to the rows of a wide tensor, 8-byte ones to the codes
+bool aligned(const void* p, int64_t ld, int size) {
+  return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0;
+}
+bool aligned_codes(const Fp8Mat& m) { return (uintptr_t)m.codes % 8 == 0 && m.ld % 8 == 0; }
+
+template <typename T, int KIND>
+mi_status_t launch_rows(const RowsArgs& a, bool vec, hipStream_t s, const char* op) {
+  auto go = [&](auto tpr, auto vpl, auto v) {
+    constexpr int TPR = decltype(tpr)::value;
+    hipLaunchKernelGGL((fp8_rows_kernel<T, KIND, TPR, decltype(vpl)::value, decltype(v)::value>),
+                       dim3(ceil_div_u(a.rows, 256 / TPR)), dim3(256), 0, s, a);
+    return check_launch(op);
+  };
+  const std::integral_constant<int, 64> wave;
+  const std::integral_constant<int, 256> block;
+  const std::true_type yes;
+  const std::integral_constant<int, 0> any;
+  const std::integral_constant<int, 1> one;
+  const std::integral_constant<int, 2> two;
+  const std::integral_constant<int, 4> four;
+  const std::integral_constant<int, 8> eight;
+  if (!vec) return go(block, any, std::false_type());
+  if (a.cols <= 512) return go(wave, one, yes);
+  if (a.cols <= 1024) return go(wave, two, yes);
+  if (a.cols <= 2048) return go(block, one, yes);
+  if (a.cols <= 4096) return go(block, two, yes);
+  if (a.cols <= 8192) return go(block, four, yes);
+  if (a.cols <= 16384) return go(block, eight, yes);
+  return go(block, any, yes);
+}
+
+template <int KIND>
+mi_status_t run_rows(const RowsArgs& a, int dtype, bool vec, hipStream_t s, const char* op) {
+  if (dtype == MI_BF16) return launch_rows<BF16, KIND>(a, vec, s, op);
+  if (dtype == MI_F16) return launch_rows<F16, KIND>(a, vec, s, op);
+  return launch_rows<float, KIND>(a, vec, s, op);
+}
+
+mi_status_t check_shape(const char* op, const mi_fp8_t* out, const mi_tensor_t* x, const char* name) {
+  MI_CHECK_ARG(out->codes.sizes[0] == x->sizes[0] && out->codes.sizes[1] == x->sizes[1],
+               "%s: codes are [%lld, %lld], %s [%lld, %lld]", op, (long long)out->codes.sizes[0],
+               (long long)out->codes.sizes[1], name, (long long)x->sizes[0], (long long)x->sizes[1]);
+  return MI_OK;
+}
+
+mi_status_t check_outputs_apart(const char* op, const mi_fp8_t* out, const char* name,
+                                const mi_tensor_t* t) {
+  MI_RETURN_IF(fp8_check_apart(op, "codes", &out->codes, name, t));
+  return fp8_check_apart(op, "scales", &out->scales, name, t);
+}
+
+}  // namespace
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" {
+
+mi_status_t mi_fp8_quantize(const mi_fp8_t* out, const mi_tensor_t* x, mi_stream_t stream) {
+  clear_error();
+  const char* op = "fp8_quantize";
+  RowsArgs a{};
+  MI_RETURN_IF(fp8_check(op, "out", out, false, true, &a.out));
+  MI_RETURN_IF(fp8_check_wide(op, "x", x, true));
+  MI_RETURN_IF(check_shape(op, out, x, "x"));
+  MI_RETURN_IF(check_outputs_apart(op, out, "x", x));
+  if (numel(*x) == 0) return MI_OK;
+  a.x = x->data;
+  a.x_ld = x->strides[0];
+  a.rows = x->sizes[0];
+  a.cols = (int)x->sizes[1];
+  const bool vec = a.cols % 8 == 0 && aligned(x->data, x->strides[0], dtype_size(x->dtype)) &&
+                   aligned_codes(a.out);
+  return run_rows<QUANT>(a, x->dtype, vec, (hipStream_t)stream, op);
+}
+
+mi_status_t mi_fp8_quantize_weight(const mi_fp8_t* out, const mi_tensor_t* weight, mi_stream_t stream) {
+  clear_error();
+  const char* op = "fp8_quantize_weight";
+  Fp8Mat m;
+  MI_RETURN_IF(fp8_check(op, "out", out, true, true, &m));
+  MI_RETURN_IF(fp8_check_wide(op, "weight", weight, true));
+  MI_RETURN_IF(check_shape(op, out, weight, "weight"));
+  MI_RETURN_IF(check_outputs_apart(op, out, "weight", weight));
+  if (numel(*weight) == 0) return MI_OK;
+  const int64_t rows = weight->sizes[0], cols = weight->sizes[1], ld = weight->strides[0];
+  if (fp8_groups(rows) > 65535) MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 65535 x 128 rows", op);
+  const dim3 grid((unsigned)fp8_groups(cols), (unsigned)fp8_groups(rows));
+  const bool vec = cols % 8 == 0 && aligned(weight->data, ld, dtype_size(weight->dtype)) && aligned_codes(m);
+  auto go = [&](auto type, auto v) {
+    hipLaunchKernelGGL((fp8_weight_kernel<decltype(type), decltype(v)::value>), grid, dim3(256), 0,
+                       (hipStream_t)stream, weight->data, ld, rows, (int)cols, m);
+    return check_launch(op);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  if (weight->dtype == MI_BF16) return vec ? go(BF16{}, yes) : go(BF16{}, no);
+  if (weight->dtype == MI_F16) return vec ? go(F16{}, yes) : go(F16{}, no);
+  return vec ? go(0.f, yes) : go(0.f, no);
+}
+
+mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const mi_tensor_t* x,
+                            const mi_tensor_t* residual, const mi_tensor_t* weight, double eps,
+                            mi_stream_t stream) {
+  clear_error();
+  const char* op = "rms_norm_fp8";
+  RowsArgs a{};
+  MI_RETURN_IF(fp8_check(op, "out", out, false, true, &a.out));
+  MI_RETURN_IF(fp8_check_wide(op, "x", x, true));
+  MI_RETURN_IF(check_shape(op, out, x, "x"));
+  MI_RETURN_IF(check_outputs_apart(op, out, "x", x));
+  const int size = dtype_size(x->dtype);
+  bool vec = x->sizes[1] % 8 == 0 && aligned(x->data, x->strides[0], size) && aligned_codes(a.out);
+  const bool has_res = residual != nullptr && residual->data != nullptr;
+  const bool has_w = weight != nullptr && weight->data != nullptr;
+  if (has_res) {
+    MI_CHECK_ARG(total != nullptr, "%s: total is NULL", op);
+    const mi_tensor_t* ts[2] = {residual, total};
+    const char* names[2] = {"residual", "total"};
+    for (int i = 0; i < 2; ++i) {
+      MI_RETURN_IF(fp8_check_wide(op, names[i], ts[i], true));
+      MI_CHECK_ARG(ts[i]->dtype == x->dtype && ts[i]->sizes[0] == x->sizes[0] &&
+                       ts[i]->sizes[1] == x->sizes[1],
+                   "%s: %s must have x's shape and type", op, names[i]);
+      MI_RETURN_IF(check_outputs_apart(op, out, names[i], ts[i]));
+      // total may be the same tensor as an input: a thread reads what it writes
+      const mi_tensor_t* in = i == 0 ? x : residual;
+      if (!(in->data == total->data && (in->sizes[0] <= 1 || in->strides[0] == total->strides[0])))
+        MI_RETURN_IF(fp8_check_apart(op, "total", total, i == 0 ? "x" : "residual", in));
+      vec = vec && aligned(ts[i]->data, ts[i]->strides[0], size);
+    }
+    MI_CHECK_ARG(total->sizes[0] <= 1 || total->strides[0] >= total->sizes[1], "%s: rows of total overlap",
+                 op);
+    a.res = residual->data;
+    a.res_ld = residual->strides[0];
+    a.total = total->data;
+    a.total_ld = total->strides[0];
+  }
+  if (has_w) {
+    MI_RETURN_IF(validate(weight, "weight"));
+    MI_CHECK_ARG(weight->ndim == 1 && weight->sizes[0] == x->sizes[1] && weight->dtype == x->dtype &&
+                     (weight->sizes[0] <= 1 || weight->strides[0] == 1),
+                 "%s: weight must be a dense vector of x's type and columns", op);
+    MI_RETURN_IF(check_outputs_apart(op, out, "weight", weight));
+    if (has_res) MI_RETURN_IF(fp8_check_apart(op, "total", total, "weight", weight));
+    vec = vec && (uintptr_t)weight->data % 16 == 0;
+    a.weight = weight->data;
+  }
+  if (has_res) {
+    MI_RETURN_IF(fp8_check_apart(op, "total", total, "codes", &out->codes));
+    MI_RETURN_IF(fp8_check_apart(op, "total", total, "scales", &out->scales));
+  }
+  if (numel(*x) == 0) return MI_OK;
+  a.x = x->data;
+  a.x_ld = x->strides[0];
+  a.rows = x->sizes[0];
+  a.cols = (int)x->sizes[1];
+  a.eps = (float)eps;
+  return has_res ? run_rows<NORM_RES>(a, x->dtype, vec, (hipStream_t)stream, op)
+                 : run_rows<NORM>(a, x->dtype, vec, (hipStream_t)stream, op);
+}
+
+}  // extern "C"

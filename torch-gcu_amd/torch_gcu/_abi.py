@@ -56,6 +56,10 @@ class MiKv8Cache(ctypes.Structure):
     _fields_ = [("k", MiTensor), ("v", MiTensor), ("k_scale", MiTensor), ("v_scale", MiTensor)]
 
 
+class MiFp8(ctypes.Structure):
+    _fields_ = [("codes", MiTensor), ("scales", MiTensor)]
+
+
 class MiError(RuntimeError):
     """A kernel-library call returned a status other than MI_OK."""
 
@@ -68,6 +72,7 @@ _ALLOC_FN = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, 
 _FREE_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)
 
 _T = ctypes.POINTER(MiTensor)
+_F8 = ctypes.POINTER(MiFp8)
 _S = ctypes.c_void_p
 _SIGNATURES = {
     "mi_abi_version": ([], ctypes.c_int32),
@@ -132,6 +137,11 @@ _SIGNATURES = {
                      ctypes.c_int),
     "mi_kv8_evict": ([ctypes.POINTER(MiKv8Cache)] + [_T] * 4 + [ctypes.c_int64] * 3 + [_T] * 3
                      + [_S], ctypes.c_int),
+    "mi_fp8_quantize": ([_F8, _T, _S], ctypes.c_int),
+    "mi_fp8_quantize_weight": ([_F8, _T, _S], ctypes.c_int),
+    "mi_rms_norm_fp8": ([_F8, _T, _T, _T, _T, ctypes.c_double, _S], ctypes.c_int),
+    "mi_fp8_linear": ([_T, _F8, _F8, _T, _T, _S], ctypes.c_int),
+    "mi_fp8_linear_silu_mul": ([_F8] * 4 + [_S], ctypes.c_int),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -572,3 +582,40 @@ def kv8_evict(cache, weights, block_table, new_table, lengths, keep, recent, sin
                              desc(lengths), keep, recent, sink, desc(kept), desc(new_lengths),
                              desc(new_weights), stream_of(weights)))
     return kept, new_lengths, new_weights
+
+
+def _fp8(t):
+    return MiFp8(*(desc(x) for x in t))
+
+
+def fp8_quantize(out, x):
+    """out: (codes, scales), as for the other fp8 calls; all matrices 2-D."""
+    check("mi_fp8_quantize", lib().mi_fp8_quantize(_fp8(out), desc(x), stream_of(x)))
+    return out
+
+
+def fp8_quantize_weight(out, weight):
+    check("mi_fp8_quantize_weight",
+          lib().mi_fp8_quantize_weight(_fp8(out), desc(weight), stream_of(weight)))
+    return out
+
+
+def rms_norm_fp8(out, total, x, residual, weight, eps):
+    check("mi_rms_norm_fp8",
+          lib().mi_rms_norm_fp8(_fp8(out), desc(total), desc(x), desc(residual), desc(weight),
+                                float(eps), stream_of(x)))
+    return out, total
+
+
+def fp8_linear(out, x, weight, bias=None, residual=None):
+    check("mi_fp8_linear",
+          lib().mi_fp8_linear(desc(out), _fp8(x), _fp8(weight), desc(bias), desc(residual),
+                              stream_of(out)))
+    return out
+
+
+def fp8_linear_silu_mul(out, x, w_gate, w_up):
+    check("mi_fp8_linear_silu_mul",
+          lib().mi_fp8_linear_silu_mul(_fp8(out), _fp8(x), _fp8(w_gate), _fp8(w_up),
+                                       stream_of(x[0])))
+    return out

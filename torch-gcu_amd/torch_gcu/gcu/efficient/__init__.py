@@ -5,7 +5,8 @@
 ``rms_norm``, ``rope``, ``rope_`` and ``silu_mul`` are new fused kernels, and
 ``linear_residual`` / ``linear_silu_mul`` are matmuls with the residual add or
 the SwiGLU product fused into their epilogue.  The ``kv8_*`` ops serve from a
-key/value cache held in 8 bits.
+key/value cache held in 8 bits, the ``fp8_*`` ops and ``rms_norm_fp8`` are linear
+layers in 8-bit floating point.
 All are dispatcher ops (``torch.ops.torch_gcu.*``) with gcu kernels only.
 """
 from __future__ import annotations
@@ -130,3 +131,52 @@ def kv8_evict(cache: KV8Cache, weights: torch.Tensor, block_table: torch.Tensor,
     caller's again; queries keep using their true positions for RoPE."""
     return torch.ops.torch_gcu.kv8_evict(*cache, weights, block_table, new_table, lengths, keep,
                                          recent, sink)
+
+
+class FP8Rows(NamedTuple):
+    """Activations in 8 bits: codes uint8 [..., columns] and scales uint8 [...,
+    ceil(columns / 128)], one for each 128 columns of a row.  An element is
+    ``codes.view(torch.float8_e4m3fn) * 2.0 ** (scale - 127)`` (on another device)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+class FP8Weight(NamedTuple):
+    """A weight [N, K] in 8 bits: codes uint8 [N, K] and scales uint8 [ceil(N / 128),
+    ceil(K / 128)], one for each block of 128 x 128, read as FP8Rows' are."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def fp8_quantize(x: torch.Tensor) -> FP8Rows:
+    """x [..., columns] (bf16, f16 or f32) as codes and scales: the smallest power of
+    two s >= 2^-110 with amax <= 448 s for each 128 columns, codes to nearest.  What is
+    infinite or NaN becomes NaN.  No gradients, here and in the ops below."""
+    return FP8Rows(*torch.ops.torch_gcu.fp8_quantize(x))
+
+
+def fp8_quantize_weight(weight: torch.Tensor) -> FP8Weight:
+    """weight [N, K] (bf16, f16 or f32) likewise, a scale for each 128 x 128 block."""
+    return FP8Weight(*torch.ops.torch_gcu.fp8_quantize_weight(weight))
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
+                 residual: Optional[torch.Tensor] = None) -> tuple[FP8Rows, torch.Tensor]:
+    """(rms_norm of total as FP8Rows, total), where total is x + residual in their type,
+    or x itself without a residual.  The norm is not rounded before it becomes codes."""
+    codes, scales, total = torch.ops.torch_gcu.rms_norm_fp8(x, weight, eps, residual)
+    return FP8Rows(codes, scales), x if residual is None else total
+
+
+def fp8_linear(x: FP8Rows, weight: FP8Weight, bias: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x @ weight^T (+ bias) (+ residual), summed in fp32 and rounded once, to dtype:
+    bf16 or f16, by default the residual's type, else bf16.  bias is a vector of that
+    type or float32."""
+    return torch.ops.torch_gcu.fp8_linear(*x, *weight, bias, residual, dtype)
+
+
+def fp8_linear_silu_mul(x: FP8Rows, w_gate: FP8Weight, w_up: FP8Weight) -> FP8Rows:
+    """silu(x @ w_gate^T) * (x @ w_up^T) as FP8Rows, rounded once, to the codes."""
+    return FP8Rows(*torch.ops.torch_gcu.fp8_linear_silu_mul(*x, *w_gate, *w_up))

@@ -32,6 +32,9 @@ class LayerConfig:
     eps: float = 1e-6
 
 
+PROJECTIONS = ("wq", "wk", "wv", "wo", "w_gate", "w_up", "w_down")
+
+
 def init_weights(cfg: LayerConfig, seed: int = 20261205, dtype=torch.bfloat16) -> dict:
     """Random-init weights, normal(0, 0.02); norm weights are ones."""
     g = torch.Generator().manual_seed(seed)
@@ -143,8 +146,11 @@ def forward_cached(weights: dict, ids: torch.Tensor, cfg: LayerConfig, cache,
     ``torch.gcu.efficient.kv8_append``.  Nothing is created on the host, so a
     captured call can be replayed after the index tensors have been updated.
     Returns the hidden states [tokens, hidden], and the queries and logsumexp
-    that ``kv8_weigh_`` takes."""
+    that ``kv8_weigh_`` takes.  With weights from ``quantize_weights`` the
+    projections run in 8-bit floating point."""
     eff = torch.gcu.efficient
+    if isinstance(weights["wq"], eff.FP8Weight):
+        return _forward_cached_fp8(weights, ids, cfg, cache, block_table, lengths, starts, pos)
     T, H, D = ids.shape[0], cfg.heads, cfg.head_dim
     x = F.embedding(ids, weights["embed"])
     h = _rms_norm(x, weights["attn_norm"], cfg.eps)
@@ -158,6 +164,31 @@ def forward_cached(weights: dict, ids: torch.Tensor, cfg: LayerConfig, cache,
     h = _rms_norm(x, weights["ffn_norm"], cfg.eps)
     m = _linear_silu_mul(h, weights["w_gate"], weights["w_up"])
     return _linear_residual(m, weights["w_down"], x), q, lse
+
+
+def quantize_weights(weights: dict) -> dict:
+    """The layer's weights with its projections in 8-bit floating point, for
+    ``forward_cached`` (gcu only)."""
+    quantize = torch.gcu.efficient.fp8_quantize_weight
+    return {n: quantize(w) if n in PROJECTIONS else w for n, w in weights.items()}
+
+
+def _forward_cached_fp8(weights, ids, cfg, cache, block_table, lengths, starts, pos):
+    """forward_cached with quantised projections: each norm gives the codes that the
+    projections behind it read, the first residual add is the second norm's, the gate
+    and up products give the codes for the down projection."""
+    eff = torch.gcu.efficient
+    T, H, D = ids.shape[0], cfg.heads, cfg.head_dim
+    x = F.embedding(ids, weights["embed"])
+    h, _ = eff.rms_norm_fp8(x, weights["attn_norm"], cfg.eps)
+    q, k, v = (eff.fp8_linear(h, weights[n], dtype=x.dtype).view(T, -1, D) for n in ("wq", "wk", "wv"))
+    _rope_(q, k, pos, cfg.theta)
+    eff.kv8_append(k, v, cache, block_table, lengths, starts)
+    a, lse = eff.kv8_attention(q, cache, block_table, lengths, starts)
+    o = eff.fp8_linear(eff.fp8_quantize(a.view(T, H * D)), weights["wo"], dtype=x.dtype)
+    h, x = eff.rms_norm_fp8(o, weights["ffn_norm"], cfg.eps, residual=x)
+    m = eff.fp8_linear_silu_mul(h, weights["w_gate"], weights["w_up"])
+    return eff.fp8_linear(m, weights["w_down"], residual=x), q, lse
 
 
 def flops(cfg: LayerConfig, batch: int, seq: int) -> int:
