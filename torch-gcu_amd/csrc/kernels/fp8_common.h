@@ -34,6 +34,10 @@ mi_status_t fp8_check_wide(const char* op, const char* name, const mi_tensor_t* 
 mi_status_t fp8_check_apart(const char* op, const char* name, const mi_tensor_t* out,
                             const char* other_name, const mi_tensor_t* other);
 
+// y float32 [rows][ld], with 16-byte aligned rows, to codes and scales (fp8_quantize.hip)
+mi_status_t fp8_quantize_f32(const float* y, int64_t ld, int64_t rows, int cols, const Fp8Mat& out,
+                             hipStream_t s, const char* op);
+
 namespace {
 
 typedef uint32_t f8_u32x2 __attribute__((ext_vector_type(2)));

@@ -35,12 +35,16 @@ __device__ __forceinline__ f32x4_t mma_fp8(i32x8_t a, i32x8_t b, f32x4_t c, int 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
-// A byte a lane, from an address of its own, to a 32-bit word a lane at lds on (the
-// counterpart of lds_copy16).
-__device__ __forceinline__ void lds_copy_byte(const uint8_t* p, void* lds) {
+// A byte a lane, from a wave-uniform base and a 32-bit offset of its own, to a 32-bit
+// word a lane at lds on (the counterpart of lds_copy16).
+__device__ __forceinline__ void lds_copy_byte(const uint8_t* base, uint32_t off, void* lds) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
-  asm volatile("s_nop 0\n\tglobal_load_lds_ubyte %0, off" : : "v"(p), "{m0}"(m0) : "memory");
+  const uint64_t b = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+  const uint64_t sb = ((uint64_t)hi << 32) | lo;
+  asm volatile("s_nop 0\n\tglobal_load_lds_ubyte %0, %1" : : "v"(off), "s"(sb), "{m0}"(m0) : "memory");
 }
 
 // silu(g) u and the largest finite magnitude's bits so far
@@ -58,24 +62,31 @@ struct F8Cfg {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, STAGES = STAGES_;
   static constexpr int NW = WM * WN, NT = 64 * NW, BM = WM * TM, BN = WN * TN;
   static constexpr int FM = TM / 16, FN = TN / 16;
-  static constexpr int RB = FN < 4 ? FN : 4;  // weight fragments held
-  static constexpr int NQA = BM / 8 / NW, NQB = BN / 8 / NW;  // 1 KiB wave copies a step
-  static constexpr int NSB = (BM + BN) / 64, NQS = (NSB + NW - 1) / NW;
-  static constexpr int LPW = NQA + NQB + NQS;
-  static constexpr int TA = BM * 128, TB = BN * 128, TS = (BM + BN) * 4, STAGE = TA + TB + TS;
+  static constexpr int RB = FN < 8 ? 2 : 4;  // weight fragments held
+  // 1 KiB wave copies a step: the activations' and of the weight the rows of each wave's
+  // first RB fragments, then the others'
+  static constexpr int NQA = BM / 8 / NW, NQB = BN / 8 / NW, NQL = NQB * RB / FN;
+  static constexpr int LPW = NQA + NQB;
+  static constexpr int TA = BM * 128, TB = BN * 128, STAGE = TA + TB;
+  // scales of KS K steps at a time, a word each, two of such sets in turn: 64 / KS rows a
+  // wave copy, then the weight's blocks (KS 8, or 4 where the LDS has no room for those)
+  static constexpr int KS = STAGES * STAGE + 2 * (BM * 32 + 512) <= 160 * 1024 ? 8 : 4;
+  static constexpr int NQS = (BM * KS / 64 + NW - 1) / NW, SET = BM * KS * 4 + 512, SCALES = STAGES * STAGE;
   static constexpr int HC = TN < 64 ? TN : 64, EP = HC + 4;  // columns of an epilogue pass
   static constexpr int CP = 128 + 16;                         // a gate's staged code rows
   static constexpr size_t cmax(size_t a, size_t b) { return a > b ? a : b; }
   static constexpr size_t LDS_BYTES =
-      cmax((size_t)STAGES * STAGE, cmax((size_t)NW * TM * EP * 4, (size_t)BM * CP + (size_t)WN * BM * 4));
-  static_assert(LDS_BYTES <= 160 * 1024 && NQA >= 1 && NQB >= 1 && FN % RB == 0, "shape");
+      cmax((size_t)SCALES + 2 * SET, cmax((size_t)NW * TM * EP * 4, (size_t)BM * CP + (size_t)WN * BM * 4));
+  static_assert(LDS_BYTES <= 160 * 1024 && NQA >= 1 && NQB >= 1 && FN % RB == 0 && NQL * FN == NQB * RB &&
+                    (STAGES - 1) * LPW < 64, "shape");
 };
 
 template <class C, int EPI>
 __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   constexpr int WN = C::WN, TM = C::TM, TN = C::TN, BM = C::BM, BN = C::BN, FM = C::FM, FN = C::FN;
-  constexpr int RB = C::RB, NQA = C::NQA, NQB = C::NQB, NQS = C::NQS, LPW = C::LPW, STAGES = C::STAGES;
-  constexpr int TA = C::TA, TB = C::TB, STAGE = C::STAGE, GROUP_M = 4;
+  constexpr int RB = C::RB, NQA = C::NQA, NQB = C::NQB, NQL = C::NQL, LPW = C::LPW, STAGES = C::STAGES;
+  constexpr int KS = C::KS, NQS = C::NQS, SET = C::SET, SC = BM * KS / 64;
+  constexpr int TA = C::TA, STAGE = C::STAGE, GROUP_M = 8;
   constexpr bool GATE = EPI == F8_GATE || EPI == F8_GATE_PART;
   constexpr bool SPLIT = EPI == F8_PART || EPI == F8_GATE_PART;
   static_assert(EPI != F8_GATE || BN == 256, "a block holds whole groups of a gate's output");
@@ -84,9 +95,8 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   // GROUP_M row panels, so the tiles an XCD runs together share panels
   int tm, tn;
   {
-    const int total = p.tiles_m * p.tiles_n;
-    int id = blockIdx.x;
-    if (total % 8 == 0) id = (id % 8) * (total / 8) + id / 8;
+    const int total = p.tiles_m * p.tiles_n, xcd = blockIdx.x % 8;
+    const int id = xcd * (total / 8) + min(xcd, total % 8) + blockIdx.x / 8;
     const int group = id / (GROUP_M * p.tiles_n), first = group * GROUP_M;
     const int size = min(p.tiles_m - first, GROUP_M), in_group = id - group * GROUP_M * p.tiles_n;
     tm = first + in_group % size;
@@ -115,6 +125,12 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   // bits; rows past the matrix read its last one and feed outputs that are not stored.
   // LDS chunk c of row r holds the row's chunk dl_swz(r, c).
   uint32_t ao[NQA], bo[NQB];
+  // the 8 rows of the B tile that copy q of the wave takes (q < NQL: of first fragments)
+  auto b_copy = [&](int q) __attribute__((always_inline)) {
+    const bool lo = q < NQL;
+    const int i = lo ? wave * NQL + q : wave * (NQB - NQL) + q - NQL, per = 2 * (lo ? RB : FN - RB);
+    return i / per * (TN / 8) + (lo ? 0 : 2 * RB) + i % per;
+  };
 #pragma unroll
   for (int q = 0; q < NQA; ++q) {
     const int r = (wave * NQA + q) * 8 + lane / 8;
@@ -122,33 +138,48 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   }
 #pragma unroll
   for (int q = 0; q < NQB; ++q) {
-    const int r = (wave * NQB + q) * 8 + lane / 8;
+    const int r = b_copy(q) * 8 + lane / 8;
     bo[q] = (uint32_t)((min(b_row(r), N - 1) - n0) * (b_up(r) ? p.w2.ld : p.w.ld) + 16 * dl_swz(r, lane % 8));
   }
-  // the scale byte of row r of the two tiles (the B tile's behind the A tile's), at K step 0
-  auto scale_at = [&](int r) __attribute__((always_inline)) -> const uint8_t* {
-    if (r < BM) return p.x.scales + (int64_t)min(m0 + r, M - 1) * p.x.sld;
-    const int64_t n = min(b_row(r - BM), N - 1) / kFp8Group;
-    return b_up(r - BM) ? p.w2.scales + n * p.w2.sld : p.w.scales + n * p.w.sld;
-  };
-  const uint8_t* so[NQS];
+  // The scales of set `set` (of the whole K): lane l of a copy takes that of row l / KS (of
+  // the weight's block l / KS) at the set's K step l % KS.  (A copy so takes 8 bytes of 8
+  // rows: a step's bytes of 64 rows, each in a cache line of its own, made M8192 N4096
+  // K11008 10 % slower.)  The offsets are made anew each time: kept, they cost registers
+  // that the main loop has not.
+  const int KB = (K + 127) / 128;
+  const uint8_t* xs = p.x.scales + (int64_t)m0 * p.x.sld;
+  constexpr int NBLK = GATE ? 1 : (BN + 127) / 128;  // blocks of one weight in a tile
+  const uint8_t* ws = p.w.scales + (int64_t)(n0 / kFp8Group) * p.w.sld;
+  auto issue_scales = [&](int set) __attribute__((always_inline)) {
+    char* s = smem + C::SCALES + (set & 1) * SET;
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int k = min(set * KS + l % KS, KB - 1);
 #pragma unroll
-  for (int q = 0; q < NQS; ++q) so[q] = scale_at((wave * NQS + q) % C::NSB * 64 + lane);
+    for (int q = 0; q < NQS; ++q) {
+      const int c = (wave * NQS + q) % SC;
+      lds_copy_byte(xs, (uint32_t)(min(c * (64 / KS) + l / KS, M - 1 - m0) * (int)p.x.sld + k), s + c * 256);
+    }
+    if (wave == C::NW - 1) {
+      const int last = (N - 1) / kFp8Group - n0 / kFp8Group;
+      lds_copy_byte(ws, (uint32_t)(min(l / KS % NBLK, last) * (int)p.w.sld + k), s + BM * KS * 4);
+    }
+    if (GATE && wave == C::NW - 2)
+      lds_copy_byte(p.w2.scales + (int64_t)(n0 / kFp8Group) * p.w2.sld, (uint32_t)k, s + BM * KS * 4 + 256);
+  };
   // copy q of K step kt (of this slice) into stage st
   auto issue_one = [&](int st, int kt, int q) __attribute__((always_inline)) {
     char* s = smem + st * STAGE;
     const int64_t k = (int64_t)(k_first + kt) * 128;
     if (q < NQA) {
       lds_copy16(A + k, ao[q], s + (wave * NQA + q) * 1024);
-    } else if (q < NQA + NQB) {
-      const int c = wave * NQB + q - NQA;
-      lds_copy16((b_up(c * 8) ? B[1] : B[0]) + k, bo[q - NQA], s + TA + c * 1024);
     } else {
-      const int c = (wave * NQS + q - NQA - NQB) % C::NSB;
-      lds_copy_byte(so[q - NQA - NQB] + k_first + kt, s + TA + TB + c * 256);
+      const int c = b_copy(q - NQA);
+      lds_copy16((b_up(c * 8) ? B[1] : B[0]) + k, bo[q - NQA], s + TA + c * 1024);
     }
   };
   auto issue = [&](int st, int kt) __attribute__((always_inline)) {
+    if (kt == 0 || (k_first + kt) % KS == 0) issue_scales((k_first + kt) / KS);
 #pragma unroll
     for (int q = 0; q < LPW; ++q) issue_one(st, kt, q);
   };
@@ -173,12 +204,13 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   auto read_b = [&](int st, int j) __attribute__((always_inline)) {
     bf[j % RB] = fragment(smem + st * STAGE + TA + (wn * TN + 16 * j) * 128);
   };
-  auto read_scales = [&](int st) __attribute__((always_inline)) {
-    const int* s = (const int*)(smem + st * STAGE + TA + TB);
+  auto read_scales = [&](int kt) __attribute__((always_inline)) {
+    const int k = k_first + kt;
+    const int* s = (const int*)(smem + C::SCALES + (k / KS & 1) * SET) + k % KS;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) sa_next[i] = s[wm * TM + 16 * i + row];
+    for (int i = 0; i < FM; ++i) sa_next[i] = s[(wm * TM + 16 * i + row) * KS];
 #pragma unroll
-    for (int h = 0; h < (GATE ? 2 : 1); ++h) sb_next[h] = s[BM + wn * TN + h * (TN / 2)];
+    for (int h = 0; h < (GATE ? 2 : 1); ++h) sb_next[h] = s[BM * KS + (GATE ? 64 * h : wn * TN / 128 * KS)];
   };
   auto take_scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -190,7 +222,7 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     acc[j][i] = mma_fp8(bf[j % RB], af[i], acc[j][i], sb[GATE && j >= FN / 2 ? 1 : 0], sa[i]);
   };
   auto first_reads = [&](int st) __attribute__((always_inline)) {
-    read_scales(st);
+    read_scales(0);
 #pragma unroll
     for (int j = 0; j < RB - 1; ++j) read_b(st, j);
 #pragma unroll
@@ -199,20 +231,31 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   };
   // One K step over stage st, a row of MFMAs (one weight fragment) at a time.  The weight
   // fragment RB - 1 rows on is read at each row's start, the activations' of the next
-  // step during the last row, each behind its last use.  From row JB on the reads are
-  // the next step's: before it, that step's copies have to have landed, and behind the
-  // barrier no wave reads stage st again, so that its refill starts there.
-  constexpr int JB = FN - RB + 1, SLOTS = (FN - JB) * FM, PER = (LPW + SLOTS - 1) / SLOTS;
+  // step during the last row, each behind its last use.  So the activations' part of a
+  // stage and the rows of the first RB fragments have been read by row 1, the other rows
+  // by row JB, from where the reads are the next step's.  Both refill as soon as they
+  // have been read (a barrier tells), which keeps STAGES - 1 steps' copies in flight over
+  // each wait: with one barrier a step, at row JB, that was STAGES - 2, and two stages
+  // waited out a copy's whole latency every step.
+  constexpr int JB = FN - RB + 1, NLO = NQA + NQL;  // copies behind the first barrier
+  static_assert(JB > 1 || NQL == NQB, "one barrier where every fragment is read by row 1");
+  constexpr int SLO = (JB > 1 ? JB - 1 : FN - 1) * FM, PLO = (NLO + SLO - 1) / SLO;
+  constexpr int SHI = (FN - JB) * FM, PHI = (LPW - NLO + SHI - 1) / SHI;
+  constexpr int AHEAD = (JB > 1 ? STAGES - 1 : STAGES - 2) * LPW;
   auto step = [&](int st, int kt, auto issue_c, auto next_c) __attribute__((always_inline)) {
     constexpr bool ISSUE = decltype(issue_c)::value, NEXT = decltype(next_c)::value;
     const int nst = st + 1 == STAGES ? 0 : st + 1;
+    // (Here and not between the rows: the compiler sinks products that stand before a
+    // branch to behind it.  A set's copies count as none in the waits, which are so a
+    // little early.)
+    if (ISSUE && (k_first + kt + STAGES) % KS == 0) issue_scales((k_first + kt + STAGES) / KS);
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      if (j == JB && NEXT) {
-        if (ISSUE) wait_vmcnt<(STAGES - 2) * LPW>();
+      if ((j == 1 && JB > 1) || (j == JB && NEXT)) {
+        if (ISSUE) wait_vmcnt<AHEAD>();
         else wait_vmcnt<0>();
         __syncthreads();
-        read_scales(nst);
+        if (j == JB) read_scales(kt + 1);
       }
       if (j + RB - 1 < FN) read_b(st, j + RB - 1);
       else if (NEXT) read_b(nst, j + RB - 1 - FN);
@@ -220,10 +263,16 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
       for (int i = 0; i < FM; ++i) {
         mfma_one(j, i);
         if (j == FN - 1 && NEXT) read_a(nst, i);
-        if (j >= JB && ISSUE)
+        if (ISSUE && j >= 1 && (j < JB || JB == 1))
 #pragma unroll
-          for (int u = 0; u < PER; ++u) {
-            const int q = ((j - JB) * FM + i) * PER + u;
+          for (int u = 0; u < PLO; ++u) {
+            const int q = ((j - 1) * FM + i) * PLO + u;
+            if (q < NLO) issue_one(st, kt + STAGES, q);
+          }
+        if (ISSUE && j >= JB && JB > 1)
+#pragma unroll
+          for (int u = 0; u < PHI; ++u) {
+            const int q = NLO + ((j - JB) * FM + i) * PHI + u;
             if (q < LPW) issue_one(st, kt + STAGES, q);
           }
         __builtin_amdgcn_sched_barrier(0);
@@ -242,7 +291,7 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     char* t = smem + (STAGES - 1) * STAGE;
 #pragma unroll
     for (int q = 0; q < NQA + NQB; ++q) {
-      const int c = q < NQA ? wave * NQA + q : wave * NQB + q - NQA, r = c * 8 + lane / 8;
+      const int c = q < NQA ? wave * NQA + q : b_copy(q - NQA), r = c * 8 + lane / 8;
       const int chunk = dl_swz(r, lane % 8), k = kt0 * 128 + 16 * chunk;
       const uint8_t* base = q < NQA ? A + ao[q] : (b_up(c * 8) ? B[1] : B[0]) + bo[q - NQA];
       base -= 16 * chunk;  // the row's start
@@ -257,11 +306,12 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
       *(u64x2_t*)(t + (q < NQA ? 0 : TA) + c * 1024 + lane * 16) = v;
     }
 #pragma unroll
-    for (int q = 0; q < NQS; ++q)
-      ((int*)(t + TA + TB))[(wave * NQS + q) % C::NSB * 64 + lane] = so[q][kt0];
+    for (int i = 0; i < FM; ++i)
+      sa[i] = p.x.scales[(int64_t)min(m0 + wm * TM + 16 * i + row, M - 1) * p.x.sld + kt0];
+    const int64_t block = min(n0 + (GATE ? 0 : wn * TN), N - 1) / kFp8Group;
+    sb[0] = p.w.scales[block * p.w.sld + kt0];
+    if constexpr (GATE) sb[1] = p.w2.scales[block * p.w2.sld + kt0];
     __syncthreads();
-    read_scales(STAGES - 1);
-    take_scales();
 #pragma unroll
     for (int i = 0; i < FM; ++i) read_a(STAGES - 1, i);
 #pragma unroll
@@ -279,16 +329,11 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     __syncthreads();
     first_reads(0);
     int st = 0, kt = 0;
+    auto next = [&]() __attribute__((always_inline)) { st = st + 1 == STAGES ? 0 : st + 1; };
     const std::true_type yes;
     const std::false_type no;
-    for (; kt < KT - STAGES; ++kt) {
-      step(st, kt, yes, yes);
-      st = st + 1 == STAGES ? 0 : st + 1;
-    }
-    for (; kt < KT - 1; ++kt) {
-      step(st, kt, no, yes);
-      st = st + 1 == STAGES ? 0 : st + 1;
-    }
+    for (; kt < KT - STAGES; ++kt, next()) step(st, kt, yes, yes);
+    for (; kt < KT - 1; ++kt, next()) step(st, kt, no, yes);
     step(st, kt, no, no);
   }
 

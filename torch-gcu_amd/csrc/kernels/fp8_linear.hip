@@ -1,16 +1,17 @@
 // Products of activations and a weight in 8-bit floating point, and the gate and up
 // products of a feed-forward layer with silu(gate) up as codes again.
-#include "fp8_gemm.h"
+#include "fp8_rows.h"
 
 namespace mi {
 namespace {
 
-typedef F8Cfg<4, 2, 64, 128, 2> F256;     // 256 x 256
+typedef F8Cfg<4, 2, 64, 128, 2> F256;     // 256 x 256 (a gate's 128 gate and 128 up columns)
 typedef F8Cfg<4, 2, 64, 64, 3> F256x128;
-typedef F8Cfg<2, 2, 64, 64, 4> F128;
-typedef F8Cfg<2, 2, 32, 32, 5> F64;
-typedef F8Cfg<2, 4, 64, 64, 3> G128;      // a gate's 128 x (128 gate, 128 up)
-typedef F8Cfg<2, 4, 32, 64, 3> G64;
+typedef F8Cfg<2, 2, 64, 64, 2> F128;
+typedef F8Cfg<2, 4, 32, 32, 3> F64x128;
+typedef F8Cfg<2, 2, 32, 32, 4> F64;
+typedef F8Cfg<2, 4, 64, 64, 2> G128;      // a gate's 128 x (128 and 128)
+typedef F8Cfg<2, 4, 32, 64, 2> G64;
 
 // out = the slices' sums in order (+ bias) (+ residual), 4 columns a thread
 __global__ __launch_bounds__(256) void fp8_combine_kernel(Fp8Gemm p, int S) {
@@ -109,38 +110,151 @@ mi_status_t launch(Fp8Gemm q, int S, hipStream_t s, const char* op) {
   return launch_combine(q, GATE, S, s, op);
 }
 
-int64_t tiles_of(const Fp8Gemm& q, int bm, int bn) {
-  return ((q.M + bm - 1) / bm) * (int64_t)((q.N + bn - 1) / bn);
+// Few rows of activations: one launch, or for a gate its y in float32 and then the codes.
+template <class C, bool GATE>
+mi_status_t launch_few(Fp8Gemm q, hipStream_t s, const char* op) {
+  static const bool attr = [] {
+    (void)hipFuncSetAttribute((const void*)fp8_rows_gemm_kernel<C, GATE>,
+                              hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    return true;
+  }();
+  (void)attr;
+  constexpr int COLS = 16 * (GATE ? C::RT / 2 : C::RT);
+  Workspace ws;
+  if (GATE) {
+    q.ldp = ((int64_t)q.N + 3) / 4 * 4;
+    MI_RETURN_IF(ws.alloc((size_t)(q.M * q.ldp) * sizeof(float), s));
+    q.part = (float*)ws.get();
+  }
+  hipLaunchKernelGGL((fp8_rows_gemm_kernel<C, GATE>), dim3(ceil_div_u(q.N, COLS)), dim3(64 * C::NW),
+                     C::lds((size_t)fp8_groups(q.K)), s, q);
+  MI_RETURN_IF(check_launch(op));
+  return GATE ? fp8_quantize_f32(q.part, q.ldp, q.M, q.N, q.codes, s, op) : MI_OK;
 }
 
+// Tile shapes and slices of K by a cost in us: rounds of `per_cu` blocks a CU, each of
+// `steps` K steps of lo (few CUs busy) to hi (all busy) to hi2 (two blocks on each) us, or
+// the weight's stream at 5.6 TB/s; launch, first latency and epilogue; what every further
+// round adds; and for slices their sums through the caches.  The constants are a fit to
+// timings of these kernels (46 products and 24 gates, M 17 .. 7700, N 256 .. 16000, K 256
+// .. 10600): what they pick was within 1 % of the fastest of the shapes on average, 18 %
+// at worst.  Slices of the larger tiles were never the fastest.
+struct Shape {
+  int bm, bn, per_cu;
+  float fixed, lo, hi, hi2, round;
+  int slices[3];
+};
+constexpr Shape kShapes[] = {{256, 256, 1, 10.1f, 1.53f, 1.74f, 0, 6.0f, {1}},
+                             {256, 128, 1, 6.3f, 0.89f, 0.89f, 0, 10.2f, {1}},
+                             {128, 128, 2, 6.2f, 0.39f, 0.60f, 0.97f, 3.4f, {1}},
+                             {64, 128, 2, 3.7f, 0.24f, 0.89f, 0.89f, 1.6f, {1}},
+                             {64, 64, 2, 3.1f, 0.195f, 0.286f, 0.63f, 5.6f, {1, 2, 4}}};
+constexpr Shape kGateShapes[] = {{256, 128, 1, 9.7f, 0.92f, 1.48f, 0, 5.6f, {1}},
+                                 {128, 128, 2, 5.7f, 0.70f, 1.10f, 2.4f, 0.f, {1, 2}},
+                                 {64, 128, 2, 4.0f, 0.46f, 0.94f, 1.9f, 5.2f, {1, 2, 4}}};
+
+struct Pick {
+  int shape, slices;
+  float cost;
+};
+
+template <int COUNT>
+Pick pick_shape(const Fp8Gemm& q, const Shape (&shapes)[COUNT], int products, float slice_fixed) {
+  const float cus = (float)cu_count();
+  const int64_t ksteps = ((int64_t)q.K + 127) / 128;
+  Pick best{0, 1, 3e38f};
+  for (int i = 0; i < COUNT; ++i) {
+    const Shape& c = shapes[i];
+    const int64_t tiles = (((int64_t)q.M + c.bm - 1) / c.bm) * (((int64_t)q.N + c.bn - 1) / c.bn);
+    for (int s : c.slices) {
+      if (s == 0 || (s > 1 && ksteps < 2 * s)) break;
+      const float steps = (float)((ksteps + s - 1) / s), load = (float)(tiles * s) / cus;
+      auto step = [&](float l) { return l <= 1.f ? c.lo + (c.hi - c.lo) * l : c.hi + (c.hi2 - c.hi) * (l - 1.f); };
+      const float full = std::floor(load / (float)c.per_cu), rest = load - full * (float)c.per_cu;
+      float t = full * steps * step((float)c.per_cu) + (rest > 0.f ? steps * step(rest) : 0.f);
+      t = c.fixed + std::max(t, (float)q.N * (float)q.K * (float)products * (1.f / 5.6e6f)) +
+          c.round * std::max(0.f, full - (rest > 0.f ? 0.f : 1.f));
+      if (s > 1) t += slice_fixed + (float)(s * products) * (float)q.M * (float)q.N * 2.2e-6f;
+      if (t < best.cost) best = Pick{i, s, t};
+    }
+  }
+  return best;
+}
+
+// The few-row kernels' cost: the weight's stream, or what the busiest CU takes in (its
+// blocks' 16 (a gate's 32) weight rows and all rows of x, at `rate` bytes a us).
+float few_cost(const Fp8Gemm& q, int products, float fixed, float rate) {
+  const float blocks = (float)(((int64_t)q.N + 15) / 16) / (float)cu_count();
+  const float bytes = (float)(16 * products + (q.M + 7) / 8 * 8) * (float)q.K;
+  return fixed + std::max((float)q.N * (float)q.K * (float)products * (1.f / 5.5e6f),
+                          std::max(1.f, blocks) * bytes / rate);
+}
+
+constexpr int kFewRows = 64;
+template <class C>
+bool fits(const Fp8Gemm& q) {
+  return q.M <= 8 * C::XR && C::lds((size_t)fp8_groups(q.K)) <= 160 * 1024;
+}
+
+// Up to 16 rows the few-row kernel (M8 N4096 K4096 5.3 us, in 64 x 64 tiles cut in four
+// 8.5; M16 N32000 K4096 28 and 32), up to 64 whichever costs less (M48 N4096 K4096 7.5 and
+// 9.3, K11008 14.5 and 13.5).  Its blocks have 16 weight rows; 32 or 64 of them were no
+// faster anywhere.
 mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
-  const int64_t cus = cu_count();
-  auto slices = [&](int64_t tiles) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>({8, cus / tiles, q.K / 256}));
-  };
-  if (q.M > 128 && tiles_of(q, 256, 256) >= cus) return launch<F256, false>(q, 1, s, op);
-  if (q.M > 128 && tiles_of(q, 256, 128) >= cus) return launch<F256x128, false>(q, 1, s, op);
-  const int64_t t = tiles_of(q, 128, 128);
-  if (q.M > 64 && 2 * t >= cus) return launch<F128, false>(q, slices(t), s, op);
-  return launch<F64, false>(q, slices(tiles_of(q, 64, 64)), s, op);
+  const Pick c = pick_shape(q, kShapes, 1, 2.5f);
+  if (q.M <= kFewRows && (q.M <= 16 || few_cost(q, 1, 2.2f, 52e3f) <= c.cost)) {
+    if (fits<R8Cfg<1, 1, 8, 2>>(q)) return launch_few<R8Cfg<1, 1, 8, 2>, false>(q, s, op);
+    if (fits<R8Cfg<2, 1, 4, 3>>(q)) return launch_few<R8Cfg<2, 1, 4, 3>, false>(q, s, op);
+    if (fits<R8Cfg<3, 1, 8, 2>>(q)) return launch_few<R8Cfg<3, 1, 8, 2>, false>(q, s, op);
+    if (fits<R8Cfg<4, 1, 4, 2>>(q)) return launch_few<R8Cfg<4, 1, 4, 2>, false>(q, s, op);
+    if (fits<R8Cfg<6, 1, 4, 2>>(q)) return launch_few<R8Cfg<6, 1, 4, 2>, false>(q, s, op);
+    if (fits<R8Cfg<8, 1, 4, 2>>(q)) return launch_few<R8Cfg<8, 1, 4, 2>, false>(q, s, op);
+  }
+  switch (c.shape) {
+    case 0: return launch<F256, false>(q, 1, s, op);
+    case 1: return launch<F256x128, false>(q, 1, s, op);
+    case 2: return launch<F128, false>(q, 1, s, op);
+    case 3: return launch<F64x128, false>(q, 1, s, op);
+    default: return launch<F64, false>(q, c.slices, s, op);
+  }
 }
 
+// The same; the few-row kernel's two launches against one or two (M16 N32000 K4096 52 us and
+// 63 in 64-row tiles, M64 N11008 K4096 30 and 25.5).
 mi_status_t run_gate(const Fp8Gemm& q, hipStream_t s, const char* op) {
-  const int64_t cus = cu_count();
-  auto slices = [&](int64_t tiles) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>({8, cus / tiles, q.K / 256}));
-  };
-  if (q.M > 128 && tiles_of(q, 256, 128) >= cus) return launch<F256, true>(q, 1, s, op);
-  if (q.M > 64) return launch<G128, true>(q, slices(tiles_of(q, 128, 128)), s, op);
-  return launch<G64, true>(q, slices(tiles_of(q, 64, 128)), s, op);
+  const Pick c = pick_shape(q, kGateShapes, 2, 2.2f);
+  if (q.M <= kFewRows && (q.M <= 16 || few_cost(q, 2, 4.8f, 42e3f) <= c.cost)) {
+    if (fits<R8Cfg<1, 2, 4, 2>>(q)) return launch_few<R8Cfg<1, 2, 4, 2>, true>(q, s, op);
+    if (fits<R8Cfg<2, 2, 4, 2>>(q)) return launch_few<R8Cfg<2, 2, 4, 2>, true>(q, s, op);
+    if (fits<R8Cfg<4, 2, 4, 2>>(q)) return launch_few<R8Cfg<4, 2, 4, 2>, true>(q, s, op);
+    if (fits<R8Cfg<8, 2, 4, 2>>(q)) return launch_few<R8Cfg<8, 2, 4, 2>, true>(q, s, op);
+  }
+  switch (c.shape) {
+    case 0: return launch<F256, true>(q, 1, s, op);
+    case 1: return launch<G128, true>(q, c.slices, s, op);
+    default: return launch<G64, true>(q, c.slices, s, op);
+  }
 }
 
 // Offsets inside a block's 256 rows are 32-bit byte counts.
 constexpr int64_t kFarRows = 1 << 22;
 
-// Rows of 16-byte aligned codes: the operand itself, or a copy in workspace.
+// Rows of 16-byte aligned codes, and scales whose rows are near: the operand itself, or
+// copies in workspace.
 mi_status_t aligned_rows(const mi_fp8_t* t, Fp8Mat* m, Workspace* ws, hipStream_t s) {
   const int64_t rows = t->codes.sizes[0], cols = t->codes.sizes[1];
+  if (t->scales.sizes[0] <= 1) {
+    m->sld = 0;
+  } else if (m->sld >= kFarRows) {
+    mi_tensor_t to = t->scales;
+    to.strides[0] = to.sizes[1];
+    to.strides[1] = 1;
+    MI_RETURN_IF(ws[1].alloc((size_t)(to.sizes[0] * to.sizes[1]), s));
+    to.data = ws[1].get();
+    MI_RETURN_IF(mi_copy(&to, &t->scales, (mi_stream_t)s));
+    m->scales = (uint8_t*)to.data;
+    m->sld = to.sizes[1];
+  }
   if ((uintptr_t)m->codes % 16 == 0 && ((m->ld % 16 == 0 && m->ld < kFarRows) || rows <= 1)) {
     if (rows <= 1) m->ld = 0;
     return MI_OK;
@@ -218,9 +332,9 @@ mi_status_t mi_fp8_linear(const mi_tensor_t* out, const mi_fp8_t* x, const mi_fp
   q.out = out->data;
   q.ldc = out->strides[0];
   q.f16 = out->dtype == MI_F16;
-  Workspace wx, ww;
-  MI_RETURN_IF(aligned_rows(x, &q.x, &wx, s));
-  MI_RETURN_IF(aligned_rows(weight, &q.w, &ww, s));
+  Workspace wx[2], ww[2];
+  MI_RETURN_IF(aligned_rows(x, &q.x, wx, s));
+  MI_RETURN_IF(aligned_rows(weight, &q.w, ww, s));
   return run_linear(q, s, op);
 }
 
@@ -246,10 +360,10 @@ mi_status_t mi_fp8_linear_silu_mul(const mi_fp8_t* out, const mi_fp8_t* x, const
       MI_RETURN_IF(fp8_check_apart(op, "out", mine, "scales", &t->scales));
     }
   if (q.M == 0 || q.N == 0) return MI_OK;
-  Workspace wx, wg, wu;
-  MI_RETURN_IF(aligned_rows(x, &q.x, &wx, s));
-  MI_RETURN_IF(aligned_rows(w_gate, &q.w, &wg, s));
-  MI_RETURN_IF(aligned_rows(w_up, &q.w2, &wu, s));
+  Workspace wx[2], wg[2], wu[2];
+  MI_RETURN_IF(aligned_rows(x, &q.x, wx, s));
+  MI_RETURN_IF(aligned_rows(w_gate, &q.w, wg, s));
+  MI_RETURN_IF(aligned_rows(w_up, &q.w2, wu, s));
   return run_gate(q, s, op);
 }
 

@@ -14,7 +14,7 @@
 namespace mi {
 namespace {
 
-constexpr int QUANT = 0, NORM = 1, NORM_RES = 2;
+constexpr int NORM = 0, NORM_RES = 1;
 
 struct RowsArgs {
   const void* x;
@@ -38,37 +38,42 @@ struct Eight {
     St e[8];
   };
   __device__ __forceinline__ float get(int i) const { return Num<T>::load(e[i]); }
-  // VEC: the row is 16-byte aligned and its length a multiple of 8
-  template <bool VEC>
+  // A row's elements col .. col + 7, zeros behind its end.  Rows may begin anywhere (a
+  // global load takes any address); those whose length is no multiple of 8 end with
+  // single elements.
+  typedef typename AnyAligned<sizeof(St)>::type vec;
   static __device__ __forceinline__ Eight load(const void* row, int col, int cols) {
     Eight r;
-    if constexpr (VEC) {
+    const St* p = (const St*)row;
+    if (cols >= 8) {
 #pragma unroll
       for (int i = 0; i < W / 4; ++i) {
-        const u32x4_t v = *((const u32x4_t*)((const St*)row + min(col, cols - 8)) + i);
+        const u32x4_t v = *((const vec*)(p + min(col, cols - 8)) + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) r.w[4 * i + j] = col < cols ? v[j] : 0u;
       }
-    } else {
+    }
+    if ((cols & 7) != 0 && col < cols && col + 8 > cols) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const St v = ((const St*)row)[min(col + i, cols - 1)];
-        r.e[i] = col + i < cols ? v : (St)0;
-      }
+      for (int i = 0; i < 8; ++i) r.e[i] = p[min(col + i, cols - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.e[i] = col + i < cols ? r.e[i] : (St)0;
+    } else if (cols < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.e[i] = (St)0;
     }
     return r;
   }
-  template <bool VEC>
   __device__ __forceinline__ void store(void* row, int col, int cols) const {
-    if constexpr (VEC) {
-      if (col < cols)
+    St* p = (St*)row + col;
+    if (col + 8 <= cols) {
 #pragma unroll
-        for (int i = 0; i < W / 4; ++i)
-          *((u32x4_t*)((St*)row + col) + i) = u32x4_t{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+      for (int i = 0; i < W / 4; ++i)
+        *((vec*)p + i) = u32x4_t{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (col + i < cols) ((St*)row)[col + i] = e[i];
+        if (col + i < cols) p[i] = e[i];
     }
   }
 };
@@ -105,10 +110,10 @@ __device__ __forceinline__ uint32_t largest_bits(const float* y) {
   return m;
 }
 
-template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, f8_u32x2 c) {
-  if constexpr (VEC) {
-    if (col < cols) *(f8_u32x2*)(row + col) = c;
+  typedef f8_u32x2 __attribute__((aligned(1))) vec;
+  if (col + 8 <= cols) {
+    *(vec*)(row + col) = c;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -116,9 +121,26 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, f8_
   }
 }
 
-// TPR threads a row, VPL x 8 elements a thread in registers; VPL 0: rows of any
+// A wave to 512 columns of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(RowsArgs a, int chunks) {
+  typedef Eight<T> E;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = id / chunks;
+  if (row >= a.rows) return;
+  const int col = (int)(id - row * chunks) * 512 + (threadIdx.x & 63) * 8;
+  const E v = E::load((const typename E::St*)a.x + row * a.x_ld, col, a.cols);
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = v.get(j);
+  uint32_t byte;
+  const f8_u32x2 c = codes_of(y, row16_max(largest_bits(y)), row16_max, &byte);
+  store_codes(a.out.codes + row * a.out.ld, col, a.cols, c);
+  if ((threadIdx.x & 15) == 0 && col < a.cols) a.out.scales[row * a.out.sld + col / kFp8Group] = (uint8_t)byte;
+}
+
+// The norm: TPR threads a row, VPL x 8 elements a thread in registers; VPL 0: rows of any
 // length, read again for the codes (the total from where it was written).
-template <typename T, int KIND, int TPR, int VPL, bool VEC>
+template <typename T, int KIND, int TPR, int VPL>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   typedef Eight<T> E;
   typedef typename E::St St;
@@ -135,15 +157,15 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   uint8_t* scales = a.out.scales + row * a.out.sld;
   E v[N], r[N];
   auto load = [&](int i, int col) __attribute__((always_inline)) {
-    v[i] = E::template load<VEC>(x, col, cols);
-    if constexpr (KIND == NORM_RES) r[i] = E::template load<VEC>(res, col, cols);
+    v[i] = E::load(x, col, cols);
+    if constexpr (KIND == NORM_RES) r[i] = E::load(res, col, cols);
   };
   float ss = 0.f;
   auto add_up = [&](int i, int col) __attribute__((always_inline)) {
     if constexpr (KIND == NORM_RES) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i].e[j] = Num<T>::store(v[i].get(j) + r[i].get(j));
-      v[i].template store<VEC>(total, col, cols);
+      v[i].store(total, col, cols);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(v[i].get(j), v[i].get(j), ss);
@@ -151,31 +173,27 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   if constexpr (VPL > 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) load(i, t * 8 + i * STEP);
-    if constexpr (KIND != QUANT)
 #pragma unroll
-      for (int i = 0; i < N; ++i) add_up(i, t * 8 + i * STEP);
-  } else if constexpr (KIND != QUANT) {
+    for (int i = 0; i < N; ++i) add_up(i, t * 8 + i * STEP);
+  } else {
     for (int c = t * 8; c < cols; c += STEP) {
       load(0, c);
       add_up(0, c);
     }
   }
-  float norm = 1.f;
-  if constexpr (KIND != QUANT) {
-    ss = wave_sum(ss);
-    if constexpr (TPR == 256) {
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
-      __syncthreads();
-      ss = (red[0] + red[1]) + (red[2] + red[3]);
-    }
-    norm = 1.0f / __builtin_sqrtf(ss / (float)cols + a.eps);
+  ss = wave_sum(ss);
+  if constexpr (TPR == 256) {
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    ss = (red[0] + red[1]) + (red[2] + red[3]);
   }
+  const float norm = 1.0f / __builtin_sqrtf(ss / (float)cols + a.eps);
   auto finish = [&](const E& s, int col) __attribute__((always_inline)) {
     float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = KIND == QUANT ? s.get(j) : s.get(j) * norm;
-    if (KIND != QUANT && a.weight != nullptr) {
-      const E w = E::template load<VEC>(a.weight, col, cols);
+    for (int j = 0; j < 8; ++j) y[j] = s.get(j) * norm;
+    if (a.weight != nullptr) {
+      const E w = E::load(a.weight, col, cols);
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] *= w.get(j);
     }
@@ -183,13 +201,13 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
     if (col >= cols) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = 0.f;
-    } else if (!VEC) {
+    } else if ((cols & 7) != 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = col + j < cols ? y[j] : 0.f;
     }
     uint32_t byte;
     const f8_u32x2 c = codes_of(y, row16_max(largest_bits(y)), row16_max, &byte);
-    store_codes<VEC>(codes, col, cols, c);
+    store_codes(codes, col, cols, c);
     if ((t & 15) == 0 && col < cols) scales[col / kFp8Group] = (uint8_t)byte;
   };
   if constexpr (VPL > 0) {
@@ -198,12 +216,12 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   } else {
     // whole rows of 16 lanes take part in a group's maximum
     for (int c = t * 8; c / kFp8Group * kFp8Group < cols; c += STEP)
-      finish(E::template load<VEC>(KIND == NORM_RES ? total : x, c, cols), c);
+      finish(E::load(KIND == NORM_RES ? total : x, c, cols), c);
   }
 }
 
 // A block of 256 threads to a 128 x 128 block of the weight, 8 rows a thread.
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void fp8_weight_kernel(const void* w, int64_t ld, int64_t rows, int cols,
                                                          Fp8Mat out) {
   typedef Eight<T> E;
@@ -214,7 +232,7 @@ __global__ __launch_bounds__(256) void fp8_weight_kernel(const void* w, int64_t 
   E v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    v[i] = E::template load<VEC>((const St*)w + min(row0 + 16 * i, rows - 1) * ld, col, cols);
+    v[i] = E::load((const St*)w + min(row0 + 16 * i, rows - 1) * ld, col, cols);
   auto block_max = [&](uint32_t m) __attribute__((always_inline)) {
     m = row16_max(m);
     m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
@@ -247,48 +265,54 @@ __global__ __launch_bounds__(256) void fp8_weight_kernel(const void* w, int64_t 
     if (row >= rows) break;
     const f8_u32x2 c = {fp8_codes4(v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3), inv),
                         fp8_codes4(v[i].get(4), v[i].get(5), v[i].get(6), v[i].get(7), inv)};
-    store_codes<VEC>(out.codes + row * out.ld, col, cols, c);
+    store_codes(out.codes + row * out.ld, col, cols, c);
   }
   if (threadIdx.x == 0) out.scales[blockIdx.y * out.sld + blockIdx.x] = (uint8_t)byte;
 }
 
-// 16-byte accesses to the rows of a wide tensor, 8-byte ones to the codes
-bool aligned(const void* p, int64_t ld, int size) {
-  return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0;
+// A wave to 512 columns.  us (bytes moved): f16 rows of 11008 out of 22016, 6011 of them, 40.0
+// (198 MB, 5.0 TB/s), with 2048 columns a wave 44.2, with a block to a row 55.7; bf16
+// 8192 x 4096 21.6, 24.8, 19.8; one row of 4096 2.7, 2.9, 2.9 (launch 2.1).
+template <typename T>
+mi_status_t launch_quantize(const RowsArgs& a, hipStream_t s, const char* op) {
+  const int64_t chunks = (a.cols + 511) / 512;
+  if ((a.rows * chunks + 3) / 4 > 0x7fffffff) MI_FAIL(MI_ERR_TOO_LARGE, "%s: too many rows", op);
+  hipLaunchKernelGGL((fp8_quantize_kernel<T>), dim3(ceil_div_u(a.rows * chunks, 4)), dim3(256), 0, s, a,
+                     (int)chunks);
+  return check_launch(op);
 }
-bool aligned_codes(const Fp8Mat& m) { return (uintptr_t)m.codes % 8 == 0 && m.ld % 8 == 0; }
 
+// Up to 1024 columns a wave holds a row, above a block; rows over 8192 are read again for
+// the codes.  us, with the residual: bf16 8192 x 1024 13.3 (with a block a row 16.4), 8192 x
+// 4096 46.4 (235 MB, 5.1 TB/s; with a wave a row 65), 8 x 4096 4.3 (9.6), 4096 x 11008 84
+// (107 with the row held).
 template <typename T, int KIND>
-mi_status_t launch_rows(const RowsArgs& a, bool vec, hipStream_t s, const char* op) {
-  auto go = [&](auto tpr, auto vpl, auto v) {
+mi_status_t launch_norm(const RowsArgs& a, hipStream_t s, const char* op) {
+  auto go = [&](auto tpr, auto vpl) {
     constexpr int TPR = decltype(tpr)::value;
-    hipLaunchKernelGGL((fp8_rows_kernel<T, KIND, TPR, decltype(vpl)::value, decltype(v)::value>),
+    hipLaunchKernelGGL((fp8_rows_kernel<T, KIND, TPR, decltype(vpl)::value>),
                        dim3(ceil_div_u(a.rows, 256 / TPR)), dim3(256), 0, s, a);
     return check_launch(op);
   };
   const std::integral_constant<int, 64> wave;
   const std::integral_constant<int, 256> block;
-  const std::true_type yes;
   const std::integral_constant<int, 0> any;
   const std::integral_constant<int, 1> one;
   const std::integral_constant<int, 2> two;
   const std::integral_constant<int, 4> four;
-  const std::integral_constant<int, 8> eight;
-  if (!vec) return go(block, any, std::false_type());
-  if (a.cols <= 512) return go(wave, one, yes);
-  if (a.cols <= 1024) return go(wave, two, yes);
-  if (a.cols <= 2048) return go(block, one, yes);
-  if (a.cols <= 4096) return go(block, two, yes);
-  if (a.cols <= 8192) return go(block, four, yes);
-  if (a.cols <= 16384) return go(block, eight, yes);
-  return go(block, any, yes);
+  if (a.cols <= 512) return go(wave, one);
+  if (a.cols <= 1024) return go(wave, two);
+  if (a.cols <= 2048) return go(block, one);
+  if (a.cols <= 4096) return go(block, two);
+  if (a.cols <= 8192) return go(block, four);
+  return go(block, any);
 }
 
 template <int KIND>
-mi_status_t run_rows(const RowsArgs& a, int dtype, bool vec, hipStream_t s, const char* op) {
-  if (dtype == MI_BF16) return launch_rows<BF16, KIND>(a, vec, s, op);
-  if (dtype == MI_F16) return launch_rows<F16, KIND>(a, vec, s, op);
-  return launch_rows<float, KIND>(a, vec, s, op);
+mi_status_t run_norm(const RowsArgs& a, int dtype, hipStream_t s, const char* op) {
+  if (dtype == MI_BF16) return launch_norm<BF16, KIND>(a, s, op);
+  if (dtype == MI_F16) return launch_norm<F16, KIND>(a, s, op);
+  return launch_norm<float, KIND>(a, s, op);
 }
 
 mi_status_t check_shape(const char* op, const mi_fp8_t* out, const mi_tensor_t* x, const char* name) {
@@ -305,6 +329,18 @@ mi_status_t check_outputs_apart(const char* op, const mi_fp8_t* out, const char*
 }
 
 }  // namespace
+
+mi_status_t fp8_quantize_f32(const float* y, int64_t ld, int64_t rows, int cols, const Fp8Mat& out,
+                             hipStream_t s, const char* op) {
+  RowsArgs a{};
+  a.x = y;
+  a.x_ld = ld;
+  a.rows = rows;
+  a.cols = cols;
+  a.out = out;
+  return launch_quantize<float>(a, s, op);
+}
+
 }  // namespace mi
 
 using namespace mi;
@@ -324,9 +360,9 @@ mi_status_t mi_fp8_quantize(const mi_fp8_t* out, const mi_tensor_t* x, mi_stream
   a.x_ld = x->strides[0];
   a.rows = x->sizes[0];
   a.cols = (int)x->sizes[1];
-  const bool vec = a.cols % 8 == 0 && aligned(x->data, x->strides[0], dtype_size(x->dtype)) &&
-                   aligned_codes(a.out);
-  return run_rows<QUANT>(a, x->dtype, vec, (hipStream_t)stream, op);
+  hipStream_t s = (hipStream_t)stream;
+  if (x->dtype == MI_BF16) return launch_quantize<BF16>(a, s, op);
+  return x->dtype == MI_F16 ? launch_quantize<F16>(a, s, op) : launch_quantize<float>(a, s, op);
 }
 
 mi_status_t mi_fp8_quantize_weight(const mi_fp8_t* out, const mi_tensor_t* weight, mi_stream_t stream) {
@@ -341,17 +377,12 @@ mi_status_t mi_fp8_quantize_weight(const mi_fp8_t* out, const mi_tensor_t* weigh
   const int64_t rows = weight->sizes[0], cols = weight->sizes[1], ld = weight->strides[0];
   if (fp8_groups(rows) > 65535) MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 65535 x 128 rows", op);
   const dim3 grid((unsigned)fp8_groups(cols), (unsigned)fp8_groups(rows));
-  const bool vec = cols % 8 == 0 && aligned(weight->data, ld, dtype_size(weight->dtype)) && aligned_codes(m);
-  auto go = [&](auto type, auto v) {
-    hipLaunchKernelGGL((fp8_weight_kernel<decltype(type), decltype(v)::value>), grid, dim3(256), 0,
-                       (hipStream_t)stream, weight->data, ld, rows, (int)cols, m);
+  auto go = [&](auto type) {
+    hipLaunchKernelGGL((fp8_weight_kernel<decltype(type)>), grid, dim3(256), 0, (hipStream_t)stream,
+                       weight->data, ld, rows, (int)cols, m);
     return check_launch(op);
   };
-  const std::true_type yes;
-  const std::false_type no;
-  if (weight->dtype == MI_BF16) return vec ? go(BF16{}, yes) : go(BF16{}, no);
-  if (weight->dtype == MI_F16) return vec ? go(F16{}, yes) : go(F16{}, no);
-  return vec ? go(0.f, yes) : go(0.f, no);
+  return weight->dtype == MI_BF16 ? go(BF16{}) : weight->dtype == MI_F16 ? go(F16{}) : go(0.f);
 }
 
 mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const mi_tensor_t* x,
@@ -364,8 +395,6 @@ mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const
   MI_RETURN_IF(fp8_check_wide(op, "x", x, true));
   MI_RETURN_IF(check_shape(op, out, x, "x"));
   MI_RETURN_IF(check_outputs_apart(op, out, "x", x));
-  const int size = dtype_size(x->dtype);
-  bool vec = x->sizes[1] % 8 == 0 && aligned(x->data, x->strides[0], size) && aligned_codes(a.out);
   const bool has_res = residual != nullptr && residual->data != nullptr;
   const bool has_w = weight != nullptr && weight->data != nullptr;
   if (has_res) {
@@ -382,7 +411,6 @@ mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const
       const mi_tensor_t* in = i == 0 ? x : residual;
       if (!(in->data == total->data && (in->sizes[0] <= 1 || in->strides[0] == total->strides[0])))
         MI_RETURN_IF(fp8_check_apart(op, "total", total, i == 0 ? "x" : "residual", in));
-      vec = vec && aligned(ts[i]->data, ts[i]->strides[0], size);
     }
     MI_CHECK_ARG(total->sizes[0] <= 1 || total->strides[0] >= total->sizes[1], "%s: rows of total overlap",
                  op);
@@ -398,7 +426,6 @@ mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const
                  "%s: weight must be a dense vector of x's type and columns", op);
     MI_RETURN_IF(check_outputs_apart(op, out, "weight", weight));
     if (has_res) MI_RETURN_IF(fp8_check_apart(op, "total", total, "weight", weight));
-    vec = vec && (uintptr_t)weight->data % 16 == 0;
     a.weight = weight->data;
   }
   if (has_res) {
@@ -411,8 +438,8 @@ mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const
   a.rows = x->sizes[0];
   a.cols = (int)x->sizes[1];
   a.eps = (float)eps;
-  return has_res ? run_rows<NORM_RES>(a, x->dtype, vec, (hipStream_t)stream, op)
-                 : run_rows<NORM>(a, x->dtype, vec, (hipStream_t)stream, op);
+  return has_res ? run_norm<NORM_RES>(a, x->dtype, (hipStream_t)stream, op)
+                 : run_norm<NORM>(a, x->dtype, (hipStream_t)stream, op);
 }
 
 }  // extern "C"
