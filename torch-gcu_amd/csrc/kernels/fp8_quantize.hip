@@ -34,7 +34,7 @@ struct Eight {
   typedef typename Num<T>::storage St;
   static constexpr int W = sizeof(St) * 2;  // 32-bit words
   union {
-    uint32_t w[W];
+    uint32_t w[W] = {};
     St e[8];
   };
   __device__ __forceinline__ float get(int i) const { return Num<T>::load(e[i]); }
@@ -43,24 +43,28 @@ struct Eight {
   // single elements.
   typedef typename AnyAligned<sizeof(St)>::type vec;
   static __device__ __forceinline__ Eight load(const void* row, int col, int cols) {
-    Eight r;
     const St* p = (const St*)row;
-    if (cols >= 8) {
+    return cols >= 8 ? load_ragged(p, whole(p, min(col, cols - 8)), col, cols) : load_ragged(p, Eight(), col, cols);
+  }
+  // elements col .. col + 7, all of which are the row's
+  static __device__ __forceinline__ Eight whole(const St* p, int col) {
+    Eight r;
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i) {
-        const u32x4_t v = *((const vec*)(p + min(col, cols - 8)) + i);
+    for (int i = 0; i < W / 4; ++i) {
+      const u32x4_t v = *((const vec*)(p + col) + i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r.w[4 * i + j] = col < cols ? v[j] : 0u;
-      }
+      for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
     }
+    return r;
+  }
+  static __device__ __forceinline__ Eight load_ragged(const St* p, Eight r, int col, int cols) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i] = col < cols ? r.w[i] : 0u;
     if ((cols & 7) != 0 && col < cols && col + 8 > cols) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.e[i] = p[min(col + i, cols - 1)];
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.e[i] = col + i < cols ? r.e[i] : (St)0;
-    } else if (cols < 8) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) r.e[i] = (St)0;
     }
     return r;
   }
@@ -220,52 +224,63 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   }
 }
 
-// A block of 256 threads to a 128 x 128 block of the weight, 8 rows a thread.
+// A block of 512 threads to a 128 x 128 block of the weight, 4 rows a thread.
 template <typename T>
-__global__ __launch_bounds__(256) void fp8_weight_kernel(const void* w, int64_t ld, int64_t rows, int cols,
+__global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t ld, int64_t rows, int cols,
                                                          Fp8Mat out) {
   typedef Eight<T> E;
   typedef typename E::St St;
-  __shared__ uint32_t red[4];
+  constexpr int R = 4, NW = 8;
+  __shared__ uint32_t red[2][NW];
   const int col = blockIdx.x * kFp8Group + (threadIdx.x & 15) * 8;
   const int64_t row0 = (int64_t)blockIdx.y * kFp8Group + (threadIdx.x >> 4);
-  E v[8];
+  // (rows past the end read the last one again, which is in the block)
+  const St* p[R];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    v[i] = E::load((const St*)w + min(row0 + 16 * i, rows - 1) * ld, col, cols);
-  auto block_max = [&](uint32_t m) __attribute__((always_inline)) {
+  for (int i = 0; i < R; ++i) p[i] = (const St*)w + min(row0 + 32 * i, rows - 1) * ld;
+  E v[R];
+  if ((cols & 7) == 0 || (int)(blockIdx.x + 1) * kFp8Group <= cols) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = E::whole(p[i], min(col, cols - 8));
+    if (col >= cols)
+#pragma unroll
+      for (int i = 0; i < R; ++i) v[i] = E();
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = E::load(p[i], col, cols);
+  }
+  auto block_max = [&](uint32_t m, int turn) __attribute__((always_inline)) {
     m = row16_max(m);
     m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
     m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+    if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = m;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    return max(max(red[0], red[1]), max(red[2], red[3]));
+    m = red[turn][0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) m = max(m, red[turn][i]);
+    return m;
   };
-  // (rows past the end read the last one again, which is in the block)
   uint32_t most = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i].get(j)) & kFp8AbsMask);
-  most = block_max(most);
+  most = block_max(most, 0);
   if (most >= kFp8Inf) {  // the same for the whole block
     most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) most = max(most, fp8_finite_bits(v[i].get(j)));
-    most = block_max(most);
+    most = block_max(most, 1);
   }
   const uint32_t byte = fp8_scale_byte(most);
   const float inv = fp8_inverse(byte);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t row = row0 + 16 * i;
-    if (row >= rows) break;
+  for (int i = 0; i < R; ++i) {
     const f8_u32x2 c = {fp8_codes4(v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3), inv),
                         fp8_codes4(v[i].get(4), v[i].get(5), v[i].get(6), v[i].get(7), inv)};
-    store_codes(out.codes + row * out.ld, col, cols, c);
+    if (row0 + 32 * i < rows) store_codes(out.codes + (row0 + 32 * i) * out.ld, col, cols, c);
   }
   if (threadIdx.x == 0) out.scales[blockIdx.y * out.sld + blockIdx.x] = (uint8_t)byte;
 }
@@ -378,7 +393,7 @@ mi_status_t mi_fp8_quantize_weight(const mi_fp8_t* out, const mi_tensor_t* weigh
   if (fp8_groups(rows) > 65535) MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 65535 x 128 rows", op);
   const dim3 grid((unsigned)fp8_groups(cols), (unsigned)fp8_groups(rows));
   auto go = [&](auto type) {
-    hipLaunchKernelGGL((fp8_weight_kernel<decltype(type)>), grid, dim3(256), 0, (hipStream_t)stream,
+    hipLaunchKernelGGL((fp8_weight_kernel<decltype(type)>), grid, dim3(512), 0, (hipStream_t)stream,
                        weight->data, ld, rows, (int)cols, m);
     return check_launch(op);
   };
