@@ -149,6 +149,12 @@ def test_sizes_past_the_limits_are_refused():
     for op in PRODUCTS:
         st, text = run(op, a)
         assert st == TOO_LARGE, text
+    for k, groups in (((1 << 30) + 1, (1 << 23) + 1),):  # columns are counted in 31 bits
+        wide = torch.zeros(1, dtype=BF16).as_strided((0, k), (0, 1))
+        a = {"wide": wide, "rows": torch.zeros(1, dtype=U8).as_strided((0, k), (0, 1)),
+             "rows_scale": torch.zeros(1, dtype=U8).as_strided((0, groups), (0, 1))}
+        st, text = run(QUANTIZE, a)
+        assert st == TOO_LARGE and "2^30" in text, text
     k = (1 << 22) - 15
     a = {**call(1, 1, 1), "x": torch.zeros(1, k, dtype=U8), "x_scale": torch.zeros(1, 1 << 15, dtype=U8),
          "w": torch.zeros(1, k, dtype=U8), "w_scale": torch.zeros(1, 1 << 15, dtype=U8)}

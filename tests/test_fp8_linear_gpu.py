@@ -135,6 +135,20 @@ def test_quantize_views():
         assert torch.equal(code.reshape(want[0].shape) & 0x7F, want[0] & 0x7F)
 
 
+def test_expanded_rows():
+    """Rows that are the same memory are read like any."""
+    row = tokens(1, 300, BF16, seed=6, empty=False)
+    wide = row.to("gcu").expand(9, 300)
+    q, one = eff.fp8_quantize(wide), oracle.quantize(row)
+    assert torch.equal(q.codes.cpu(), one[0].expand(9, 300)) and torch.equal(q.scales.cpu(), one[1].expand(9, 3))
+    y, total = eff.rms_norm_fp8(wide, None, residual=wide)
+    assert torch.equal(total.cpu(), (2 * row).expand(9, 300))
+    x = eff.FP8Rows(q.codes[:1].expand(70, 300), q.scales[:1].expand(70, 3))
+    w = eff.fp8_quantize_weight(torch.randn(200, 300, generator=gen(1)).to("gcu"))
+    got = eff.fp8_linear(x, w).cpu()
+    assert torch.equal(got, got[:1].expand(70, 200))
+
+
 def test_quantize_empty():
     for shape in ((0, 128), (3, 0), (2, 0, 5)):
         got = eff.fp8_quantize(torch.empty(shape, dtype=BF16, device="gcu"))
@@ -257,6 +271,68 @@ def test_linear_is_exact_on_whole_numbers(m, n, k, ends):
     assert got.dtype == dtype and torch.equal(got.cpu(), out.float().to(dtype))
 
 
+# the largest sizes of each tile shape and cut of K that stay quick on the CPU, with and
+# without whole groups (what runs: 256 x 256, 256 x 128, 128 x 128, 64 x 128, then 64 x 64
+# whole, in two and in four)
+LARGE = [(4778, 2992, 1111), (1804, 7699, 640), (909, 8018, 1110), (1523, 5177, 256), (259, 6711, 1131),
+         (4991, 407, 1152), (2456, 3229, 1102), (265, 6681, 128), (777, 4096, 512), (2655, 68, 4231),
+         (70, 3238, 4608), (25, 64, 7072), (42, 65, 4608), (65, 66, 64), (128, 4096, 1024)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_linear_of_every_tile_shape(m, n, k):
+    x, w = whole_numbers(m, n, k, m + n + k)
+    res = torch.randint(-64, 65, (m, n), generator=gen(5)).to(BF16)
+    got = eff.fp8_linear(gcu(x), gcu(w, eff.FP8Weight), residual=res.to("gcu"))
+    assert torch.equal(got.cpu(), (exact_product(x, w) + res.float()).to(BF16))
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_linear_of_the_largest_and_smallest_scales(m):
+    """2^-127 and 2^127, alone and against each other, in every way of the product."""
+    n, k = 140, 300
+    (x, _), (w, _) = whole_numbers(m, n, k, 23)
+    base = exact_product((x, torch.full((m, 3), 127, dtype=U8)), (w, torch.full((2, 3), 127, dtype=U8))).double()
+    for a, b in ((0, 254), (254, 0), (0, 127), (254, 127), (1, 1), (127, 0)):
+        got = eff.fp8_linear(gcu((x, torch.full((m, 3), a, dtype=U8))),
+                             gcu((w, torch.full((2, 3), b, dtype=U8)), eff.FP8Weight)).cpu()
+        want = (base * 2.0 ** (a + b - 254)).float().to(BF16)
+        if a + b > 370:  # (a term of 2 x 2^127 is float32's infinity, and two of them a NaN)
+            assert bool(((got == want) | ~got.isfinite()).all())
+        elif a + b < 128:  # (results under float32's normal range may be 0)
+            assert bool(((got.double() - want.double()).abs() <= 2.0 ** -126).all())
+        else:
+            assert torch.equal(got, want), (a, b)
+
+
+def test_offsets_past_32_bits():
+    """Weights and activations of more than 4 GiB: the first and last rows count."""
+    k, rows = 4096, (1 << 20) + 4096 + 5
+    big = torch.zeros(rows, k, dtype=U8, device="gcu")
+    scale = torch.full((rows, 32), 127, dtype=U8, device="gcu")
+    few, _ = whole_numbers(7, 1, k, 29)
+    few = (few[0], torch.full((7, 32), 127, dtype=U8))
+    at = [0, 1, rows - 2, rows - 1]
+    lines = whole_numbers(4, 1, k, 31)[0][0]
+    for i, r in enumerate(at):
+        big[r].copy_(lines[i].to("gcu"))
+    want = exact_product(few, (lines, torch.full((1, 32), 127, dtype=U8)))
+    blocks = scale[: -(-rows // 128)]
+    for m in (7, 70):  # few rows, and tiles
+        x = gcu((few[0].repeat(10, 1)[:m], few[1].repeat(10, 1)[:m]))
+        got = eff.fp8_linear(x, eff.FP8Weight(big, blocks))
+        assert torch.equal(got[:7, at].cpu(), want.to(BF16)) and float(got[:, 4: rows - 4].cpu().float().abs().max()) == 0
+        del got
+    got = eff.fp8_linear(eff.FP8Rows(big, scale), gcu((few[0], few[1][:1]), eff.FP8Weight))
+    assert torch.equal(got[at].cpu(), want.t().to(BF16))
+    wide = torch.zeros(rows, k, dtype=BF16, device="gcu")
+    wide[rows - 1].fill_(3.0)
+    q = eff.fp8_quantize(wide)
+    assert oracle.numbers(q.codes[rows - 2:].cpu(), q.scales[rows - 2:].cpu()).tolist() == [[0.0] * k, [3.0] * k]
+    q, _ = eff.rms_norm_fp8(wide, None, 0.0)
+    check_codes((q.codes[rows - 1:], q.scales[rows - 1:]), torch.ones(1, k), norm_error(k))
+
+
 def rounding_of(x, w):
     """(sum, bound, deviation) of a product: 64 bits, what an output can be off by, and
     the root of the variance of that."""
@@ -372,6 +448,9 @@ def test_linear_without_columns():
     b = torch.arange(5.0).to(BF16).to("gcu")
     assert torch.equal(eff.fp8_linear(x, w, bias=b).cpu(), torch.arange(5.0).to(BF16).expand(3, 5))
     assert int((eff.fp8_linear_silu_mul(x, w, w).codes.cpu() & 0x7F).sum()) == 0
+    x = eff.FP8Rows(torch.empty(200, 0, dtype=U8, device="gcu"), torch.empty(200, 0, dtype=U8, device="gcu"))
+    assert torch.equal(eff.fp8_linear(x, w, bias=b).cpu(), torch.arange(5.0).to(BF16).expand(200, 5))
+    assert int((eff.fp8_linear_silu_mul(x, w, w).codes.cpu() & 0x7F).sum()) == 0
     none = eff.FP8Rows(torch.empty(0, 16, dtype=U8, device="gcu"), torch.empty(0, 1, dtype=U8, device="gcu"))
     w = eff.FP8Weight(torch.zeros(5, 16, dtype=U8, device="gcu"), torch.zeros(1, 1, dtype=U8, device="gcu"))
     assert eff.fp8_linear(none, w).shape == (0, 5) and eff.fp8_linear_silu_mul(none, w, w).codes.shape == (0, 5)
@@ -392,6 +471,10 @@ def small_gates(m, n, k, seed):
     return x, (wg[0], wg[1] - min(5, int(math.log2(k) / 2))), wu
 
 
+GATES_LARGE = [(669, 8246, 1185), (3236, 2016, 640), (4869, 404, 1153), (470, 8372, 64), (4800, 137, 4545),
+               (81, 2404, 2193), (25, 69, 2528), (147, 207, 1137), (65, 70, 912), (17, 65, 305), (33, 67, 272)]
+
+
 def check_gate(got, gate, up, gate_off=0.0, up_off=0.0):
     y = oracle.silu_mul(gate, up)
     # exp2's argument is rounded (|g| 2^-24 of the exponential) and two fast functions of about
@@ -401,7 +484,7 @@ def check_gate(got, gate, up, gate_off=0.0, up_off=0.0):
     check_codes(got, y, d + extra / y.abs().clamp(min=1e-300))
 
 
-@pytest.mark.parametrize("m,n,k", GATES)
+@pytest.mark.parametrize("m,n,k", GATES + GATES_LARGE)
 def test_gate_on_whole_numbers(m, n, k):
     x, wg, wu = small_gates(m, n, k, m + n + k)
     got = eff.fp8_linear_silu_mul(gcu(x), gcu(wg, eff.FP8Weight), gcu(wu, eff.FP8Weight))

@@ -27,8 +27,8 @@ mi_status_t fp8_check(const char* op, const char* name, const mi_fp8_t* t, bool 
     MI_CHECK_ARG(rows_apart(c) && rows_apart(s), "%s: rows of %s overlap", op, name);
     MI_RETURN_IF(fp8_check_apart(op, "codes", &c, "scales", &s));
   }
-  if (c.sizes[0] > 0x7fffffff || c.sizes[1] > 0x7fffff00)
-    MI_FAIL(MI_ERR_TOO_LARGE, "%s: %s has more than 2^31 rows or columns", op, name);
+  if (c.sizes[0] > 0x7fffffff || c.sizes[1] > (1 << 30))
+    MI_FAIL(MI_ERR_TOO_LARGE, "%s: %s has 2^31 rows or more, or more than 2^30 columns", op, name);
   *m = Fp8Mat{(uint8_t*)c.data, (uint8_t*)s.data, c.strides[0], s.strides[0]};
   return MI_OK;
 }
