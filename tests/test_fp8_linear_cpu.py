@@ -163,6 +163,17 @@ def test_sizes_past_the_limits_are_refused():
         assert st == TOO_LARGE, text
 
 
+def test_more_outputs_than_a_grid_holds_are_refused():
+    n = 1 << 28  # columns, 16 of them a block
+    w, scale = torch.zeros(1, 1, dtype=U8).expand(n, 1), torch.zeros(1, 1, dtype=U8).expand(n // 128, 1)
+    a = {**call(1, 1, 1), "w": w, "w_scale": scale, "up": w, "up_scale": scale, "bias": None, "add": None,
+         "x_scale": torch.zeros(1, 1, dtype=U8), "out": torch.empty(1, n, dtype=BF16),
+         "gated": torch.empty(1, n, dtype=U8), "gated_scale": torch.empty(1, n // 128, dtype=U8)}
+    for op in PRODUCTS:
+        st, text = run(op, a)
+        assert st == TOO_LARGE and "too many outputs" in text, text
+
+
 def test_empty_calls_do_nothing():
     for op in ORDER:
         for shape in ((0, 200, 300), (5, 0, 300)):

@@ -149,6 +149,21 @@ def test_expanded_rows():
     assert torch.equal(got, got[:1].expand(70, 200))
 
 
+@pytest.mark.parametrize("k", [8, 1032])
+def test_more_rows_than_a_grids_first_dimension(k):
+    """2^20 blocks of 4 rows (of one, above 1024 columns), and a few more."""
+    m = (1 << 22) + 7 if k == 8 else (1 << 20) + 7
+    x = (torch.arange(m, device="cuda")[:, None] % 251 + torch.arange(k, device="cuda")).to(BF16)
+    got = torch.zeros(m, k, dtype=U8, device="cuda"), torch.zeros(m, -(-k // 128), dtype=U8, device="cuda")
+    for call in (lambda o, x: _abi.fp8_quantize(o, x), lambda o, x: _abi.rms_norm_fp8(o, None, x, None, None, 1e-6)):
+        few = tuple(torch.zeros_like(t[:251]) for t in got)
+        call(got, x), call(few, x[:251])
+        for t, f in zip(got, few):
+            assert torch.equal(t[: m // 251 * 251].view(-1, *f.shape), f.expand(m // 251, *f.shape))
+            assert torch.equal(t[m // 251 * 251:], f[: m % 251])
+            t.zero_()
+
+
 def test_quantize_empty():
     for shape in ((0, 128), (3, 0), (2, 0, 5)):
         got = eff.fp8_quantize(torch.empty(shape, dtype=BF16, device="gcu"))

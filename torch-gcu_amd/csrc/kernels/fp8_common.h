@@ -21,6 +21,13 @@ struct Fp8Mat {
   int64_t ld, sld;  // row strides, in bytes
 };
 
+// Any number of blocks as a grid (a dimension holds fewer than 2^32 threads); the
+// kernel's block is fp8_block(), and those past the last end at once.
+inline dim3 fp8_grid(int64_t blocks) {
+  const int64_t x = blocks < (1 << 20) ? blocks : 1 << 20;
+  return dim3((unsigned)x, ceil_div_u(blocks, x));
+}
+
 inline int64_t fp8_groups(int64_t n) { return (n + kFp8Group - 1) / kFp8Group; }
 
 // Checks of the entry points (fp8_check.cpp); they read descriptors only.
@@ -41,6 +48,9 @@ mi_status_t fp8_quantize_f32(const float* y, int64_t ld, int64_t rows, int cols,
 namespace {
 
 typedef uint32_t f8_u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ int64_t fp8_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 constexpr uint32_t kFp8AbsMask = 0x7fffffffu, kFp8Inf = 0x7f800000u;
 
 // The scale byte of a group whose largest finite magnitude has these float bits:

@@ -79,6 +79,8 @@ struct F8Cfg {
       cmax((size_t)SCALES + 2 * SET, cmax((size_t)NW * TM * EP * 4, (size_t)BM * CP + (size_t)WN * BM * 4));
   static_assert(LDS_BYTES <= 160 * 1024 && NQA >= 1 && NQB >= 1 && FN % RB == 0 && NQL * FN == NQB * RB &&
                     (STAGES - 1) * LPW < 64, "shape");
+  // a set of scales is written while the one before it is still read
+  static_assert(KS >= STAGES, "sets");
 };
 
 template <class C, int EPI>

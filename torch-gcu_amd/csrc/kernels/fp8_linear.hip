@@ -79,6 +79,12 @@ mi_status_t launch_combine(const Fp8Gemm& q, bool gate, int S, hipStream_t s, co
   return check_launch(op);
 }
 
+// A grid's first dimension holds fewer than 2^32 threads.
+mi_status_t check_grid(int64_t blocks, int threads, const char* op) {
+  if (blocks * threads >= (int64_t)1 << 32) MI_FAIL(MI_ERR_TOO_LARGE, "%s: too many outputs", op);
+  return MI_OK;
+}
+
 template <class C, int EPI>
 mi_status_t launch_tiles(Fp8Gemm q, int S, hipStream_t s, const char* op) {
   static const bool attr = [] {
@@ -90,6 +96,7 @@ mi_status_t launch_tiles(Fp8Gemm q, int S, hipStream_t s, const char* op) {
   constexpr int BN = EPI == F8_GATE || EPI == F8_GATE_PART ? C::BN / 2 : C::BN;
   q.tiles_m = (q.M + C::BM - 1) / C::BM;
   q.tiles_n = (q.N + BN - 1) / BN;
+  MI_RETURN_IF(check_grid((int64_t)q.tiles_m * q.tiles_n, C::NT, op));
   hipLaunchKernelGGL((fp8_gemm_kernel<C, EPI>), dim3((unsigned)(q.tiles_m * q.tiles_n), (unsigned)S),
                      dim3(C::NT), C::LDS_BYTES, s, q);
   return check_launch(op);
@@ -120,6 +127,7 @@ mi_status_t launch_few(Fp8Gemm q, hipStream_t s, const char* op) {
   }();
   (void)attr;
   constexpr int COLS = 16 * (GATE ? C::RT / 2 : C::RT);
+  MI_RETURN_IF(check_grid(((int64_t)q.N + COLS - 1) / COLS, 64 * C::NW, op));
   Workspace ws;
   if (GATE) {
     q.ldp = ((int64_t)q.N + 3) / 4 * 4;

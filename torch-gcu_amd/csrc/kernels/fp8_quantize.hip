@@ -129,7 +129,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, f8_
 template <typename T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(RowsArgs a, int chunks) {
   typedef Eight<T> E;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = id / chunks;
+  const int64_t id = fp8_block() * 4 + (threadIdx.x >> 6), row = id / chunks;
   if (row >= a.rows) return;
   const int col = (int)(id - row * chunks) * 512 + (threadIdx.x & 63) * 8;
   const E v = E::load((const typename E::St*)a.x + row * a.x_ld, col, a.cols);
@@ -151,8 +151,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   constexpr int STEP = TPR * 8, N = VPL > 0 ? VPL : 1;
   __shared__ float red[4];
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-  if (TPR < 256 && row >= a.rows) return;
+  const int64_t row = fp8_block() * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= a.rows) return;
   const int cols = a.cols;
   const St* x = (const St*)a.x + row * a.x_ld;
   const St* res = KIND == NORM_RES ? (const St*)a.res + row * a.res_ld : nullptr;
@@ -291,9 +291,9 @@ __global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t 
 template <typename T>
 mi_status_t launch_quantize(const RowsArgs& a, hipStream_t s, const char* op) {
   const int64_t chunks = (a.cols + 511) / 512;
-  if ((a.rows * chunks + 3) / 4 > 0x7fffffff) MI_FAIL(MI_ERR_TOO_LARGE, "%s: too many rows", op);
-  hipLaunchKernelGGL((fp8_quantize_kernel<T>), dim3(ceil_div_u(a.rows * chunks, 4)), dim3(256), 0, s, a,
-                     (int)chunks);
+  const int64_t blocks = (a.rows * chunks + 3) / 4;
+  if (blocks > (int64_t)65535 << 20) MI_FAIL(MI_ERR_TOO_LARGE, "%s: too many elements", op);
+  hipLaunchKernelGGL((fp8_quantize_kernel<T>), fp8_grid(blocks), dim3(256), 0, s, a, (int)chunks);
   return check_launch(op);
 }
 
@@ -306,7 +306,7 @@ mi_status_t launch_norm(const RowsArgs& a, hipStream_t s, const char* op) {
   auto go = [&](auto tpr, auto vpl) {
     constexpr int TPR = decltype(tpr)::value;
     hipLaunchKernelGGL((fp8_rows_kernel<T, KIND, TPR, decltype(vpl)::value>),
-                       dim3(ceil_div_u(a.rows, 256 / TPR)), dim3(256), 0, s, a);
+                       fp8_grid((a.rows + 256 / TPR - 1) / (256 / TPR)), dim3(256), 0, s, a);
     return check_launch(op);
   };
   const std::integral_constant<int, 64> wave;
@@ -390,7 +390,8 @@ mi_status_t mi_fp8_quantize_weight(const mi_fp8_t* out, const mi_tensor_t* weigh
   MI_RETURN_IF(check_outputs_apart(op, out, "weight", weight));
   if (numel(*weight) == 0) return MI_OK;
   const int64_t rows = weight->sizes[0], cols = weight->sizes[1], ld = weight->strides[0];
-  if (fp8_groups(rows) > 65535) MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 65535 x 128 rows", op);
+  if (fp8_groups(rows) > 65535 || fp8_groups(cols) >= (1 << 23))
+    MI_FAIL(MI_ERR_TOO_LARGE, "%s: more than 65535 x 128 rows, or 2^30 - 127 columns", op);
   const dim3 grid((unsigned)fp8_groups(cols), (unsigned)fp8_groups(rows));
   auto go = [&](auto type) {
     hipLaunchKernelGGL((fp8_weight_kernel<decltype(type)>), grid, dim3(512), 0, (hipStream_t)stream,
