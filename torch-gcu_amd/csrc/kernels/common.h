@@ -362,10 +362,13 @@ __device__ __forceinline__ float silu_mul_f32(float a, float b) {
 // while one is in flight every wait for an LDS read it emits is lgkmcnt(0),
 // so a fragment read issued ahead of the MFMA before it is waited for
 // there.  Callers wait for their copies themselves (vmcnt) before the
-// barrier that publishes them.  The s_nop is the wait state an LDS DMA
-// needs after M0 is written.  The base must be wave-uniform; it is read
+// barrier that publishes them.  The base must be wave-uniform; it is read
 // from the first lane (free when it is already in scalar registers, which
-// the "s" operand needs).
+// the "s" operand needs).  It is copied by the scalar unit here: a vector
+// instruction's write of a scalar register (readfirstlane) may be read as an
+// address only 5 wait states later, which the compiler does not see to for
+// inline assembly, while the scalar unit waits by itself.  The copy is also
+// the wait state an LDS DMA needs after M0 is written.
 __device__ __forceinline__ void lds_copy16(const void* base, uint32_t off, void* lds) {
   const uint32_t m0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
   // (readfirstlane returns int: each word goes through uint32_t so that the
@@ -374,7 +377,8 @@ __device__ __forceinline__ void lds_copy16(const void* base, uint32_t off, void*
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
   const uint64_t sb = ((uint64_t)hi << 32) | lo;
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(sb), "{m0}"(m0)
+  uint64_t at;
+  asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(at) : "v"(off), "s"(sb), "{m0}"(m0)
                : "memory");
 }
 

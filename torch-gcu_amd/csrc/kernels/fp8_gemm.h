@@ -44,7 +44,9 @@ __device__ __forceinline__ void lds_copy_byte(const uint8_t* base, uint32_t off,
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
   const uint64_t sb = ((uint64_t)hi << 32) | lo;
-  asm volatile("s_nop 0\n\tglobal_load_lds_ubyte %0, %1" : : "v"(off), "s"(sb), "{m0}"(m0) : "memory");
+  uint64_t at;  // (as in lds_copy16)
+  asm volatile("s_mov_b64 %0, %2\n\tglobal_load_lds_ubyte %1, %0" : "=&s"(at) : "v"(off), "s"(sb), "{m0}"(m0)
+               : "memory");
 }
 
 // silu(g) u and the largest finite magnitude's bits so far
@@ -403,66 +405,97 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     return;
   }
   // out = acc (+ bias) (+ residual), rounded once: HC columns of the wave's tile at a
-  // time through LDS, for whole row segments
-  constexpr int HC = C::HC, EP = C::EP, LPR = HC / 8, RPI = 64 / LPR;
+  // time through LDS, for whole row segments.  Where all of the tile's columns exist and
+  // rows are aligned, no load stands behind a condition: a pass's residual is asked for at
+  // once, before its products go to LDS (rows past the end read the last one), and not a
+  // row at a time behind a branch.
+  constexpr int HC = C::HC, EP = C::EP, LPR = HC / 8, RPI = 64 / LPR, NI = TM / RPI, NB = NI < 4 ? NI : 4;
   float* es = (float*)smem + wave * TM * EP;
   typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
   uint16_t* out = (uint16_t*)p.out;
   const bool vec_out = p.ldc % 8 == 0 && (uintptr_t)out % 16 == 0;
   const bool vec_res = p.ldr % 8 == 0 && (uintptr_t)p.res % 16 == 0;
-  auto wide = [&](uint16_t v) __attribute__((always_inline)) { return p.f16 ? f16_to_f32(v) : bf16_to_f32(v); };
+  const bool whole = vec_out && (p.res == nullptr || vec_res) && n0 + BN <= N;
+  auto finish = [&](auto half_c) __attribute__((always_inline)) {
+    constexpr bool HALF = decltype(half_c)::value;
+    auto wide = [](uint16_t v) __attribute__((always_inline)) { return HALF ? f16_to_f32(v) : bf16_to_f32(v); };
+    auto narrow = [](float y) __attribute__((always_inline)) { return HALF ? f32_to_f16(y) : f32_to_bf16(y); };
 #pragma unroll
-  for (int h = 0; h < TN / HC; ++h) {
-    __builtin_amdgcn_wave_barrier();
+    for (int h = 0; h < TN / HC; ++h) {
+      const int c = (lane % LPR) * 8, n = n0 + wn * TN + h * HC + c;
+      u16x8_t res[NI];
+      if (whole && p.res != nullptr) {
 #pragma unroll
-    for (int j = 0; j < HC / 16; ++j)
+        for (int it = 0; it < NI; ++it)
+          res[it] = *(const u16x8_t*)(p.res + (int64_t)min(mw + it * RPI + lane / LPR, M - 1) * p.ldr + n);
+      } else {
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-        *(f32x4_t*)(es + (16 * i + row) * EP + 16 * j + 4 * (lane >> 4)) = acc[h * (HC / 16) + j][i];
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int c = (lane % LPR) * 8, n = n0 + wn * TN + h * HC + c;
-    float bias[8] = {};
-    if (p.bias != nullptr)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int at = min(n + e, N - 1);
-        bias[e] = p.bias_dtype == MI_F32 ? ((const float*)p.bias)[at] : wide(((const uint16_t*)p.bias)[at]);
+        for (int it = 0; it < NI; ++it) res[it] = (u16x8_t)(uint16_t)0x8000;  // y + -0 is y
       }
-#pragma unroll 4
-    for (int it = 0; it < TM / RPI; ++it) {
-      const int r = it * RPI + lane / LPR, m = mw + r;
-      if (m >= M || n >= N) continue;
-      const f32x4_t lo = *(const f32x4_t*)(es + r * EP + c), hi = *(const f32x4_t*)(es + r * EP + c + 4);
-      float y[8];
+      float bias[8] = {};
+      if (p.bias != nullptr)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (e < 4 ? lo[e & 3] : hi[e & 3]) + bias[e];
-      if (p.res != nullptr) {
-        const uint16_t* src = p.res + (int64_t)m * p.ldr + n;
-        if (vec_res && n + 7 < N) {
-          const u16x8_t v = *(const u16x8_t*)src;
+        for (int e = 0; e < 8; ++e) {
+          const int at = min(n + e, N - 1);
+          bias[e] = p.bias_dtype == MI_F32 ? ((const float*)p.bias)[at] : wide(((const uint16_t*)p.bias)[at]);
+        }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] += wide(v[e]);
+      for (int j = 0; j < HC / 16; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+          *(f32x4_t*)(es + (16 * i + row) * EP + 16 * j + 4 * (lane >> 4)) = acc[h * (HC / 16) + j][i];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      if (whole) {
+#pragma unroll
+        for (int b = 0; b < NI; b += NB) {
+          f32x4_t y[NB][2];
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              y[i][u] = *(const f32x4_t*)(es + ((b + i) * RPI + lane / LPR) * EP + c + 4 * u);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            u16x8_t v;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = narrow(y[i][e >> 2][e & 3] + bias[e] + wide(res[b + i][e]));
+            const int m = mw + (b + i) * RPI + lane / LPR;
+            if (m < M) *(u16x8_t*)(out + (int64_t)m * p.ldc + n) = v;
+          }
+        }
+        continue;
+      }
+#pragma unroll 1
+      for (int it = 0; it < NI; ++it) {
+        const int r = it * RPI + lane / LPR, m = mw + r;
+        if (m >= M || n >= N) continue;
+        const uint16_t* src = p.res == nullptr ? nullptr : p.res + (int64_t)m * p.ldr + n;
+        uint16_t* dst = out + (int64_t)m * p.ldc + n;
+        const bool all = n + 7 < N;
+        u16x8_t v = (u16x8_t)(uint16_t)0x8000;
+        if (src != nullptr && vec_res && all) {
+          v = *(const u16x8_t*)src;
+        } else if (src != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = src[min(e, N - 1 - n)];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = narrow(es[r * EP + c + e] + bias[e] + wide(v[e]));
+        if (vec_out && all) {
+          *(u16x8_t*)dst = v;
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (n + e < N) y[e] += wide(src[e]);
+            if (n + e < N) dst[e] = v[e];
         }
       }
-      u16x8_t v;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = p.f16 ? f32_to_f16(y[e]) : f32_to_bf16(y[e]);
-      uint16_t* dst = out + (int64_t)m * p.ldc + n;
-      if (vec_out && n + 7 < N) {
-        *(u16x8_t*)dst = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < N) dst[e] = v[e];
-      }
     }
-  }
+  };
+  if (p.f16) finish(std::true_type{});
+  else finish(std::false_type{});
 }
 
 }  // namespace

@@ -102,16 +102,21 @@ mi_status_t launch_tiles(Fp8Gemm q, int S, hipStream_t s, const char* op) {
   return check_launch(op);
 }
 
+template <class C, bool GATE>
+mi_status_t launch(const Fp8Gemm& q, hipStream_t s, const char* op) {
+  return launch_tiles<C, GATE ? F8_GATE : F8_OUT>(q, 1, s, op);
+}
+
 // One launch, or S slices of K and their sum.
 template <class C, bool GATE>
-mi_status_t launch(Fp8Gemm q, int S, hipStream_t s, const char* op) {
+mi_status_t launch_slices(Fp8Gemm q, int S, hipStream_t s, const char* op) {
   Workspace ws;
   q.ldp = ((int64_t)q.N + 3) / 4 * 4;
   if (S > 1 && ws.alloc((size_t)(GATE ? 2 : 1) * S * q.M * q.ldp * sizeof(float), s) != MI_OK) {
     clear_error();  // the whole K in one block needs no workspace
     S = 1;
   }
-  if (S <= 1) return launch_tiles<C, GATE ? F8_GATE : F8_OUT>(q, 1, s, op);
+  if (S <= 1) return launch<C, GATE>(q, s, op);
   q.part = (float*)ws.get();
   MI_RETURN_IF((launch_tiles<C, GATE ? F8_GATE_PART : F8_PART>(q, S, s, op)));
   return launch_combine(q, GATE, S, s, op);
@@ -219,11 +224,11 @@ mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
     if (fits<R8Cfg<8, 1, 4, 2>>(q)) return launch_few<R8Cfg<8, 1, 4, 2>, false>(q, s, op);
   }
   switch (c.shape) {
-    case 0: return launch<F256, false>(q, 1, s, op);
-    case 1: return launch<F256x128, false>(q, 1, s, op);
-    case 2: return launch<F128, false>(q, 1, s, op);
-    case 3: return launch<F64x128, false>(q, 1, s, op);
-    default: return launch<F64, false>(q, c.slices, s, op);
+    case 0: return launch<F256, false>(q, s, op);
+    case 1: return launch<F256x128, false>(q, s, op);
+    case 2: return launch<F128, false>(q, s, op);
+    case 3: return launch<F64x128, false>(q, s, op);
+    default: return launch_slices<F64, false>(q, c.slices, s, op);
   }
 }
 
@@ -238,9 +243,9 @@ mi_status_t run_gate(const Fp8Gemm& q, hipStream_t s, const char* op) {
     if (fits<R8Cfg<8, 2, 4, 2>>(q)) return launch_few<R8Cfg<8, 2, 4, 2>, true>(q, s, op);
   }
   switch (c.shape) {
-    case 0: return launch<F256, true>(q, 1, s, op);
-    case 1: return launch<G128, true>(q, c.slices, s, op);
-    default: return launch<G64, true>(q, c.slices, s, op);
+    case 0: return launch<F256, true>(q, s, op);
+    case 1: return launch_slices<G128, true>(q, c.slices, s, op);
+    default: return launch_slices<G64, true>(q, c.slices, s, op);
   }
 }
 
