@@ -51,8 +51,6 @@ typedef uint32_t f8_u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ int64_t fp8_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
-constexpr uint32_t kFp8AbsMask = 0x7fffffffu, kFp8Inf = 0x7f800000u;
-
 // The scale byte of a group whose largest finite magnitude has these float bits:
 // the smallest power of two s >= 2^-110 with amax <= 448 s.  448 is 1.75 x 2^8, so the
 // exponent is amax's less 8, and one more where its mantissa is over 1.75.  (2^-110
@@ -65,24 +63,19 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax) {
 __device__ __forceinline__ float fp8_inverse(uint32_t byte) {
   return __uint_as_float((254u - byte) << 23);
 }
-// The bits of |x| where x is finite, else 0: the largest of them is the largest
-// finite magnitude (floats that are not negative order as their bits do).
-__device__ __forceinline__ uint32_t fp8_finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & kFp8AbsMask;
-  return b < kFp8Inf ? b : 0u;
-}
-// Four values times a power of two as codes, to nearest, ties to even; what is not
-// finite becomes NaN (e4m3 has no infinity).  The caller's scale keeps the finite ones
-// within 448.
+// x, or NaN where it is infinite (0 inf is NaN): e4m3 has no infinity.
+__device__ __forceinline__ float fp8_no_inf(float x) { return __builtin_fmaf(x, 0.f, x); }
+// The larger of m and |x|, of m and a NaN m.
+__device__ __forceinline__ float fp8_larger(float m, float x) { return __builtin_fmaxf(m, __builtin_fabsf(x)); }
+// Four values times a power of two as codes, to nearest, ties to even; NaN stays NaN.  The
+// caller's scale keeps the others within 448.
 __device__ __forceinline__ uint32_t fp8_codes4(float a, float b, float c, float d, float inv) {
-  auto f = [&](float x) __attribute__((always_inline)) {
-    return (__float_as_uint(x) & kFp8Inf) == kFp8Inf ? NAN : x * inv;
-  };
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(f(a), f(b), 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f(c), f(d), r, true);
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, r, true);
 }
 
-// The largest over each row of 16 lanes, in all of them.
+// The largest over each row of 16 lanes, in all of them (of floats that are not negative:
+// they order as their bits do).
 __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
   auto step = [&](uint32_t o) __attribute__((always_inline)) { v = v > o ? v : o; };
   step((uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));

@@ -49,10 +49,10 @@ __device__ __forceinline__ void lds_copy_byte(const uint8_t* base, uint32_t off,
                : "memory");
 }
 
-// silu(g) u and the largest finite magnitude's bits so far
-__device__ __forceinline__ float gate_of(float g, float u, uint32_t* most) {
-  const float y = silu_mul_f32(g, u);
-  *most = max(*most, fp8_finite_bits(y));
+// silu(g) u, NaN where it is not finite, and the largest magnitude so far
+__device__ __forceinline__ float gate_of(float g, float u, float* most) {
+  const float y = fp8_no_inf(silu_mul_f32(g, u));
+  *most = fp8_larger(*most, y);
   return y;
 }
 
@@ -358,17 +358,23 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   __syncthreads();  // every wave is done with the stages
   if constexpr (EPI == F8_GATE) {
     uint32_t* most = (uint32_t*)(smem + BM * C::CP);  // [WN][BM]
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      uint32_t mx = 0;
+    if (n0 + BN / 2 > N) {  // columns past the end take no part in a maximum
 #pragma unroll
       for (int j = 0; j < FN / 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = n0 + wn * (TN / 2) + 16 * j + 4 * (lane >> 4) + e;
-          const float g = acc[j][i][e], u = n < N ? acc[j + FN / 2][i][e] : 0.f;
-          acc[j][i][e] = gate_of(n < N ? g : 0.f, u, &mx);
-        }
+        for (int e = 0; e < 4; ++e)
+          if (n0 + wn * (TN / 2) + 16 * j + 4 * (lane >> 4) + e >= N)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) acc[j][i][e] = acc[j + FN / 2][i][e] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      float mine = 0.f;
+#pragma unroll
+      for (int j = 0; j < FN / 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][i][e] = gate_of(acc[j][i][e], acc[j + FN / 2][i][e], &mine);
+      uint32_t mx = __float_as_uint(mine);
       mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, 64));
       mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, 64));
       if (lane < 16) most[wn * BM + wm * TM + 16 * i + row] = mx;
@@ -406,15 +412,18 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   }
   // out = acc (+ bias) (+ residual), rounded once: HC columns of the wave's tile at a
   // time through LDS, for whole row segments.  Where all of the tile's columns exist and
-  // rows are aligned, no load stands behind a condition: a pass's residual is asked for at
-  // once, before its products go to LDS (rows past the end read the last one), and not a
-  // row at a time behind a branch.
+  // rows are aligned, nothing stands behind a condition: a pass's residual is asked for at
+  // once, before its products go to LDS, and rows past the end are the wave's last one
+  // again, read before it is first written.  (A tile's epilogue of 14 us with a residual
+  // so became 8; with a condition at each store 9.)
   constexpr int HC = C::HC, EP = C::EP, LPR = HC / 8, RPI = 64 / LPR, NI = TM / RPI, NB = NI < 4 ? NI : 4;
   float* es = (float*)smem + wave * TM * EP;
   typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
   uint16_t* out = (uint16_t*)p.out;
   const bool vec_out = p.ldc % 8 == 0 && (uintptr_t)out % 16 == 0;
   const bool vec_res = p.ldr % 8 == 0 && (uintptr_t)p.res % 16 == 0;
+  if (mw >= M) return;
+  const int last = M - 1 - mw;
   const bool whole = vec_out && (p.res == nullptr || vec_res) && n0 + BN <= N;
   auto finish = [&](auto half_c) __attribute__((always_inline)) {
     constexpr bool HALF = decltype(half_c)::value;
@@ -427,7 +436,7 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
       if (whole && p.res != nullptr) {
 #pragma unroll
         for (int it = 0; it < NI; ++it)
-          res[it] = *(const u16x8_t*)(p.res + (int64_t)min(mw + it * RPI + lane / LPR, M - 1) * p.ldr + n);
+          res[it] = *(const u16x8_t*)(p.res + (int64_t)(mw + min(it * RPI + lane / LPR, last)) * p.ldr + n);
       } else {
 #pragma unroll
         for (int it = 0; it < NI; ++it) res[it] = (u16x8_t)(uint16_t)0x8000;  // y + -0 is y
@@ -456,14 +465,13 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
           for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-              y[i][u] = *(const f32x4_t*)(es + ((b + i) * RPI + lane / LPR) * EP + c + 4 * u);
+              y[i][u] = *(const f32x4_t*)(es + min((b + i) * RPI + lane / LPR, last) * EP + c + 4 * u);
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             u16x8_t v;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = narrow(y[i][e >> 2][e & 3] + bias[e] + wide(res[b + i][e]));
-            const int m = mw + (b + i) * RPI + lane / LPR;
-            if (m < M) *(u16x8_t*)(out + (int64_t)m * p.ldc + n) = v;
+            *(u16x8_t*)(out + (int64_t)(mw + min((b + i) * RPI + lane / LPR, last)) * p.ldc + n) = v;
           }
         }
         continue;

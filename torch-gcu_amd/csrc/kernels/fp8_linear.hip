@@ -42,8 +42,7 @@ __global__ __launch_bounds__(256) void fp8_gate_combine_kernel(Fp8Gemm p, int S)
   const int64_t m = id / groups;
   const int group = (int)(id - m * groups), n = group * kFp8Group + 4 * (threadIdx.x & 31);
   const bool live = m < p.M;
-  float y[4] = {};
-  uint32_t most = 0;
+  float y[4] = {}, mine = 0.f;
   if (live && n < p.N) {
     const int64_t slice = p.M * p.ldp;
     const float* src = p.part + m * p.ldp + n;
@@ -55,9 +54,9 @@ __global__ __launch_bounds__(256) void fp8_gate_combine_kernel(Fp8Gemm p, int S)
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e < p.N) y[e] = gate_of(g[e], u[e], &most);
+      if (n + e < p.N) y[e] = gate_of(g[e], u[e], &mine);
   }
-  most = row16_max(most);
+  uint32_t most = row16_max(__float_as_uint(mine));
   most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
   if (!live) return;
   const uint32_t byte = fp8_scale_byte(most);

@@ -82,36 +82,18 @@ struct Eight {
   }
 };
 
-// The scale byte of a group that `lanes` lanes hold 8 elements of each (most: the
-// largest |bits| over the group, whatever it holds), and the codes of this lane's.
-// Groups that hold an infinity or a NaN look at their finite elements again.
-template <typename Max>
-__device__ __forceinline__ f8_u32x2 codes_of(const float* y, uint32_t most, Max group_max,
-                                             uint32_t* byte) {
-  if (most >= kFp8Inf) {
-    uint32_t m = 0;
+// The codes of a lane's 8 values of a group that a row of 16 lanes holds, and the group's
+// scale byte.
+__device__ __forceinline__ f8_u32x2 codes_of(float* y, uint32_t* byte) {
+  float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, fp8_finite_bits(y[i]));
-    *byte = fp8_scale_byte(group_max(m));
-    const float inv = fp8_inverse(*byte);
-    return f8_u32x2{fp8_codes4(y[0], y[1], y[2], y[3], inv), fp8_codes4(y[4], y[5], y[6], y[7], inv)};
+  for (int i = 0; i < 8; ++i) {
+    y[i] = fp8_no_inf(y[i]);
+    most = fp8_larger(most, y[i]);
   }
-  *byte = fp8_scale_byte(most);
+  *byte = fp8_scale_byte(row16_max(__float_as_uint(most)));
   const float inv = fp8_inverse(*byte);
-  f8_u32x2 r;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h] * inv, y[4 * h + 1] * inv, 0, false);
-    r[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2] * inv, y[4 * h + 3] * inv, c, true);
-  }
-  return r;
-}
-
-__device__ __forceinline__ uint32_t largest_bits(const float* y) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(y[i]) & kFp8AbsMask);
-  return m;
+  return f8_u32x2{fp8_codes4(y[0], y[1], y[2], y[3], inv), fp8_codes4(y[4], y[5], y[6], y[7], inv)};
 }
 
 __device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, f8_u32x2 c) {
@@ -137,7 +119,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(RowsArgs a, int chunk
 #pragma unroll
   for (int j = 0; j < 8; ++j) y[j] = v.get(j);
   uint32_t byte;
-  const f8_u32x2 c = codes_of(y, row16_max(largest_bits(y)), row16_max, &byte);
+  const f8_u32x2 c = codes_of(y, &byte);
   store_codes(a.out.codes + row * a.out.ld, col, a.cols, c);
   if ((threadIdx.x & 15) == 0 && col < a.cols) a.out.scales[row * a.out.sld + col / kFp8Group] = (uint8_t)byte;
 }
@@ -210,7 +192,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
       for (int j = 0; j < 8; ++j) y[j] = col + j < cols ? y[j] : 0.f;
     }
     uint32_t byte;
-    const f8_u32x2 c = codes_of(y, row16_max(largest_bits(y)), row16_max, &byte);
+    const f8_u32x2 c = codes_of(y, &byte);
     store_codes(codes, col, cols, c);
     if ((t & 15) == 0 && col < cols) scales[col / kFp8Group] = (uint8_t)byte;
   };
@@ -231,7 +213,7 @@ __global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t 
   typedef Eight<T> E;
   typedef typename E::St St;
   constexpr int R = 4, NW = 8;
-  __shared__ uint32_t red[2][NW];
+  __shared__ uint32_t red[NW];
   const int col = blockIdx.x * kFp8Group + (threadIdx.x & 15) * 8;
   const int64_t row0 = (int64_t)blockIdx.y * kFp8Group + (threadIdx.x >> 4);
   // (rows past the end read the last one again, which is in the block)
@@ -249,37 +231,28 @@ __global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t 
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = E::load(p[i], col, cols);
   }
-  auto block_max = [&](uint32_t m, int turn) __attribute__((always_inline)) {
-    m = row16_max(m);
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-    if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = red[turn][0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) m = max(m, red[turn][i]);
-    return m;
-  };
-  uint32_t most = 0;
+  float y[R][8], mine = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[i].get(j)) & kFp8AbsMask);
-  most = block_max(most, 0);
-  if (most >= kFp8Inf) {  // the same for the whole block
-    most = 0;
+    for (int j = 0; j < 8; ++j) {
+      y[i][j] = fp8_no_inf(v[i].get(j));
+      mine = fp8_larger(mine, y[i][j]);
+    }
+  uint32_t most = row16_max(__float_as_uint(mine));
+  most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+  most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = red[0];
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, fp8_finite_bits(v[i].get(j)));
-    most = block_max(most, 1);
-  }
+  for (int i = 1; i < NW; ++i) most = max(most, red[i]);
   const uint32_t byte = fp8_scale_byte(most);
   const float inv = fp8_inverse(byte);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const f8_u32x2 c = {fp8_codes4(v[i].get(0), v[i].get(1), v[i].get(2), v[i].get(3), inv),
-                        fp8_codes4(v[i].get(4), v[i].get(5), v[i].get(6), v[i].get(7), inv)};
+    const f8_u32x2 c = {fp8_codes4(y[i][0], y[i][1], y[i][2], y[i][3], inv),
+                        fp8_codes4(y[i][4], y[i][5], y[i][6], y[i][7], inv)};
     if (row0 + 32 * i < rows) store_codes(out.codes + (row0 + 32 * i) * out.ld, col, cols, c);
   }
   if (threadIdx.x == 0) out.scales[blockIdx.y * out.sld + blockIdx.x] = (uint8_t)byte;
