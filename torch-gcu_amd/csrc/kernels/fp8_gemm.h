@@ -69,6 +69,8 @@ struct F8Cfg {
   // first RB fragments, then the others'
   static constexpr int NQA = BM / 8 / NW, NQB = BN / 8 / NW, NQL = NQB * RB / FN;
   static constexpr int LPW = NQA + NQB;
+  // one wave a SIMD, whose registers hold the next step's activations too
+  static constexpr bool PAIRS = TM * TN > 64 * 128;
   static constexpr int TA = BM * 128, TB = BN * 128, STAGE = TA + TB;
   // scales of KS K steps at a time, a word each, two of such sets in turn: 64 / KS rows a
   // wave copy, then the weight's blocks (KS 8, or 4 where the LDS has no room for those)
@@ -81,16 +83,18 @@ struct F8Cfg {
       cmax((size_t)SCALES + 2 * SET, cmax((size_t)NW * TM * EP * 4, (size_t)BM * CP + (size_t)WN * BM * 4));
   static_assert(LDS_BYTES <= 160 * 1024 && NQA >= 1 && NQB >= 1 && FN % RB == 0 && NQL * FN == NQB * RB &&
                     (STAGES - 1) * LPW < 64, "shape");
+  static_assert(!PAIRS || (FM == 8 && FN == 8 && NQA == 8 && NQB == 8 && STAGES == 2), "the order of its step");
   // a set of scales is written while the one before it is still read
   static_assert(KS >= STAGES, "sets");
 };
 
 template <class C, int EPI>
-__global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
+__global__ __launch_bounds__(C::NT, C::PAIRS ? 1 : 2) void fp8_gemm_kernel(Fp8Gemm p) {
   constexpr int WN = C::WN, TM = C::TM, TN = C::TN, BM = C::BM, BN = C::BN, FM = C::FM, FN = C::FN;
   constexpr int RB = C::RB, NQA = C::NQA, NQB = C::NQB, NQL = C::NQL, LPW = C::LPW, STAGES = C::STAGES;
   constexpr int KS = C::KS, NQS = C::NQS, SET = C::SET, SC = BM * KS / 64;
   constexpr int TA = C::TA, STAGE = C::STAGE, GROUP_M = 8;
+  constexpr bool PAIRS = C::PAIRS;
   constexpr bool GATE = EPI == F8_GATE || EPI == F8_GATE_PART;
   constexpr bool SPLIT = EPI == F8_PART || EPI == F8_GATE_PART;
   static_assert(EPI != F8_GATE || BN == 256, "a block holds whole groups of a gate's output");
@@ -131,6 +135,7 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   uint32_t ao[NQA], bo[NQB];
   // the 8 rows of the B tile that copy q of the wave takes (q < NQL: of first fragments)
   auto b_copy = [&](int q) __attribute__((always_inline)) {
+    if (PAIRS) return wave * NQB + q;
     const bool lo = q < NQL;
     const int i = lo ? wave * NQL + q : wave * (NQB - NQL) + q - NQL, per = 2 * (lo ? RB : FN - RB);
     return i / per * (TN / 8) + (lo ? 0 : 2 * RB) + i % per;
@@ -182,16 +187,16 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
       lds_copy16((b_up(c * 8) ? B[1] : B[0]) + k, bo[q - NQA], s + TA + c * 1024);
     }
   };
-  auto issue = [&](int st, int kt) __attribute__((always_inline)) {
+  auto issue = [&](int st, int kt, int copies) __attribute__((always_inline)) {
     if (kt == 0 || (k_first + kt) % KS == 0) issue_scales((k_first + kt) / KS);
 #pragma unroll
-    for (int q = 0; q < LPW; ++q) issue_one(st, kt, q);
+    for (int q = 0; q < copies; ++q) issue_one(st, kt, q);
   };
-  // fragments: lane l reads row l % 16, chunks l / 16 and 4 + l / 16
+  // fragments: lane l reads row l % 16, chunks l / 16 (half 0) and 4 + l / 16
   const int row = lane & 15;
-  const int ro0 = row * 128 + 16 * dl_swz(row, lane >> 4), ro1 = row * 128 + 16 * dl_swz(row, 4 + (lane >> 4));
-  auto fragment = [&](const char* t) __attribute__((always_inline)) {
-    const u32x4_t lo = *(const u32x4_t*)(t + ro0), hi = *(const u32x4_t*)(t + ro1);
+  const int ro[2] = {row * 128 + 16 * dl_swz(row, lane >> 4), row * 128 + 16 * dl_swz(row, 4 + (lane >> 4))};
+  auto whole_of = [](const u32x4_t* v) __attribute__((always_inline)) {
+    const u32x4_t lo = v[0], hi = v[1];
     return i32x8_t{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
   };
   // acc[j][i]: outputs m = 16 i + l % 16, n = 16 j + 4 (l / 16) + 0 .. 3 of the wave's
@@ -200,13 +205,13 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
   for (int j = 0; j < FN; ++j)
 #pragma unroll
     for (int i = 0; i < FM; ++i) acc[j][i] = f32x4_t{};
-  i32x8_t af[FM], bf[RB];
+  u32x4_t af[PAIRS ? 2 : 1][FM][2], bf[RB][2];
   int sa[FM], sb[2], sa_next[FM], sb_next[2];
-  auto read_a = [&](int st, int i) __attribute__((always_inline)) {
-    af[i] = fragment(smem + st * STAGE + (wm * TM + 16 * i) * 128);
+  auto read_a = [&](int set, int st, int i, int h) __attribute__((always_inline)) {
+    af[set][i][h] = *(const u32x4_t*)(smem + st * STAGE + (wm * TM + 16 * i) * 128 + ro[h]);
   };
-  auto read_b = [&](int st, int j) __attribute__((always_inline)) {
-    bf[j % RB] = fragment(smem + st * STAGE + TA + (wn * TN + 16 * j) * 128);
+  auto read_b = [&](int st, int j, int h) __attribute__((always_inline)) {
+    bf[j % RB][h] = *(const u32x4_t*)(smem + st * STAGE + TA + (wn * TN + 16 * j) * 128 + ro[h]);
   };
   auto read_scales = [&](int kt) __attribute__((always_inline)) {
     const int k = k_first + kt;
@@ -222,15 +227,16 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     sb[0] = sb_next[0];
     if constexpr (GATE) sb[1] = sb_next[1];
   };
-  auto mfma_one = [&](int j, int i) __attribute__((always_inline)) {
-    acc[j][i] = mma_fp8(bf[j % RB], af[i], acc[j][i], sb[GATE && j >= FN / 2 ? 1 : 0], sa[i]);
+  auto mfma_one = [&](int set, int j, int i) __attribute__((always_inline)) {
+    acc[j][i] =
+        mma_fp8(whole_of(bf[j % RB]), whole_of(af[set][i]), acc[j][i], sb[GATE && j >= FN / 2 ? 1 : 0], sa[i]);
   };
   auto first_reads = [&](int st) __attribute__((always_inline)) {
     read_scales(0);
 #pragma unroll
-    for (int j = 0; j < RB - 1; ++j) read_b(st, j);
+    for (int j = 0; j < RB - 1; ++j) read_b(st, j, 0), read_b(st, j, 1);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) read_a(st, i);
+    for (int i = 0; i < FM; ++i) read_a(0, st, i, 0), read_a(0, st, i, 1);
     take_scales();
   };
   // One K step over stage st, a row of MFMAs (one weight fragment) at a time.  The weight
@@ -261,12 +267,14 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
         __syncthreads();
         if (j == JB) read_scales(kt + 1);
       }
-      if (j + RB - 1 < FN) read_b(st, j + RB - 1);
-      else if (NEXT) read_b(nst, j + RB - 1 - FN);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        mfma_one(j, i);
-        if (j == FN - 1 && NEXT) read_a(nst, i);
+        if (i == 0 || i == FM / 2) {
+          if (j + RB - 1 < FN) read_b(st, j + RB - 1, i > 0);
+          else if (NEXT) read_b(nst, j + RB - 1 - FN, i > 0);
+        }
+        mfma_one(0, j, i);
+        if (j == FN - 1 && NEXT) read_a(0, nst, i, 0), read_a(0, nst, i, 1);
         if (ISSUE && j >= 1 && (j < JB || JB == 1))
 #pragma unroll
           for (int u = 0; u < PLO; ++u) {
@@ -285,29 +293,76 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     if (NEXT) take_scales();
   };
 
+  // One K step of PAIRS, whose SET-th fragments hold its activations: 64 products, and
+  // between them, one at most, the halves of fragments and the copies that later steps
+  // need.  (Two reads at a time cost 6 % of the cycles: one wave issues them all, and waits
+  // where LDS is behind.)  The next step's activations are read in rows 1 to 4.  At row 5 a
+  // barrier lets the stage's weight refill, and what holds the next step's activations in
+  // the step after: 6 of the weight's copies come at once, the other 2 and those of the
+  // activations in the next step.  So each copy has half a step or more until the barrier
+  // that waits for it.
+  auto pair_step = [&](auto set_c, int st, int kt, auto issue_c, auto next_c) __attribute__((always_inline)) {
+    constexpr int SET_ = decltype(set_c)::value;
+    constexpr bool ISSUE = decltype(issue_c)::value, NEXT = decltype(next_c)::value;
+    const int nst = 1 - st;
+    if (ISSUE && (kt + 2) % KS == 0) issue_scales((kt + 2) / KS);
+#pragma unroll
+    for (int n = 0; n < FN * FM; ++n) {
+      const int j = n / FM, i = n % FM;
+      if (NEXT && (n == FM || n == 5 * FM)) {
+        if (ISSUE) wait_vmcnt<8>();  // behind row 1's are the weight's 8, behind row 5's the activations'
+        else wait_vmcnt<0>();
+        __syncthreads();
+        if (n > FM) read_scales(kt + 1);
+      }
+      if (i % 4 == 0) {
+        if (j + RB - 1 < FN) read_b(st, j + RB - 1, i / 4);
+        else if (NEXT) read_b(nst, j + RB - 1 - FN, i / 4);
+      }
+      if (NEXT && j >= 1 && j < 5 && n % 2 == 1) read_a(1 - SET_, nst, n / 4 - 2, n / 2 % 2);
+      mfma_one(SET_, j, i);
+      if (n % 4 == 2) {
+        if (n < FM && NEXT) issue_one(nst, kt + 1, NQA + 6 + n / 4);
+        if (j >= 1 && j < 5 && ISSUE) issue_one(st, kt + 2, n / 4 - 2);
+        if (j >= 5 && ISSUE) issue_one(st, kt + 2, NQA + n / 4 - 10);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (NEXT) take_scales();
+  };
+
+  // Pairs of steps take an even number: an odd last one goes first and by itself, through
+  // the last stage, as do the last K % 128 columns with zeros behind them.
+  const int odd = PAIRS ? KT & 1 : 0;
+  KT -= odd;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s)
-    if (s < KT) issue(s, s);
-  if (K % 128 != 0 && (!SPLIT || blockIdx.y + 1 == gridDim.y)) {
-    // the last K % 128 columns first, zeros behind them, through the last stage
-    typedef u64x2_t __attribute__((aligned(1))) u64x2_u;
-    const int kt0 = K / 128;
-    char* t = smem + (STAGES - 1) * STAGE;
+    if (s < KT) issue(s, s, LPW);
+  auto alone = [&](bool tail) __attribute__((always_inline)) {
+    const int kt0 = tail ? K / 128 : KT;
+    if (!tail) {
 #pragma unroll
-    for (int q = 0; q < NQA + NQB; ++q) {
-      const int c = q < NQA ? wave * NQA + q : b_copy(q - NQA), r = c * 8 + lane / 8;
-      const int chunk = dl_swz(r, lane % 8), k = kt0 * 128 + 16 * chunk;
-      const uint8_t* base = q < NQA ? A + ao[q] : (b_up(c * 8) ? B[1] : B[0]) + bo[q - NQA];
-      base -= 16 * chunk;  // the row's start
-      u64x2_t v;
-      if (K >= 16) {
-        v = shift_down(*(const u64x2_u*)(base + min(k, K - 16)), max(0, k - (K - 16)));
-      } else {
-        v = u64x2_t{};
-        for (int e = 0; e < 16; ++e)
-          if (k + e < K) v[e >> 3] |= (uint64_t)base[k + e] << (8 * (e & 7));
+      for (int q = 0; q < LPW; ++q) issue_one(STAGES - 1, KT, q);
+      wait_vmcnt<0>();
+    } else {
+      typedef u64x2_t __attribute__((aligned(1))) u64x2_u;
+      char* t = smem + (STAGES - 1) * STAGE;
+#pragma unroll
+      for (int q = 0; q < NQA + NQB; ++q) {
+        const int c = q < NQA ? wave * NQA + q : b_copy(q - NQA), r = c * 8 + lane / 8;
+        const int chunk = dl_swz(r, lane % 8), k = kt0 * 128 + 16 * chunk;
+        const uint8_t* base = q < NQA ? A + ao[q] : (b_up(c * 8) ? B[1] : B[0]) + bo[q - NQA];
+        base -= 16 * chunk;  // the row's start
+        u64x2_t v;
+        if (K >= 16) {
+          v = shift_down(*(const u64x2_u*)(base + min(k, K - 16)), max(0, k - (K - 16)));
+        } else {
+          v = u64x2_t{};
+          for (int e = 0; e < 16; ++e)
+            if (k + e < K) v[e >> 3] |= (uint64_t)base[k + e] << (8 * (e & 7));
+        }
+        *(u64x2_t*)(t + (q < NQA ? 0 : TA) + c * 1024 + lane * 16) = v;
       }
-      *(u64x2_t*)(t + (q < NQA ? 0 : TA) + c * 1024 + lane * 16) = v;
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -317,18 +372,26 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     if constexpr (GATE) sb[1] = p.w2.scales[block * p.w2.sld + kt0];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < FM; ++i) read_a(STAGES - 1, i);
+    for (int i = 0; i < FM; ++i) read_a(0, STAGES - 1, i, 0), read_a(0, STAGES - 1, i, 1);
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      read_b(STAGES - 1, j);
+      read_b(STAGES - 1, j, 0), read_b(STAGES - 1, j, 1);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) mfma_one(j, i);
+      for (int i = 0; i < FM; ++i) mfma_one(0, j, i);
     }
     __syncthreads();
+  };
+  const bool tail = K % 128 != 0 && (!SPLIT || blockIdx.y + 1 == gridDim.y);
+  if constexpr (PAIRS) {
+#pragma unroll 1
+    for (int t = 1 - odd; t < (tail ? 2 : 1); ++t) alone(t != 0);
+  } else {
+    if (tail) alone(true);
   }
-  if (STAGES - 1 < KT) issue(STAGES - 1, STAGES - 1);
+  constexpr int FIRST = PAIRS ? LPW - 2 : LPW;  // (the step before's copies of the last stage)
+  if (STAGES - 1 < KT) issue(STAGES - 1, STAGES - 1, FIRST);
   if (KT > 0) {
-    if (STAGES <= KT) wait_vmcnt<(STAGES - 1) * LPW>();
+    if (STAGES <= KT) wait_vmcnt<(STAGES - 2) * LPW + FIRST>();
     else wait_vmcnt<0>();
     __syncthreads();
     first_reads(0);
@@ -336,9 +399,16 @@ __global__ __launch_bounds__(C::NT, 2) void fp8_gemm_kernel(Fp8Gemm p) {
     auto next = [&]() __attribute__((always_inline)) { st = st + 1 == STAGES ? 0 : st + 1; };
     const std::true_type yes;
     const std::false_type no;
-    for (; kt < KT - STAGES; ++kt, next()) step(st, kt, yes, yes);
-    for (; kt < KT - 1; ++kt, next()) step(st, kt, no, yes);
-    step(st, kt, no, no);
+    if constexpr (PAIRS) {
+      const std::integral_constant<int, 0> one;
+      const std::integral_constant<int, 1> two;
+      for (; kt < KT - 2; kt += 2) pair_step(one, 0, kt, yes, yes), pair_step(two, 1, kt + 1, yes, yes);
+      pair_step(one, 0, kt, no, yes), pair_step(two, 1, kt + 1, no, no);
+    } else {
+      for (; kt < KT - STAGES; ++kt, next()) step(st, kt, yes, yes);
+      for (; kt < KT - 1; ++kt, next()) step(st, kt, no, yes);
+      step(st, kt, no, no);
+    }
   }
 
   const int mw = m0 + wm * TM;

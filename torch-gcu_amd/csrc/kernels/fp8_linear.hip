@@ -5,7 +5,7 @@
 namespace mi {
 namespace {
 
-typedef F8Cfg<4, 2, 64, 128, 2> F256;     // 256 x 256 (a gate's 128 gate and 128 up columns)
+typedef F8Cfg<2, 2, 128, 128, 2> F256;    // 256 x 256 (a gate's 128 gate and 128 up columns)
 typedef F8Cfg<4, 2, 64, 64, 3> F256x128;
 typedef F8Cfg<2, 2, 64, 64, 2> F128;
 typedef F8Cfg<2, 4, 32, 32, 3> F64x128;
