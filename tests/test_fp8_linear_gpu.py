@@ -291,7 +291,10 @@ def test_linear_is_exact_on_whole_numbers(m, n, k, ends):
 # whole, in two and in four)
 LARGE = [(4778, 2992, 1111), (1804, 7699, 640), (909, 8018, 1110), (1523, 5177, 256), (259, 6711, 1131),
          (4991, 407, 1152), (2456, 3229, 1102), (265, 6681, 128), (777, 4096, 512), (2655, 68, 4231),
-         (70, 3238, 4608), (25, 64, 7072), (42, 65, 4608), (65, 66, 64), (128, 4096, 1024)]
+         (70, 3238, 4608), (25, 64, 7072), (42, 65, 4608), (65, 66, 64), (128, 4096, 1024),
+         (2183, 6916, 768), (1922, 7104, 896), (4742, 3242, 700), (1935, 7097, 776), (4688, 838, 131),
+         (5979, 652, 265), (577, 6619, 393), (5784, 642, 514), (331, 6085, 133), (389, 4938, 257),
+         (352, 5695, 512), (3757, 514, 385), (2750, 781, 384)]
 
 
 @pytest.mark.parametrize("m,n,k", LARGE)
@@ -442,7 +445,8 @@ def test_linear_views_and_leading_dims():
     assert torch.equal(got.cpu(), (exact_product(x, w) + res.cpu().float()).to(BF16))
 
 
-@pytest.mark.parametrize("m,n,k", [(7, 200, 300), (40, 4096, 2048), (90, 500, 640), (300, 700, 256), (1500, 1100, 128)])
+@pytest.mark.parametrize("m,n,k", [(7, 200, 300), (40, 4096, 2048), (90, 500, 640), (300, 700, 256), (1500, 1100, 128),
+                                   (333, 640, 260), (1000, 6784, 128), (1922, 7104, 896)])
 def test_linear_in_place_and_untouched_surroundings(m, n, k):
     x, w = whole_numbers(m, n, k, 17)
     for left, pitch in ((8, n + 24), (3, n + 13)):
@@ -487,7 +491,9 @@ def small_gates(m, n, k, seed):
 
 
 GATES_LARGE = [(669, 8246, 1185), (3236, 2016, 640), (4869, 404, 1153), (470, 8372, 64), (4800, 137, 4545),
-               (81, 2404, 2193), (25, 69, 2528), (147, 207, 1137), (65, 70, 912), (17, 65, 305), (33, 67, 272)]
+               (81, 2404, 2193), (25, 69, 2528), (147, 207, 1137), (65, 70, 912), (17, 65, 305), (33, 67, 272),
+               (3765, 2118, 512), (980, 7194, 640), (5586, 1309, 386), (2188, 2971, 513), (2389, 1667, 128),
+               (2968, 1292, 133), (5729, 523, 519), (5959, 561, 395), (80, 4030, 2953), (696, 896, 5120)]
 
 
 def check_gate(got, gate, up, gate_off=0.0, up_off=0.0):

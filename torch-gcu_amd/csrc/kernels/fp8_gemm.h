@@ -428,23 +428,22 @@ __global__ __launch_bounds__(C::NT, C::PAIRS ? 1 : 2) void fp8_gemm_kernel(Fp8Ge
   __syncthreads();  // every wave is done with the stages
   if constexpr (EPI == F8_GATE) {
     uint32_t* most = (uint32_t*)(smem + BM * C::CP);  // [WN][BM]
-    if (n0 + BN / 2 > N) {  // columns past the end take no part in a maximum
+    float mine[FM] = {};
 #pragma unroll
-      for (int j = 0; j < FN / 2; ++j)
+    for (int j = 0; j < FN / 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n0 + wn * (TN / 2) + 16 * j + 4 * (lane >> 4) + e >= N)
+      for (int e = 0; e < 4; ++e) {
+        // (columns past the end take no part in a maximum)
+        const bool there = n0 + wn * (TN / 2) + 16 * j + 4 * (lane >> 4) + e < N;
 #pragma unroll
-            for (int i = 0; i < FM; ++i) acc[j][i][e] = acc[j + FN / 2][i][e] = 0.f;
-    }
+        for (int i = 0; i < FM; ++i) {
+          const float u = there ? acc[j + FN / 2][i][e] : 0.f, g = there ? acc[j][i][e] : 0.f;
+          acc[j][i][e] = gate_of(g, u, &mine[i]);
+        }
+      }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      float mine = 0.f;
-#pragma unroll
-      for (int j = 0; j < FN / 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][i][e] = gate_of(acc[j][i][e], acc[j + FN / 2][i][e], &mine);
-      uint32_t mx = __float_as_uint(mine);
+      uint32_t mx = __float_as_uint(mine[i]);
       mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16, 64));
       mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32, 64));
       if (lane < 16) most[wn * BM + wm * TM + 16 * i + row] = mx;

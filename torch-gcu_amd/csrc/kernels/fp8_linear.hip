@@ -5,12 +5,11 @@
 namespace mi {
 namespace {
 
-typedef F8Cfg<2, 2, 128, 128, 2> F256;    // 256 x 256 (a gate's 128 gate and 128 up columns)
-typedef F8Cfg<4, 2, 64, 64, 3> F256x128;
+typedef F8Cfg<2, 2, 128, 128, 2> F256;  // 256 x 256 (a gate's 128 gate and 128 up columns)
 typedef F8Cfg<2, 2, 64, 64, 2> F128;
-typedef F8Cfg<2, 4, 32, 32, 3> F64x128;
+typedef F8Cfg<2, 2, 32, 64, 2> F64x128;
 typedef F8Cfg<2, 2, 32, 32, 4> F64;
-typedef F8Cfg<2, 4, 64, 64, 2> G128;      // a gate's 128 x (128 and 128)
+typedef F8Cfg<2, 4, 64, 64, 2> G128;    // a gate's 128 x (128 and 128)
 typedef F8Cfg<2, 4, 32, 64, 2> G64;
 
 // out = the slices' sums in order (+ bias) (+ residual), 4 columns a thread
@@ -148,22 +147,23 @@ mi_status_t launch_few(Fp8Gemm q, hipStream_t s, const char* op) {
 // `steps` K steps of lo (few CUs busy) to hi (all busy) to hi2 (two blocks on each) us, or
 // the weight's stream at 5.6 TB/s; launch, first latency and epilogue; what every further
 // round adds; and for slices their sums through the caches.  The constants are a fit to
-// timings of these kernels (46 products and 24 gates, M 17 .. 7700, N 256 .. 16000, K 256
-// .. 10600): what they pick was within 1 % of the fastest of the shapes on average, 18 %
-// at worst.  Slices of the larger tiles were never the fastest.
+// timings of these kernels (111 products and 59 gates, M 17 .. 9000, N 256 .. 16000, K 256
+// .. 11008): what they pick was within 1 % of the fastest of the shapes on average, 7 % (a
+// gate 17 %) at worst.  Slices of the larger tiles were never the fastest; tiles of 256 x
+// 128, of 128 x 128 with eight waves and of 64 x 128 with eight are left out: with all of
+// them the fastest is 0.5 % faster.
 struct Shape {
   int bm, bn, per_cu;
   float fixed, lo, hi, hi2, round;
   int slices[3];
 };
-constexpr Shape kShapes[] = {{256, 256, 1, 10.1f, 1.53f, 1.74f, 0, 6.0f, {1}},
-                             {256, 128, 1, 6.3f, 0.89f, 0.89f, 0, 10.2f, {1}},
-                             {128, 128, 2, 6.2f, 0.39f, 0.60f, 0.97f, 3.4f, {1}},
-                             {64, 128, 2, 3.7f, 0.24f, 0.89f, 0.89f, 1.6f, {1}},
-                             {64, 64, 2, 3.1f, 0.195f, 0.286f, 0.63f, 5.6f, {1, 2, 4}}};
-constexpr Shape kGateShapes[] = {{256, 128, 1, 9.7f, 0.92f, 1.48f, 0, 5.6f, {1}},
-                                 {128, 128, 2, 5.7f, 0.70f, 1.10f, 2.4f, 0.f, {1, 2}},
-                                 {64, 128, 2, 4.0f, 0.46f, 0.94f, 1.9f, 5.2f, {1, 2, 4}}};
+constexpr Shape kShapes[] = {{256, 256, 1, 11.3f, 0.97f, 1.32f, 0, 8.0f, {1}},
+                             {128, 128, 2, 6.4f, 0.222f, 0.64f, 0.932f, 1.84f, {1}},
+                             {64, 128, 2, 4.05f, 0.18f, 0.59f, 0.741f, 2.39f, {1}},
+                             {64, 64, 2, 3.1f, 0.209f, 0.291f, 0.604f, 1.07f, {1, 2, 4}}};
+constexpr Shape kGateShapes[] = {{256, 128, 1, 8.3f, 0.975f, 1.063f, 0, 10.3f, {1}},
+                                 {128, 128, 2, 5.3f, 0.684f, 1.065f, 1.95f, 6.7f, {1}},
+                                 {64, 128, 2, 4.3f, 0.442f, 0.635f, 1.42f, 4.15f, {1, 2, 4}}};
 
 struct Pick {
   int shape, slices;
@@ -186,7 +186,7 @@ Pick pick_shape(const Fp8Gemm& q, const Shape (&shapes)[COUNT], int products, fl
       float t = full * steps * step((float)c.per_cu) + (rest > 0.f ? steps * step(rest) : 0.f);
       t = c.fixed + std::max(t, (float)q.N * (float)q.K * (float)products * (1.f / 5.6e6f)) +
           c.round * std::max(0.f, full - (rest > 0.f ? 0.f : 1.f));
-      if (s > 1) t += slice_fixed + (float)(s * products) * (float)q.M * (float)q.N * 2.2e-6f;
+      if (s > 1) t += slice_fixed + (float)(s * products) * (float)q.M * (float)q.N * 2.0e-6f;
       if (t < best.cost) best = Pick{i, s, t};
     }
   }
@@ -213,7 +213,7 @@ bool fits(const Fp8Gemm& q) {
 // 9.3, K11008 14.5 and 13.5).  Its blocks have 16 weight rows; 32 or 64 of them were no
 // faster anywhere.
 mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
-  const Pick c = pick_shape(q, kShapes, 1, 2.5f);
+  const Pick c = pick_shape(q, kShapes, 1, 2.6f);
   if (q.M <= kFewRows && (q.M <= 16 || few_cost(q, 1, 2.2f, 52e3f) <= c.cost)) {
     if (fits<R8Cfg<1, 1, 8, 2>>(q)) return launch_few<R8Cfg<1, 1, 8, 2>, false>(q, s, op);
     if (fits<R8Cfg<2, 1, 4, 3>>(q)) return launch_few<R8Cfg<2, 1, 4, 3>, false>(q, s, op);
@@ -224,9 +224,8 @@ mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
   }
   switch (c.shape) {
     case 0: return launch<F256, false>(q, s, op);
-    case 1: return launch<F256x128, false>(q, s, op);
-    case 2: return launch<F128, false>(q, s, op);
-    case 3: return launch<F64x128, false>(q, s, op);
+    case 1: return launch<F128, false>(q, s, op);
+    case 2: return launch<F64x128, false>(q, s, op);
     default: return launch_slices<F64, false>(q, c.slices, s, op);
   }
 }
@@ -234,7 +233,7 @@ mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
 // The same; the few-row kernel's two launches against one or two (M16 N32000 K4096 52 us and
 // 63 in 64-row tiles, M64 N11008 K4096 30 and 25.5).
 mi_status_t run_gate(const Fp8Gemm& q, hipStream_t s, const char* op) {
-  const Pick c = pick_shape(q, kGateShapes, 2, 2.2f);
+  const Pick c = pick_shape(q, kGateShapes, 2, 2.7f);
   if (q.M <= kFewRows && (q.M <= 16 || few_cost(q, 2, 4.8f, 42e3f) <= c.cost)) {
     if (fits<R8Cfg<1, 2, 4, 2>>(q)) return launch_few<R8Cfg<1, 2, 4, 2>, true>(q, s, op);
     if (fits<R8Cfg<2, 2, 4, 2>>(q)) return launch_few<R8Cfg<2, 2, 4, 2>, true>(q, s, op);
@@ -243,7 +242,7 @@ mi_status_t run_gate(const Fp8Gemm& q, hipStream_t s, const char* op) {
   }
   switch (c.shape) {
     case 0: return launch<F256, true>(q, s, op);
-    case 1: return launch_slices<G128, true>(q, c.slices, s, op);
+    case 1: return launch<G128, true>(q, s, op);
     default: return launch_slices<G64, true>(q, c.slices, s, op);
   }
 }
