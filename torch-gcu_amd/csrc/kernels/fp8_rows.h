@@ -1,5 +1,13 @@
 // The kernel of 8-bit floating point products with few rows of activations: the
 // linear layers of a decode step.
+//
+// The weight is read once, and what bounds it is that stream (and up to 4096 x 4096 a
+// launch, the first copies' latency and the waves' join): so a block has as few weight rows
+// as an instruction takes, 16, which gives many blocks, and its waves share the K instead,
+// each with its own copies in flight and no barrier between first and last.  The rows of
+// activations, which every block reads, come from the caches.  us a launch: M1 N4096 K4096
+// 5.0 (16.8 MB, 3.4 TB/s), M24 N4096 K11008 11.4 (4.0 TB/s), a gate of M8 N11008 K4096 16.5
+// (90 MB, 5.5 TB/s) and 3.5 for its codes' launch.
 #pragma once
 
 #include "fp8_gemm.h"
