@@ -633,6 +633,52 @@ def test_two_graphs_that_take_turns(m):
         assert same(outs[0], want[0]) and same(outs[1], want[1])
 
 
+@pytest.mark.parametrize("m", [5, 60, 300])
+def test_graph_of_calls_that_copy_their_rows(m):
+    """Codes that begin at odd bytes are copied to workspace inside the captured call."""
+    k, n = 517, 300
+    w = whole_numbers(1, n, k, 4)[1]
+    wide = torch.zeros(m, k + 40, dtype=U8, device="gcu")
+    rows = eff.FP8Rows(wide[:, 3: 3 + k], torch.full((m, 5), 127, dtype=U8, device="gcu"))
+    weight = gcu(w, eff.FP8Weight)
+
+    def calls():
+        y = eff.fp8_linear(rows, weight)
+        return (y, *eff.fp8_linear_silu_mul(rows, weight, weight))
+
+    def fill(seed):
+        code = whole_numbers(m, 1, k, seed)[0][0]
+        wide.copy_(torch.nn.functional.pad(code, (3, 37)).to("gcu"))
+
+    fill(1)
+    calls()
+    torch.gcu.synchronize()
+    g = torch.gcu.GCUGraph()
+    with torch.gcu.graph(g):
+        outs = calls()
+    for seed in range(2, 6):
+        fill(seed)
+        want = calls()
+        torch.gcu.synchronize()
+        g.replay()
+        torch.gcu.synchronize()
+        assert all(torch.equal(a.cpu(), b.cpu()) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("m", [1, 9, 70])
+def test_linear_of_the_most_columns(m):
+    """Longer rows than the few-row kernel has room for scales; offsets near 2^30 bytes."""
+    k, n = (1 << 22) - 16, 70
+    at = torch.cat([torch.randint(0, k, (500,), generator=gen(2)), torch.tensor([0, k - 1, k - 17])])
+    x, w = torch.zeros(m, k, dtype=U8), torch.zeros(n, k, dtype=U8)
+    xs, ws = whole_numbers(m, n, len(at), 5)
+    x[:, at], w[:, at] = xs[0], ws[0]
+    scale = lambda r: torch.full((r, -(-k // 128)), 127, dtype=U8)  # noqa: E731
+    got = eff.fp8_linear(gcu((x, scale(m))), gcu((w, scale(1)), eff.FP8Weight))
+    value = lambda t: t.view(torch.float8_e4m3fn).double()  # noqa: E731
+    assert torch.equal(got.cpu().double(), (value(x) @ value(w).t()).to(BF16).double())
+
+
 def test_two_streams_at_once():
     sets = [chain_inputs(24, 2048, 1500, s) for s in (1, 20)]
     want = [chain(*s) for s in sets]

@@ -314,7 +314,7 @@ __global__ __launch_bounds__(C::NT, C::PAIRS ? 1 : 2) void fp8_gemm_kernel(Fp8Ge
     if (NEXT) take_scales();
   };
 
-  // One K step of PAIRS, whose SET-th fragments hold its activations: 64 products, and
+  // One K step of PAIRS, with its activations in set NOW of the fragments: 64 products, and
   // between them, one at most, the halves of fragments and the copies that later steps
   // need.  (Two reads at a time cost 6 % of the cycles: one wave issues them all, and waits
   // where LDS is behind.)  The next step's activations are read in rows 1 to 4.  At row 5 a
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(C::NT, C::PAIRS ? 1 : 2) void fp8_gemm_kernel(Fp8Ge
   // activations in the next step.  So each copy has half a step or more until the barrier
   // that waits for it.
   auto pair_step = [&](auto set_c, int st, int kt, auto issue_c, auto next_c) __attribute__((always_inline)) {
-    constexpr int SET_ = decltype(set_c)::value;
+    constexpr int NOW = decltype(set_c)::value;
     constexpr bool ISSUE = decltype(issue_c)::value, NEXT = decltype(next_c)::value;
     const int nst = 1 - st;
     if (ISSUE && (kt + 2) % KS == 0) issue_scales((kt + 2) / KS);
@@ -340,8 +340,8 @@ __global__ __launch_bounds__(C::NT, C::PAIRS ? 1 : 2) void fp8_gemm_kernel(Fp8Ge
         if (j + RB - 1 < FN) read_b(st, j + RB - 1, i / 4);
         else if (NEXT) read_b(nst, j + RB - 1 - FN, i / 4);
       }
-      if (NEXT && j >= 1 && j < 5 && n % 2 == 1) read_a(1 - SET_, nst, n / 4 - 2, n / 2 % 2);
-      mfma_one(SET_, j, i);
+      if (NEXT && j >= 1 && j < 5 && n % 2 == 1) read_a(1 - NOW, nst, n / 4 - 2, n / 2 % 2);
+      mfma_one(NOW, j, i);
       if (n % 4 == 2) {
         if (n < FM && NEXT) issue_one(nst, kt + 1, NQA + 6 + n / 4);
         if (j >= 1 && j < 5 && ISSUE) issue_one(st, kt + 2, n / 4 - 2);

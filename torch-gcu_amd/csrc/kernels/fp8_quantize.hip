@@ -206,7 +206,9 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   }
 }
 
-// A block of 512 threads to a 128 x 128 block of the weight, 4 rows a thread.
+// A block of 512 threads to a 128 x 128 block of the weight, 4 rows a thread: bf16 11008 x
+// 4096 26 us (135 MB, 5.2 TB/s), f32 1000 x 1500 5.3 (in 256 threads, with loads behind
+// conditions, 31 and 12.8).
 template <typename T>
 __global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t ld, int64_t rows, int cols,
                                                          Fp8Mat out) {
