@@ -397,6 +397,8 @@ mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const
       MI_CHECK_ARG(ts[i]->dtype == x->dtype && ts[i]->sizes[0] == x->sizes[0] &&
                        ts[i]->sizes[1] == x->sizes[1],
                    "%s: %s must have x's shape and type", op, names[i]);
+    }
+    for (int i = 0; i < 2; ++i) {
       MI_RETURN_IF(check_outputs_apart(op, out, names[i], ts[i]));
       // total may be the same tensor as an input: a thread reads what it writes
       const mi_tensor_t* in = i == 0 ? x : residual;
