@@ -181,7 +181,8 @@ def _forward_cached_fp8(weights, ids, cfg, cache, block_table, lengths, starts, 
     T, H, D = ids.shape[0], cfg.heads, cfg.head_dim
     x = F.embedding(ids, weights["embed"])
     h, _ = eff.rms_norm_fp8(x, weights["attn_norm"], cfg.eps)
-    q, k, v = (eff.fp8_linear(h, weights[n], dtype=x.dtype).view(T, -1, D) for n in ("wq", "wk", "wv"))
+    q, k, v = (eff.fp8_linear(h, w, dtype=x.dtype).view(T, w.codes.shape[0] // D, D)
+               for w in (weights["wq"], weights["wk"], weights["wv"]))
     _rope_(q, k, pos, cfg.theta)
     eff.kv8_append(k, v, cache, block_table, lengths, starts)
     a, lse = eff.kv8_attention(q, cache, block_table, lengths, starts)
