@@ -138,90 +138,44 @@ mi_status_t launch_few(Fp8Gemm q, hipStream_t s, const char* op) {
     q.part = (float*)ws.get();
   }
   hipLaunchKernelGGL((fp8_rows_gemm_kernel<C, GATE>), dim3(ceil_div_u(q.N, COLS)), dim3(64 * C::NW),
-                     C::lds((size_t)fp8_groups(q.K)), s, q);
+                     C::F.lds((size_t)fp8_groups(q.K)), s, q);
   MI_RETURN_IF(check_launch(op));
   return GATE ? fp8_quantize_f32(q.part, q.ldp, q.M, q.N, q.codes, s, op) : MI_OK;
 }
 
-// Tile shapes and slices of K by a cost in us: rounds of `per_cu` blocks a CU, each of
-// `steps` K steps of lo (few CUs busy) to hi (all busy) to hi2 (two blocks on each) us, or
-// the weight's stream at 5.6 TB/s; launch, first latency and epilogue; what every further
-// round adds; and for slices their sums through the caches.  The constants are a fit to
-// timings of these kernels (111 products and 59 gates, M 17 .. 9000, N 256 .. 16000, K 256
-// .. 11008): what they pick was within 1 % of the fastest of the shapes on average, 7 % (a
-// gate 17 %) at worst.  Slices of the larger tiles were never the fastest; tiles of 256 x
-// 128, of 128 x 128 with eight waves and of 64 x 128 with eight are left out: with all of
-// them the fastest is 0.5 % faster.
-struct Shape {
-  int bm, bn, per_cu;
-  float fixed, lo, hi, hi2, round;
-  int slices[3];
-};
-constexpr Shape kShapes[] = {{256, 256, 1, 11.3f, 0.97f, 1.32f, 0, 8.0f, {1}},
-                             {128, 128, 2, 6.4f, 0.222f, 0.64f, 0.932f, 1.84f, {1}},
-                             {64, 128, 2, 4.05f, 0.18f, 0.59f, 0.741f, 2.39f, {1}},
-                             {64, 64, 2, 3.1f, 0.209f, 0.291f, 0.604f, 1.07f, {1, 2, 4}}};
-constexpr Shape kGateShapes[] = {{256, 128, 1, 8.3f, 0.975f, 1.063f, 0, 10.3f, {1}},
-                                 {128, 128, 2, 5.3f, 0.684f, 1.065f, 1.95f, 6.7f, {1}},
-                                 {64, 128, 2, 4.3f, 0.442f, 0.635f, 1.42f, 4.15f, {1, 2, 4}}};
+template <class C, bool GATE>
+constexpr bool is_shape(const Fp8Shape& s) {
+  return s.bm == C::BM && s.bn == (GATE ? C::BN / 2 : C::BN) &&
+         (s.per_cu == (int)(kFp8Lds / C::LDS_BYTES) || (s.per_cu == 2 && C::LDS_BYTES * 2 <= kFp8Lds));
+}
+static_assert(is_shape<F256, false>(kFp8Shapes[0]) && is_shape<F128, false>(kFp8Shapes[1]) &&
+                  is_shape<F64x128, false>(kFp8Shapes[2]) && is_shape<F64, false>(kFp8Shapes[3]) &&
+                  is_shape<F256, true>(kFp8GateShapes[0]) && is_shape<G128, true>(kFp8GateShapes[1]) &&
+                  is_shape<G64, true>(kFp8GateShapes[2]),
+              "the rule's shapes are the kernels', with no more blocks a CU than its LDS holds");
 
-struct Pick {
-  int shape, slices;
-  float cost;
-};
-
-template <int COUNT>
-Pick pick_shape(const Fp8Gemm& q, const Shape (&shapes)[COUNT], int products, float slice_fixed) {
-  const float cus = (float)cu_count();
-  const int64_t ksteps = ((int64_t)q.K + 127) / 128;
-  Pick best{0, 1, 3e38f};
-  for (int i = 0; i < COUNT; ++i) {
-    const Shape& c = shapes[i];
-    const int64_t tiles = (((int64_t)q.M + c.bm - 1) / c.bm) * (((int64_t)q.N + c.bn - 1) / c.bn);
-    for (int s : c.slices) {
-      if (s == 0 || (s > 1 && ksteps < 2 * s)) break;
-      const float steps = (float)((ksteps + s - 1) / s), load = (float)(tiles * s) / cus;
-      auto step = [&](float l) { return l <= 1.f ? c.lo + (c.hi - c.lo) * l : c.hi + (c.hi2 - c.hi) * (l - 1.f); };
-      const float full = std::floor(load / (float)c.per_cu), rest = load - full * (float)c.per_cu;
-      float t = full * steps * step((float)c.per_cu) + (rest > 0.f ? steps * step(rest) : 0.f);
-      t = c.fixed + std::max(t, (float)q.N * (float)q.K * (float)products * (1.f / 5.6e6f)) +
-          c.round * std::max(0.f, full - (rest > 0.f ? 0.f : 1.f));
-      if (s > 1) t += slice_fixed + (float)(s * products) * (float)q.M * (float)q.N * 2.0e-6f;
-      if (t < best.cost) best = Pick{i, s, t};
-    }
-  }
-  return best;
+// Up to 16 rows: no more columns than a few-row kernel's grid holds, whichever way is taken.
+mi_status_t check_columns(const Fp8Gemm& q, const Fp8Few& f, const char* op) {
+  return q.M <= 16 ? check_grid(((int64_t)q.N + 15) / 16, 64 * f.nw, op) : MI_OK;
 }
 
-// The few-row kernels' cost: the weight's stream, or what the busiest CU takes in (its
-// blocks' 16 (a gate's 32) weight rows and all rows of x, at `rate` bytes a us).
-float few_cost(const Fp8Gemm& q, int products, float fixed, float rate) {
-  const float blocks = (float)(((int64_t)q.N + 15) / 16) / (float)cu_count();
-  const float bytes = (float)(16 * products + (q.M + 7) / 8 * 8) * (float)q.K;
-  return fixed + std::max((float)q.N * (float)q.K * (float)products * (1.f / 5.5e6f),
-                          std::max(1.f, blocks) * bytes / rate);
+template <int I = 0>
+mi_status_t run_few(int i, const Fp8Gemm& q, hipStream_t s, const char* op) {
+  if constexpr (I < (int)(sizeof(kFp8Few) / sizeof(kFp8Few[0])))
+    return i == I ? launch_few<R8Cfg<kFp8Few, I>, false>(q, s, op) : run_few<I + 1>(i, q, s, op);
+  MI_FAIL(MI_ERR_INVALID, "%s: no such kernel", op);
+}
+template <int I = 0>
+mi_status_t run_gate_few(int i, const Fp8Gemm& q, hipStream_t s, const char* op) {
+  if constexpr (I < (int)(sizeof(kFp8GateFew) / sizeof(kFp8GateFew[0])))
+    return i == I ? launch_few<R8Cfg<kFp8GateFew, I>, true>(q, s, op) : run_gate_few<I + 1>(i, q, s, op);
+  MI_FAIL(MI_ERR_INVALID, "%s: no such kernel", op);
 }
 
-constexpr int kFewRows = 64;
-template <class C>
-bool fits(const Fp8Gemm& q) {
-  return q.M <= 8 * C::XR && C::lds((size_t)fp8_groups(q.K)) <= 160 * 1024;
-}
-
-// Up to 16 rows the few-row kernel (M8 N4096 K4096 5.3 us, in 64 x 64 tiles cut in four
-// 8.5; M16 N32000 K4096 28 and 32), up to 64 whichever costs less (M48 N4096 K4096 7.5 and
-// 9.3, K11008 14.5 and 13.5).  Its blocks have 16 weight rows; 32 or 64 of them were no
-// faster anywhere.
 mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
-  const Pick c = pick_shape(q, kShapes, 1, 2.6f);
-  if (q.M <= kFewRows && (q.M <= 16 || few_cost(q, 1, 2.2f, 52e3f) <= c.cost)) {
-    if (fits<R8Cfg<1, 1, 8, 2>>(q)) return launch_few<R8Cfg<1, 1, 8, 2>, false>(q, s, op);
-    if (fits<R8Cfg<2, 1, 4, 3>>(q)) return launch_few<R8Cfg<2, 1, 4, 3>, false>(q, s, op);
-    if (fits<R8Cfg<3, 1, 8, 2>>(q)) return launch_few<R8Cfg<3, 1, 8, 2>, false>(q, s, op);
-    if (fits<R8Cfg<4, 1, 4, 2>>(q)) return launch_few<R8Cfg<4, 1, 4, 2>, false>(q, s, op);
-    if (fits<R8Cfg<6, 1, 4, 2>>(q)) return launch_few<R8Cfg<6, 1, 4, 2>, false>(q, s, op);
-    if (fits<R8Cfg<8, 1, 4, 2>>(q)) return launch_few<R8Cfg<8, 1, 4, 2>, false>(q, s, op);
-  }
+  MI_RETURN_IF(check_columns(q, kFp8Few[0], op));
+  const Fp8Way c = fp8_pick_linear(q.M, q.N, q.K, cu_count());
+  if (c.few >= 0) return run_few(c.few, q, s, op);
   switch (c.shape) {
     case 0: return launch<F256, false>(q, s, op);
     case 1: return launch<F128, false>(q, s, op);
@@ -230,16 +184,10 @@ mi_status_t run_linear(const Fp8Gemm& q, hipStream_t s, const char* op) {
   }
 }
 
-// The same; the few-row kernel's two launches against one or two (M16 N32000 K4096 52 us and
-// 63 in 64-row tiles, M64 N11008 K4096 30 and 25.5).
 mi_status_t run_gate(const Fp8Gemm& q, hipStream_t s, const char* op) {
-  const Pick c = pick_shape(q, kGateShapes, 2, 2.7f);
-  if (q.M <= kFewRows && (q.M <= 16 || few_cost(q, 2, 4.8f, 42e3f) <= c.cost)) {
-    if (fits<R8Cfg<1, 2, 4, 2>>(q)) return launch_few<R8Cfg<1, 2, 4, 2>, true>(q, s, op);
-    if (fits<R8Cfg<2, 2, 4, 2>>(q)) return launch_few<R8Cfg<2, 2, 4, 2>, true>(q, s, op);
-    if (fits<R8Cfg<4, 2, 4, 2>>(q)) return launch_few<R8Cfg<4, 2, 4, 2>, true>(q, s, op);
-    if (fits<R8Cfg<8, 2, 4, 2>>(q)) return launch_few<R8Cfg<8, 2, 4, 2>, true>(q, s, op);
-  }
+  MI_RETURN_IF(check_columns(q, kFp8GateFew[0], op));
+  const Fp8Way c = fp8_pick_gate(q.M, q.N, q.K, cu_count());
+  if (c.few >= 0) return run_gate_few(c.few, q, s, op);
   switch (c.shape) {
     case 0: return launch<F256, true>(q, s, op);
     case 1: return launch<G128, true>(q, s, op);

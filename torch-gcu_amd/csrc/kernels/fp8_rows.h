@@ -11,24 +11,21 @@
 #pragma once
 
 #include "fp8_gemm.h"
+#include "fp8_rule.h"
 
 namespace mi {
 namespace {
 
 // XR x 8 rows of activations (M <= 8 XR), RT tiles of 16 weight rows a block, whose NW
-// waves take units of 128 of K in turn, each through a ring of D of its own.
-template <int XR_, int RT_, int NW_, int D_>
+// waves take units of 128 of K in turn, each through a ring of D of its own: WAYS[I] of the
+// rule's.
+template <const Fp8Few* WAYS, int I>
 struct R8Cfg {
-  static constexpr int XR = XR_, RT = RT_, NW = NW_, D = D_;
+  static constexpr Fp8Few F = WAYS[I];
+  static constexpr int XR = F.xr, RT = F.rt, NW = F.nw, D = F.d;
   static constexpr int MT = (XR + 1) / 2;                 // tiles of 16 activation rows
-  static constexpr int LPU = 2 * RT + XR;                 // 1 KiB copies a unit
-  static constexpr int UNIT = LPU * 1024, RING = NW * D * UNIT;
-  static constexpr int RED = NW * RT * MT * 1024;         // partial tiles
-  static constexpr int BODY = RING > RED ? RING : RED;
-  // and the scales of n groups, whole waves of them
-  static constexpr size_t lds(size_t n) {
-    return BODY + (8 * XR * n + 63) / 64 * 256 + 2 * ((n + 63) / 64 * 256);
-  }
+  static constexpr int LPU = F.copies();                  // 1 KiB copies a unit
+  static constexpr int UNIT = LPU * 1024, BODY = F.body();
   static_assert(D >= 2 && LPU * (D - 1) < 64, "copies in flight are counted in 6 bits");
 };
 
