@@ -213,3 +213,9 @@ def test_every_way_has_sizes_that_go_it(tmp_path):
              for way, sizes in ways.items() for size in sizes]
     for size, way in zip(named, picks(tmp_path, [n[:4] for n in named])):
         assert way == size[4], size
+
+
+def test_more_columns_than_small_tiles_have_a_grid_for(tmp_path):
+    """Go to the largest tiles."""
+    sizes = [(op, m, 1 << 30, 16) for op in ("linear", "gate") for m in (17, 64, 65)]
+    assert picks(tmp_path, sizes) == [("tile", 0, 1)] * 6

@@ -64,6 +64,8 @@ constexpr Fp8Few kFp8Few[] = {{1, 1, 8, 2}, {2, 1, 4, 3}, {3, 1, 8, 2}, {4, 1, 4
 constexpr Fp8Few kFp8GateFew[] = {{1, 2, 4, 2}, {2, 2, 4, 2}, {4, 2, 4, 2}, {8, 2, 4, 2}};
 
 constexpr size_t kFp8Lds = 160 * 1024;
+// Blocks of up to 512 threads that a grid's first dimension holds.
+constexpr int64_t kFp8Blocks = ((int64_t)1 << 23) - 1;
 
 // A few-row kernel (index, or -1), or a tile shape and its slices of K.
 struct Fp8Way {
@@ -90,6 +92,7 @@ Fp8Way fp8_pick(int M, int N, int K, int cus, const Fp8Shape (&shapes)[SHAPES], 
   for (int i = 0; i < SHAPES; ++i) {
     const Fp8Shape& c = shapes[i];
     const int64_t across = ((int64_t)N + c.bn - 1) / c.bn, tiles = ((int64_t)M + c.bm - 1) / c.bm * across;
+    if (i > 0 && tiles > kFp8Blocks) continue;
     for (int s : c.slices) {
       if (s == 0 || (s > 1 && groups < 2 * s)) break;
       const float steps = (float)((groups + s - 1) / s), per_cu = (float)c.per_cu;
@@ -105,8 +108,9 @@ Fp8Way fp8_pick(int M, int N, int K, int cus, const Fp8Shape (&shapes)[SHAPES], 
   for (int i = 0; i < FEWS; ++i) {
     const Fp8Few& f = fews[i];
     const size_t lds = f.lds((size_t)groups);
-    if (M > 8 * f.xr || lds > kFp8Lds) continue;
-    const float blocks = (float)(((int64_t)N + 15) / 16) / (float)cus, per_cu = (float)(kFp8Lds / lds);
+    const int64_t columns = ((int64_t)N + 15) / 16;
+    if (M > 8 * f.xr || lds > kFp8Lds || columns > kFp8Blocks) continue;
+    const float blocks = (float)columns / (float)cus, per_cu = (float)(kFp8Lds / lds);
     const float full = std::floor(blocks / per_cu), rest = blocks - full * per_cu;
     const float block = (float)(16 * fit.products + (M + 7) / 8 * 8) * (float)K;
     const float busiest = (full * per_cu + (rest > 0.f ? std::max(1.f, rest) : 0.f)) * block;
