@@ -615,7 +615,7 @@ mi_status_t mi_rms_norm_fp8(const mi_fp8_t* out, const mi_tensor_t* total, const
  * float32, residual of out's type, which may be out itself.  The products go
  * through the scaled e4m3 matrix instructions and add up in fp32; one instruction
  * adds 8 neighbours of K at a time with 13 bits below the largest of them, which
- * is off by 1.5e-5 of a sum of normal numbers, a sixth of f16's rounding.  Rows of
+ * is off by 1.5e-5 of a sum of normal numbers, a thirteenth of f16's rounding.  Rows of
  * codes that are not 16-byte aligned are copied to workspace first; K is cut in
  * slices, added in a fixed order, where tiles are few. */
 mi_status_t mi_fp8_linear(const mi_tensor_t* out, const mi_fp8_t* x, const mi_fp8_t* weight,

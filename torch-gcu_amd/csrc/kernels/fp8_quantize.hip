@@ -207,8 +207,8 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
 }
 
 // A block of 512 threads to a 128 x 128 block of the weight, 4 rows a thread: bf16 11008 x
-// 4096 26 us (135 MB, 5.2 TB/s), f32 1000 x 1500 5.3 (in 256 threads, with loads behind
-// conditions, 31 and 12.8).
+// 4096 23.7 us (135 MB, 5.7 TB/s, a part of it from the last-level cache), f32 1000 x 1500 4.9
+// (in 256 threads, with loads behind conditions, 31 and 12.8).
 template <typename T>
 __global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t ld, int64_t rows, int cols,
                                                          Fp8Mat out) {
@@ -260,9 +260,9 @@ __global__ __launch_bounds__(512) void fp8_weight_kernel(const void* w, int64_t 
   if (threadIdx.x == 0) out.scales[blockIdx.y * out.sld + blockIdx.x] = (uint8_t)byte;
 }
 
-// A wave to 512 columns.  us (bytes moved): f16 rows of 11008 out of 22016, 6011 of them, 40.0
-// (198 MB, 5.0 TB/s), with 2048 columns a wave 44.2, with a block to a row 55.7; bf16
-// 8192 x 4096 21.6, 24.8, 19.8; one row of 4096 2.7, 2.9, 2.9 (launch 2.1).
+// A wave to 512 columns: f16 rows of 11008 out of 22016, 6011 of them, 37.4 us (198 MB, 5.3
+// TB/s), with 2048 columns a wave 10 % more, with a block to a row 39 %; bf16 8192 x 4096 with
+// these 15 % more and 8 % less; one row of 4096 2.0 us, 7 % more with either.
 template <typename T>
 mi_status_t launch_quantize(const RowsArgs& a, hipStream_t s, const char* op) {
   const int64_t chunks = (a.cols + 511) / 512;
